@@ -37,7 +37,8 @@
 extern "C" {
 #endif
 
-typedef enum { SAE_F32 = 0, SAE_BF16 = 1 } sae_dtype;
+/* SAE_ROWS8: rows held in 8 bits ("Rows held in 8 bits" below); taken where a declaration says so. */
+typedef enum { SAE_F32 = 0, SAE_BF16 = 1, SAE_ROWS8 = 2 } sae_dtype;
 
 enum {
   SAE_OK = 0,
@@ -318,7 +319,8 @@ int sae_build_feature_index(const int32_t *idx, const int64_t *row_off, const in
 
 /* out[f, :] = sum_{s in segment f} coef[s] * dense[slot_tok[s], :]   for every f in [0, F)
  * (rows with an empty segment are written as zeros, so `out` needs no prior clearing);
- * optionally bias_out[f] = sum coef[s].  dense [B, d] in dense_dtype, out [F, d] fp32.
+ * optionally bias_out[f] = sum coef[s].  dense [B, d] in dense_dtype (SAE_F32, SAE_BF16 or SAE_ROWS8), out [F, d]
+ * fp32.  d a multiple of 4 (any d for SAE_ROWS8).
  * With coef = val and dense = grad_recon this is dW_D; with coef = d(pre) and dense = x it
  * is dW_E^T and bias_out = db_E.
  * Replaces the sorted atomic-add SpMM (kernels/kernels.py:137-225) and the dense
@@ -348,7 +350,7 @@ int sae_adam_step(float *p, const void *g, int g_dtype, float *m, float *v, int6
 
 /* Adam on a feature-major weight matrix [F, d] whose gradient is given in factored form:
  *   g[f, :] = sum_{s in segment f of the feature index} coef[s] * dense[slot_tok[s], :]
- * (the quantity sae_sparse_grad_rows would write).  The row gradient is formed in registers and
+ * (the quantity sae_sparse_grad_rows would write; dense in SAE_F32, SAE_BF16 or SAE_ROWS8).  The row gradient is formed in registers and
  * consumed at once; no dense gradient is stored.  Same update rule, scalars and by-products
  * (shadow_bf16, row_norm_out) as sae_adam_step; bias_grad_out (nullable) receives
  * sum_{s in segment f} coef[s], the gradient of the per-feature bias.  Bit-identical to
@@ -488,6 +490,36 @@ int sae_dense_to_code(const void *dense, int dtype, int64_t B, int64_t F, const 
  * entry in [0, n_src_rows) (an entry outside leaves its output row untouched). */
 int sae_gather_rows(const void *src, int src_dtype, const int64_t *row_idx, int64_t n_src_rows, int64_t n_rows,
                     int64_t d, void *dst, int dst_dtype, double scale, void *stream);
+
+/* ---- Rows held in 8 bits ----------------------------------------------------------------------------------
+ * A row of d values as one record of sae_rows8_pitch(d) bytes, blocks = ceil(d / 32):
+ *   int8  code[32 * blocks]   zeros behind the d-th
+ *   uint8 field[blocks]       value[j] = code[j] * step, step = 2^(field[j / 32] - 127); 0: a block of zeros; 255: the block
+ *                             held an infinity or a NaN, and every value of it reads as NaN
+ *   zeros up to a multiple of 16 bytes
+ * The step is the smallest power of two (not below 2^-126) that brings the block's largest magnitude to 127 or less after
+ * rounding to nearest, ties to even: between 1/127.5 and 1/63.75 of that magnitude.  A value is off by at most half a step;
+ * within 0.4 % of the largest float, where no larger step is left, codes stop at 127 and it is off by at most one.
+ * Every value is exact in bf16, and writing values that were read gives the same values.
+ * No counterpart in the reference, which keeps activations, cached or saved for the backward pass, in float rows.
+ * Buffers of records are 16-byte aligned. */
+int64_t sae_rows8_pitch(int64_t d);
+
+/* rows[i] = record of src[i, :], i < n.  src: SAE_F32 or SAE_BF16, row i at element i * src_stride (unit stride inside a
+ * row).  bf16_copy (nullable): bf16 [n, d], the rounded source itself, what a bf16 product reads, from the same pass. */
+int sae_rows8_quantize(const void *src, int src_dtype, int64_t n, int64_t d, int64_t src_stride, void *rows, void *bf16_copy,
+                       void *stream);
+
+/* dst[i, :] = cast(scale * values of record row_idx[i]), i < n_rows; row_idx: device int64 or NULL (record i).  dst [n_rows, d]
+ * in SAE_F32 or SAE_BF16.  An index outside [0, n_src_rows) reads nothing and gives a row of NaN. */
+int sae_rows8_gather(const void *rows, const int64_t *row_idx, int64_t n_src_rows, int64_t n_rows, int64_t d, void *dst,
+                     int dst_dtype, double scale, void *stream);
+
+/* dst[c, r] = src[r, c] for r < rows and 0 for rows <= r < dst_pitch: an operand whose token axis has become the contiguous
+ * one, filled up to the contraction lengths the GEMM entry points take.  src [rows, cols] in SAE_F32, SAE_BF16 or SAE_ROWS8
+ * (records of cols values), dst [cols, dst_pitch] in SAE_F32 or SAE_BF16 (fp32 to bf16 rounds to nearest even). */
+int sae_transpose_padded(const void *src, int src_dtype, int64_t rows, int64_t cols, void *dst, int dst_dtype, int64_t dst_pitch,
+                         void *stream);
 
 /* ---- Training metrics from the sparse code ----------------------------------------------------------
  * The per-step quantities behind FrequencyMetric, MeanFeatureActMetric and L0Metric (metrics.py:102-127,

@@ -5,9 +5,9 @@ The directory name is not a Python identifier; load it under the alias `lm_saes_
 """
 
 from . import _lib, ops  # noqa: F401
-from .ops import FeatureIndex, SparseCode  # noqa: F401
+from .ops import FeatureIndex, Rows8, SparseCode  # noqa: F401
 
-__all__ = ["_lib", "ops", "SparseCode", "FeatureIndex"]
+__all__ = ["_lib", "ops", "SparseCode", "FeatureIndex", "Rows8"]
 
 from .config import SAEConfig, SparseDictionaryConfig  # noqa: E402,F401
 from .activation_functions import JumpReLU  # noqa: E402,F401

@@ -14,7 +14,7 @@ from ctypes import c_char_p, c_double, c_int, c_int64, c_void_p
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libsae_hip.so")
 
-SAE_F32, SAE_BF16 = 0, 1
+SAE_F32, SAE_BF16, SAE_ROWS8 = 0, 1, 2
 
 # name -> (restype, argtypes); mirrors include/sae_hip.h declaration by declaration
 _P, _I, _L, _F = c_void_p, c_int, c_int64, c_double
@@ -57,6 +57,10 @@ SIGNATURES = {
     "sae_adam_step_lowp": (_I, [_P, _P, _I, _P, _P, _L, _F, _F, _F, _F, _L, _P, _L, _P, _P]),
     "sae_adam_step_sparse_rows_lowp": (_I, [_P, _P, _P, _P, _P, _I, _P, _P, _P, _L, _L, _F, _F, _F, _F, _L, _P, _P, _P, _P, _P, _L, _P, _P, _P, _P]),
     "sae_gather_rows": (_I, [_P, _I, _P, _L, _L, _L, _P, _I, _F, _P]),
+    "sae_rows8_pitch": (_L, [_L]),
+    "sae_rows8_quantize": (_I, [_P, _I, _L, _L, _L, _P, _P, _P]),
+    "sae_rows8_gather": (_I, [_P, _P, _L, _L, _L, _P, _I, _F, _P]),
+    "sae_transpose_padded": (_I, [_P, _I, _L, _L, _P, _I, _L, _P]),
     "sae_transpose_to_bf16": (_I, [_P, _I, _P, _L, _L, _P, _P, _P]),
     "sae_code_to_dense": (_I, [_P, _P, _P, _P, _L, _L, _P, _P, _P]),
     "sae_code_to_dense_t": (_I, [_P, _P, _P, _P, _L, _L, _P, _P]),

@@ -284,7 +284,7 @@ __global__ void sq_nnz_finish_kernel(const double *__restrict__ partial, int64_t
 // NT threads: 256, or fewer for rows whose pieces do not fill four waves (a row of 768 elements has 192 pieces: a fourth
 // wave would hold a place on its SIMD and do nothing but help staging; a wave that owns no piece adds nothing to any sum,
 // so the results are the same bits)
-template <bool DENSE_BF16, int U, int NT = 256>
+template <int DENSE, int U, int NT = 256>
 __global__ __launch_bounds__(NT) void adam_sparse_rows_kernel(
     const int32_t *__restrict__ feat_ptr, const int32_t *__restrict__ feat_slot,
     const int32_t *__restrict__ slot_tok, const float *__restrict__ coef, const void *__restrict__ dense,
@@ -303,7 +303,7 @@ __global__ __launch_bounds__(NT) void adam_sparse_rows_kernel(
   const int xo = extra_map ? extra_map[f] : -1;   // row of the dense gradient block that adds to this feature, or -1
   const int lo = feat_ptr[f], hi = feat_ptr[f + 1];
   const int n_seg = d >> 2;
-  const size_t row_bytes = (size_t)d * (DENSE_BF16 ? 2 : 4);
+  const size_t row_bytes = dense_row_bytes<DENSE>(d);
   const char *dbase = reinterpret_cast<const char *>(dense);
   const int64_t base4 = (int64_t)f * n_seg;
 
@@ -335,7 +335,7 @@ __global__ __launch_bounds__(NT) void adam_sparse_rows_kernel(
       g[u] = (xo >= 0 && seg < n_seg) ? reinterpret_cast<const float4 *>(extra_rows)[(int64_t)xo * n_seg + seg]
                                       : make_float4(0.f, 0.f, 0.f, 0.f);
     }
-    gather_rows_staged<DENSE_BF16, NT, U>(g, lo, hi, feat_slot, slot_tok, coef, dbase, row_bytes, seg0, n_seg, s_coef, s_tok);
+    gather_rows_staged<DENSE, NT, U>(g, lo, hi, feat_slot, slot_tok, coef, dbase, row_bytes, seg0, n_seg, s_coef, s_tok);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int seg = seg0 + u * NT;
@@ -403,7 +403,7 @@ namespace sae {
 // tests) this form is slower than a workgroup per row, 2.86 against 2.51 ms at the headline shape and 6.3 against
 // 4.9 ms over a cross-layer transcoder's rows of 768, whatever the grid: it is not dispatched.  Five waves per SIMD are asked for: at 98 registers (104 allocated) only four fit,
 // and the pass falls from 1.46 to 1.69 ms.
-template <bool DENSE_BF16, int U, bool S_BF16>
+template <int DENSE, int U, bool S_BF16>
 __global__ __launch_bounds__(256, 5) void adam_sparse_rows_persistent_kernel(
     const int32_t *__restrict__ feat_ptr, const int32_t *__restrict__ feat_slot,
     const int32_t *__restrict__ slot_tok, const float *__restrict__ coef, const void *__restrict__ dense,
@@ -419,7 +419,7 @@ __global__ __launch_bounds__(256, 5) void adam_sparse_rows_persistent_kernel(
   const float gs = grad_scale ? grad_scale[0] : 1.f;
   const int n_seg = d >> 2;
   const int passes = (n_seg + 256 * U - 1) / (256 * U);
-  const size_t row_bytes = (size_t)d * (DENSE_BF16 ? 2 : 4);
+  const size_t row_bytes = dense_row_bytes<DENSE>(d);
   const char *dbase = reinterpret_cast<const char *>(dense);
   typedef typename std::conditional<S_BF16, nt_u32x2, nt_f32x4>::type raw_t;   // four elements as they lie in memory
   struct Raw { raw_t p[U], m[U], v[U]; };
@@ -470,7 +470,7 @@ __global__ __launch_bounds__(256, 5) void adam_sparse_rows_persistent_kernel(
         g[u] = (xo >= 0 && seg < n_seg) ? reinterpret_cast<const float4 *>(extra_rows)[(int64_t)xo * n_seg + seg]
                                         : make_float4(0.f, 0.f, 0.f, 0.f);
       }
-      gather_rows_staged<DENSE_BF16, 256, U>(g, lo, hi, feat_slot, slot_tok, coef, dbase, row_bytes, seg0, n_seg, s_coef, s_tok);
+      gather_rows_staged<DENSE, 256, U>(g, lo, hi, feat_slot, slot_tok, coef, dbase, row_bytes, seg0, n_seg, s_coef, s_tok);
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         const int seg = seg0 + u * 256;
@@ -544,7 +544,7 @@ static int adam_step_sparse_rows_impl(bool lowp, const int32_t *feat_ptr, const 
               SAE_ERR_WORKSPACE, "adam_step_sparse_rows: the gradient sums need an aligned workspace of %lld bytes",
               (long long)(16 * F));
   SAE_REQUIRE(F > 0 && d > 0 && step >= 1, SAE_ERR_INVALID_ARG, "adam_step_sparse_rows: bad sizes / step");
-  SAE_REQUIRE(dense_dtype == SAE_F32 || dense_dtype == SAE_BF16, SAE_ERR_INVALID_ARG, "adam_step_sparse_rows: bad dtype %d", dense_dtype);
+  SAE_REQUIRE(dense_dtype == SAE_F32 || dense_dtype == SAE_BF16 || dense_dtype == SAE_ROWS8, SAE_ERR_INVALID_ARG, "adam_step_sparse_rows: bad dtype %d", dense_dtype);
   SAE_REQUIRE(d % 4 == 0 && F < (1LL << 31) && d < (1LL << 31), SAE_ERR_UNSUPPORTED,
               "adam_step_sparse_rows: d_model=%lld must be a multiple of 4", (long long)d);
   SAE_REQUIRE((((uintptr_t)p | (uintptr_t)m | (uintptr_t)v | (uintptr_t)dense) & 15) == 0, SAE_ERR_INVALID_ARG,
@@ -579,10 +579,12 @@ static int adam_step_sparse_rows_impl(bool lowp, const int32_t *feat_ptr, const 
   hipLaunchKernelGGL((adam_sparse_rows_persistent_kernel<BF, UU, true>), dim3(grid), dim3(256), 0, st, feat_ptr, feat_slot, \
                      slot_tok, coef, dense, p, m, v, (int)F, (int)d, a, nullptr, row_norm_out, bias_grad_out, grad_scale,  \
                      partial, extra_map, extra_rows, extra_bias)
-      if (dense_dtype == SAE_BF16) {
-        if (d <= 1024) SAE_ADAM_ROWS_LOWP(true, 1); else SAE_ADAM_ROWS_LOWP(true, 2);
+      if (dense_dtype == SAE_ROWS8) {
+        if (d <= 1024) SAE_ADAM_ROWS_LOWP(SAE_ROWS8, 1); else SAE_ADAM_ROWS_LOWP(SAE_ROWS8, 2);
+      } else if (dense_dtype == SAE_BF16) {
+        if (d <= 1024) SAE_ADAM_ROWS_LOWP(SAE_BF16, 1); else SAE_ADAM_ROWS_LOWP(SAE_BF16, 2);
       } else {
-        if (d <= 1024) SAE_ADAM_ROWS_LOWP(false, 1); else SAE_ADAM_ROWS_LOWP(false, 2);
+        if (d <= 1024) SAE_ADAM_ROWS_LOWP(SAE_F32, 1); else SAE_ADAM_ROWS_LOWP(SAE_F32, 2);
       }
 #undef SAE_ADAM_ROWS_LOWP
     } else if (u == 1 && d <= 768 && d > 512) {   // 129-192 pieces: three waves
@@ -590,12 +592,16 @@ static int adam_step_sparse_rows_impl(bool lowp, const int32_t *feat_ptr, const 
   hipLaunchKernelGGL((adam_sparse_rows_kernel<BF, 1, 192>), dim3((unsigned)F), dim3(192), 0, st, feat_ptr, feat_slot, slot_tok, \
                      coef, dense, p, m, v, (int)d, a, reinterpret_cast<uint16_t *>(shadow_bf16), row_norm_out,            \
                      bias_grad_out, grad_scale, partial, extra_map, extra_rows, extra_bias, row_grad_coef)
-      if (dense_dtype == SAE_BF16) SAE_ADAM_ROWS_192(true); else SAE_ADAM_ROWS_192(false);
+      if (dense_dtype == SAE_ROWS8) SAE_ADAM_ROWS_192(SAE_ROWS8);
+      else if (dense_dtype == SAE_BF16) SAE_ADAM_ROWS_192(SAE_BF16);
+      else SAE_ADAM_ROWS_192(SAE_F32);
 #undef SAE_ADAM_ROWS_192
+    } else if (dense_dtype == SAE_ROWS8) {
+      if (u == 1) SAE_ADAM_ROWS(SAE_ROWS8, 1); else if (u == 2) SAE_ADAM_ROWS(SAE_ROWS8, 2); else SAE_ADAM_ROWS(SAE_ROWS8, 4);
     } else if (dense_dtype == SAE_BF16) {
-      if (u == 1) SAE_ADAM_ROWS(true, 1); else if (u == 2) SAE_ADAM_ROWS(true, 2); else SAE_ADAM_ROWS(true, 4);
+      if (u == 1) SAE_ADAM_ROWS(SAE_BF16, 1); else if (u == 2) SAE_ADAM_ROWS(SAE_BF16, 2); else SAE_ADAM_ROWS(SAE_BF16, 4);
     } else {
-      if (u == 1) SAE_ADAM_ROWS(false, 1); else if (u == 2) SAE_ADAM_ROWS(false, 2); else SAE_ADAM_ROWS(false, 4);
+      if (u == 1) SAE_ADAM_ROWS(SAE_F32, 1); else if (u == 2) SAE_ADAM_ROWS(SAE_F32, 2); else SAE_ADAM_ROWS(SAE_F32, 4);
     }
 #undef SAE_ADAM_ROWS
   }
@@ -723,7 +729,7 @@ namespace sae {
 
 // One workgroup per feature: rebuilds the feature's gradient row exactly as adam_sparse_rows_kernel does
 // (same accumulation order, so the same bits) and reduces sum g^2 and #(g != 0) into partial[2 f], partial[2 f + 1].
-template <bool DENSE_BF16>
+template <int DENSE>
 __global__ __launch_bounds__(256) void sparse_rows_sq_nnz_kernel(
     const int32_t *__restrict__ feat_ptr, const int32_t *__restrict__ feat_slot, const int32_t *__restrict__ slot_tok,
     const float *__restrict__ coef, const void *__restrict__ dense, int d, double *__restrict__ partial,
@@ -745,7 +751,7 @@ __global__ __launch_bounds__(256) void sparse_rows_sq_nnz_kernel(
     return;
   }
   const int n_seg = d >> 2;
-  const size_t row_bytes = (size_t)d * (DENSE_BF16 ? 2 : 4);
+  const size_t row_bytes = dense_row_bytes<DENSE>(d);
   const char *dbase = reinterpret_cast<const char *>(dense);
   double sq = 0.0;
   int nz = 0;
@@ -757,7 +763,7 @@ __global__ __launch_bounds__(256) void sparse_rows_sq_nnz_kernel(
       g[u] = (xo >= 0 && seg < n_seg) ? reinterpret_cast<const float4 *>(extra_rows)[(int64_t)xo * n_seg + seg]
                                       : make_float4(0.f, 0.f, 0.f, 0.f);
     }
-    gather_rows_fma<DENSE_BF16>(g, lo, hi, feat_slot, slot_tok, coef, dbase, row_bytes, seg0, n_seg);
+    gather_rows_fma<DENSE>(g, lo, hi, feat_slot, slot_tok, coef, dbase, row_bytes, seg0, n_seg);
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
       float s4 = g[u].x * g[u].x;   // a 4-element fp32 partial keeps the fp64 adds off the critical path
@@ -818,7 +824,7 @@ extern "C" int sae_sparse_rows_grad_sq_nnz(const int32_t *feat_ptr, const int32_
   SAE_REQUIRE(feat_ptr && feat_slot && slot_tok && coef && dense && acc && workspace, SAE_ERR_INVALID_ARG,
               "sparse_rows_grad_sq_nnz: null pointer");
   SAE_REQUIRE(F > 0 && d > 0, SAE_ERR_INVALID_ARG, "sparse_rows_grad_sq_nnz: bad sizes");
-  SAE_REQUIRE(dense_dtype == SAE_F32 || dense_dtype == SAE_BF16, SAE_ERR_INVALID_ARG, "sparse_rows_grad_sq_nnz: bad dtype %d", dense_dtype);
+  SAE_REQUIRE(dense_dtype == SAE_F32 || dense_dtype == SAE_BF16 || dense_dtype == SAE_ROWS8, SAE_ERR_INVALID_ARG, "sparse_rows_grad_sq_nnz: bad dtype %d", dense_dtype);
   SAE_REQUIRE(d % 4 == 0 && F < (1LL << 31) && d < (1LL << 31), SAE_ERR_UNSUPPORTED,
               "sparse_rows_grad_sq_nnz: d_model=%lld must be a multiple of 4", (long long)d);
   SAE_REQUIRE((((uintptr_t)dense | (uintptr_t)workspace) & 15) == 0, SAE_ERR_INVALID_ARG,
@@ -827,11 +833,14 @@ extern "C" int sae_sparse_rows_grad_sq_nnz(const int32_t *feat_ptr, const int32_
               (long long)workspace_bytes, (long long)(16 * F));
   hipStream_t st = (hipStream_t)stream;
   double *partial = reinterpret_cast<double *>(workspace);
-  if (dense_dtype == SAE_BF16)
-    hipLaunchKernelGGL(sparse_rows_sq_nnz_kernel<true>, dim3((unsigned)F), dim3(256), 0, st, feat_ptr, feat_slot, slot_tok, coef,
+  if (dense_dtype == SAE_ROWS8)
+    hipLaunchKernelGGL(sparse_rows_sq_nnz_kernel<SAE_ROWS8>, dim3((unsigned)F), dim3(256), 0, st, feat_ptr, feat_slot, slot_tok, coef,
+                       dense, (int)d, partial, bias_grad_out, extra_map, extra_rows, extra_bias);
+  else if (dense_dtype == SAE_BF16)
+    hipLaunchKernelGGL(sparse_rows_sq_nnz_kernel<SAE_BF16>, dim3((unsigned)F), dim3(256), 0, st, feat_ptr, feat_slot, slot_tok, coef,
                        dense, (int)d, partial, bias_grad_out, extra_map, extra_rows, extra_bias);
   else
-    hipLaunchKernelGGL(sparse_rows_sq_nnz_kernel<false>, dim3((unsigned)F), dim3(256), 0, st, feat_ptr, feat_slot, slot_tok, coef,
+    hipLaunchKernelGGL(sparse_rows_sq_nnz_kernel<SAE_F32>, dim3((unsigned)F), dim3(256), 0, st, feat_ptr, feat_slot, slot_tok, coef,
                        dense, (int)d, partial, bias_grad_out, extra_map, extra_rows, extra_bias);
   hipLaunchKernelGGL(sq_nnz_finish_kernel, dim3(1), dim3(1024), 0, st, partial, F, acc);
   return check_launch("sparse_rows_grad_sq_nnz");

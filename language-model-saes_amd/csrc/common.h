@@ -137,24 +137,60 @@ struct __attribute__((aligned(16))) u32x4 {
   uint32_t x, y, z, w;
 };
 
+// ---- rows held in 8 bits (SAE_ROWS8; the record is described in rows8.hip) --------------------------------------
+constexpr int R8_BLOCK = 32;
+__host__ __device__ __forceinline__ int64_t r8_blocks(int64_t d) { return (d + R8_BLOCK - 1) / R8_BLOCK; }
+__host__ __device__ __forceinline__ int64_t r8_pitch(int64_t d) { return (r8_blocks(d) * (R8_BLOCK + 1) + 15) & ~(int64_t)15; }
+
+// ---- gathered rows of a dense operand (DENSE: SAE_F32, SAE_BF16 or SAE_ROWS8) -------------------------------------
+template <int DENSE>
+__host__ __device__ __forceinline__ size_t dense_row_bytes(int64_t d) {
+  return DENSE == SAE_ROWS8 ? (size_t)r8_pitch(d) : (size_t)d * (DENSE == SAE_BF16 ? 2 : 4);
+}
+// four elements of a row as they lie in memory: requested by load(row, seg), widened to fp32 by widen()
+template <int DENSE>
+struct DensePiece;
+template <>
+struct DensePiece<SAE_F32> {
+  float4 r;
+  __device__ __forceinline__ void load(const char *row, int seg, int) { r = reinterpret_cast<const float4 *>(row)[seg]; }
+  __device__ __forceinline__ float4 widen() const { return r; }
+};
+template <>
+struct DensePiece<SAE_BF16> {
+  uint2 r;
+  __device__ __forceinline__ void load(const char *row, int seg, int) { r = reinterpret_cast<const uint2 *>(row)[seg]; }
+  __device__ __forceinline__ float4 widen() const {
+    return make_float4(__uint_as_float(r.x << 16), __uint_as_float(r.x & 0xffff0000u), __uint_as_float(r.y << 16),
+                       __uint_as_float(r.y & 0xffff0000u));
+  }
+};
+template <>
+struct DensePiece<SAE_ROWS8> {
+  uint32_t codes, field;   // four codes, and the exponent field of their block's step
+  __device__ __forceinline__ void load(const char *row, int seg, int n_seg) {
+    codes = reinterpret_cast<const uint32_t *>(row)[seg];
+    field = reinterpret_cast<const uint8_t *>(row)[((n_seg + 7) >> 3) * R8_BLOCK + (seg >> 3)];
+  }
+  __device__ __forceinline__ float4 widen() const {   // code * step: exact, and NaN throughout where the step is infinite
+    const float step = __uint_as_float(field << 23);
+    return make_float4((float)(int8_t)codes * step, (float)(int8_t)(codes >> 8) * step, (float)(int8_t)(codes >> 16) * step,
+                       (float)(int8_t)(codes >> 24) * step);
+  }
+};
+
 // g[u] += sum over the segment's (slot, token) pairs of coef[slot] * dense[token, 4-element piece seg0 + ROW_THREADS u], pairs
 // in ascending order (the order every route to these gradient rows uses, so all of them give the same bits).
 // A pair costs three dependent loads (slot, then coefficient and token, then the row): pairs are taken in groups
 // whose index and row loads are all issued before the first multiply-add, which hides that chain on long segments.
-template <bool DENSE_BF16, int ROW_THREADS = 256>
+template <int DENSE, int ROW_THREADS = 256>
 __device__ __forceinline__ void gather_rows_fma(float4 (&g)[4], int lo, int hi, const int32_t *__restrict__ feat_slot,
                                                 const int32_t *__restrict__ slot_tok, const float *__restrict__ coef,
                                                 const char *dbase, size_t row_bytes, int seg0, int n_seg) {
-  constexpr int C = DENSE_BF16 ? 4 : 2;
-  typedef typename std::conditional<DENSE_BF16, uint2, float4>::type piece_t;
+  constexpr int C = DENSE == SAE_F32 ? 2 : 4;
+  typedef DensePiece<DENSE> piece_t;
   auto fma_piece = [&](float4 &acc, float c, const piece_t &r) {
-    float4 x;
-    if constexpr (DENSE_BF16) {
-      x.x = __uint_as_float(r.x << 16); x.y = __uint_as_float(r.x & 0xffff0000u);
-      x.z = __uint_as_float(r.y << 16); x.w = __uint_as_float(r.y & 0xffff0000u);
-    } else {
-      x = r;
-    }
+    const float4 x = r.widen();
     acc.x = fmaf(c, x.x, acc.x); acc.y = fmaf(c, x.y, acc.y);
     acc.z = fmaf(c, x.z, acc.z); acc.w = fmaf(c, x.w, acc.w);
   };
@@ -164,11 +200,11 @@ __device__ __forceinline__ void gather_rows_fma(float4 (&g)[4], int lo, int hi, 
 #pragma unroll
     for (int j = 0; j < C; ++j) sl[j] = feat_slot[i + j];
     float c[C];
-    const piece_t *row[C];
+    const char *row[C];
 #pragma unroll
     for (int j = 0; j < C; ++j) {
       c[j] = coef[sl[j]];
-      row[j] = reinterpret_cast<const piece_t *>(dbase + (size_t)slot_tok[sl[j]] * row_bytes);
+      row[j] = dbase + (size_t)slot_tok[sl[j]] * row_bytes;
     }
     piece_t r[C][4];
 #pragma unroll
@@ -176,7 +212,7 @@ __device__ __forceinline__ void gather_rows_fma(float4 (&g)[4], int lo, int hi, 
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
         const int seg = seg0 + u * ROW_THREADS;
-        if (seg < n_seg) r[j][u] = row[j][seg];
+        if (seg < n_seg) r[j][u].load(row[j], seg, n_seg);
       }
 #pragma unroll
     for (int j = 0; j < C; ++j)
@@ -187,11 +223,15 @@ __device__ __forceinline__ void gather_rows_fma(float4 (&g)[4], int lo, int hi, 
   for (; i < hi; ++i) {
     const int sl = feat_slot[i];
     const float c = coef[sl];
-    const piece_t *row = reinterpret_cast<const piece_t *>(dbase + (size_t)slot_tok[sl] * row_bytes);
+    const char *row = dbase + (size_t)slot_tok[sl] * row_bytes;
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
       const int seg = seg0 + u * ROW_THREADS;
-      if (seg < n_seg) fma_piece(g[u], c, row[seg]);
+      if (seg < n_seg) {
+        piece_t r;
+        r.load(row, seg, n_seg);
+        fma_piece(g[u], c, r);
+      }
     }
   }
 }
@@ -202,21 +242,15 @@ __device__ __forceinline__ void gather_rows_fma(float4 (&g)[4], int lo, int hi, 
 // index loads are paid once per chunk instead of once per group of pairs; the rows of a group of pairs are then
 // all requested before the first multiply-add.  U pieces per thread (piece u at seg0 + ROW_THREADS u); pairs in
 // ascending order as above, so the bits are the same.  s_coef / s_tok: ROW_THREADS entries of LDS each.
-template <bool DENSE_BF16, int ROW_THREADS, int U>
+template <int DENSE, int ROW_THREADS, int U>
 __device__ __forceinline__ void gather_rows_staged(float4 (&g)[U], int lo, int hi, const int32_t *__restrict__ feat_slot,
                                                    const int32_t *__restrict__ slot_tok, const float *__restrict__ coef,
                                                    const char *dbase, size_t row_bytes, int seg0, int n_seg,
                                                    float *s_coef, int32_t *s_tok) {
-  constexpr int C = (DENSE_BF16 ? 8 : 4) / (U == 4 ? 2 : 1);   // pairs whose rows are in flight together
-  typedef typename std::conditional<DENSE_BF16, uint2, float4>::type piece_t;
+  constexpr int C = (DENSE == SAE_F32 ? 4 : 8) / (U == 4 ? 2 : 1);   // pairs whose rows are in flight together
+  typedef DensePiece<DENSE> piece_t;
   auto fma_piece = [&](float4 &acc, float c, const piece_t &r) {
-    float4 x;
-    if constexpr (DENSE_BF16) {
-      x.x = __uint_as_float(r.x << 16); x.y = __uint_as_float(r.x & 0xffff0000u);
-      x.z = __uint_as_float(r.y << 16); x.w = __uint_as_float(r.y & 0xffff0000u);
-    } else {
-      x = r;
-    }
+    const float4 x = r.widen();
     acc.x = fmaf(c, x.x, acc.x); acc.y = fmaf(c, x.y, acc.y);
     acc.z = fmaf(c, x.z, acc.z); acc.w = fmaf(c, x.w, acc.w);
   };
@@ -235,10 +269,10 @@ __device__ __forceinline__ void gather_rows_staged(float4 (&g)[U], int lo, int h
       piece_t r[C][U];
 #pragma unroll
       for (int j = 0; j < C; ++j) {
-        const piece_t *row = reinterpret_cast<const piece_t *>(dbase + (size_t)s_tok[i + j] * row_bytes);
+        const char *row = dbase + (size_t)s_tok[i + j] * row_bytes;
 #pragma unroll
         for (int u = 0; u < U; ++u)
-          if (seg0 + u * ROW_THREADS < n_seg) r[j][u] = row[seg0 + u * ROW_THREADS];
+          if (seg0 + u * ROW_THREADS < n_seg) r[j][u].load(row, seg0 + u * ROW_THREADS, n_seg);
       }
 #pragma unroll
       for (int j = 0; j < C; ++j) {
@@ -250,10 +284,14 @@ __device__ __forceinline__ void gather_rows_staged(float4 (&g)[U], int lo, int h
     }
     for (; i < n; ++i) {
       const float c = s_coef[i];
-      const piece_t *row = reinterpret_cast<const piece_t *>(dbase + (size_t)s_tok[i] * row_bytes);
+      const char *row = dbase + (size_t)s_tok[i] * row_bytes;
 #pragma unroll
       for (int u = 0; u < U; ++u)
-        if (seg0 + u * ROW_THREADS < n_seg) fma_piece(g[u], c, row[seg0 + u * ROW_THREADS]);
+        if (seg0 + u * ROW_THREADS < n_seg) {
+          piece_t r;
+          r.load(row, seg0 + u * ROW_THREADS, n_seg);
+          fma_piece(g[u], c, r);
+        }
     }
   }
 }

@@ -217,7 +217,7 @@ __global__ __launch_bounds__(FI_THREADS) void fi_order_long_kernel(const int32_t
 }
 
 // out[f, :] = sum_{s in segment f} coef[s] * dense[slot_tok[s], :]
-template <bool DENSE_BF16>
+template <int DENSE>
 __global__ __launch_bounds__(FI_THREADS) void sparse_grad_rows_kernel(
     const int32_t *__restrict__ feat_ptr, const int32_t *__restrict__ feat_slot,
     const int32_t *__restrict__ slot_tok, const float *__restrict__ coef, const void *__restrict__ dense,
@@ -225,7 +225,7 @@ __global__ __launch_bounds__(FI_THREADS) void sparse_grad_rows_kernel(
   const int f = blockIdx.x, tid = threadIdx.x;
   const int lo = feat_ptr[f], hi = feat_ptr[f + 1];
   const int n_seg = d >> 2;  // float4 segments of the output row
-  const size_t row_bytes = (size_t)d * (DENSE_BF16 ? 2 : 4);
+  const size_t row_bytes = dense_row_bytes<DENSE>(d);
   const char *dbase = reinterpret_cast<const char *>(dense);
   float *orow = out + (size_t)f * d;
 
@@ -239,7 +239,7 @@ __global__ __launch_bounds__(FI_THREADS) void sparse_grad_rows_kernel(
     float4 acc[4];
 #pragma unroll
     for (int u = 0; u < 4; ++u) acc[u] = make_float4(0.f, 0.f, 0.f, 0.f);
-    gather_rows_fma<DENSE_BF16, FI_THREADS>(acc, lo, hi, feat_slot, slot_tok, coef, dbase, row_bytes, seg0, n_seg);
+    gather_rows_fma<DENSE, FI_THREADS>(acc, lo, hi, feat_slot, slot_tok, coef, dbase, row_bytes, seg0, n_seg);
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
       const int seg = seg0 + u * FI_THREADS;
@@ -247,6 +247,10 @@ __global__ __launch_bounds__(FI_THREADS) void sparse_grad_rows_kernel(
     }
   }
 }
+
+// the same for a dense operand held as rows8 (rows8.hip)
+int rows8_grad_rows(const int32_t *feat_ptr, const int32_t *feat_slot, const int32_t *slot_tok, const float *coef, const void *dense,
+                    float *out, float *bias_out, int64_t F, int64_t d, hipStream_t st);
 
 }  // namespace sae
 
@@ -299,15 +303,16 @@ extern "C" int sae_sparse_grad_rows(const int32_t *feat_ptr, const int32_t *feat
   SAE_REQUIRE(feat_ptr && feat_slot && slot_tok && coef && dense && out, SAE_ERR_INVALID_ARG,
               "sparse_grad_rows: null pointer");
   SAE_REQUIRE(F > 0 && d > 0, SAE_ERR_INVALID_ARG, "sparse_grad_rows: F and d must be positive");
-  SAE_REQUIRE(dense_dtype == SAE_F32 || dense_dtype == SAE_BF16, SAE_ERR_INVALID_ARG, "sparse_grad_rows: bad dtype %d", dense_dtype);
-  SAE_REQUIRE(d % 4 == 0, SAE_ERR_UNSUPPORTED, "sparse_grad_rows: d_model=%lld must be a multiple of 4", (long long)d);
-  SAE_REQUIRE(F < (1LL << 31), SAE_ERR_UNSUPPORTED, "sparse_grad_rows: F too large");
+  SAE_REQUIRE(dense_dtype == SAE_F32 || dense_dtype == SAE_BF16 || dense_dtype == SAE_ROWS8, SAE_ERR_INVALID_ARG, "sparse_grad_rows: bad dtype %d", dense_dtype);
+  SAE_REQUIRE(dense_dtype == SAE_ROWS8 || d % 4 == 0, SAE_ERR_UNSUPPORTED, "sparse_grad_rows: d_model=%lld must be a multiple of 4", (long long)d);
+  SAE_REQUIRE(F < (1LL << 31) && (dense_dtype != SAE_ROWS8 || d < (1LL << 30)), SAE_ERR_UNSUPPORTED, "sparse_grad_rows: F or d too large");
   hipStream_t st = (hipStream_t)stream;
+  if (dense_dtype == SAE_ROWS8) return rows8_grad_rows(feat_ptr, feat_slot, slot_tok, coef, dense, out, bias_out, F, d, st);
   if (dense_dtype == SAE_BF16)
-    hipLaunchKernelGGL(sparse_grad_rows_kernel<true>, dim3((unsigned)F), dim3(FI_THREADS), 0, st, feat_ptr, feat_slot,
+    hipLaunchKernelGGL(sparse_grad_rows_kernel<SAE_BF16>, dim3((unsigned)F), dim3(FI_THREADS), 0, st, feat_ptr, feat_slot,
                        slot_tok, coef, dense, out, bias_out, (int)d);
   else
-    hipLaunchKernelGGL(sparse_grad_rows_kernel<false>, dim3((unsigned)F), dim3(FI_THREADS), 0, st, feat_ptr, feat_slot,
+    hipLaunchKernelGGL(sparse_grad_rows_kernel<SAE_F32>, dim3((unsigned)F), dim3(FI_THREADS), 0, st, feat_ptr, feat_slot,
                        slot_tok, coef, dense, out, bias_out, (int)d);
   return check_launch("sparse_grad_rows");
 }

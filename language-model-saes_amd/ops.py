@@ -12,7 +12,7 @@ from typing import Optional, Tuple
 import torch
 
 from . import _lib
-from ._lib import SAE_BF16, SAE_F32, check
+from ._lib import SAE_BF16, SAE_F32, SAE_ROWS8, check
 
 
 def _stream(t: torch.Tensor) -> int:
@@ -131,6 +131,80 @@ class FeatureIndex:
     feat_ptr: torch.Tensor   # int32 [F + 1]
     feat_slot: torch.Tensor  # int32 [n_slots]
     slot_tok: torch.Tensor   # int32 [n_slots]
+
+
+ROWS8_BLOCK = 32             # values that share a step in rows held in 8 bits
+
+
+def rows8_pitch(d: int) -> int:
+    """Bytes of one record of d values (`sae_rows8_pitch`)."""
+    nb = -(-d // ROWS8_BLOCK)
+    return -(-(nb * (ROWS8_BLOCK + 1)) // 16) * 16
+
+
+@dataclass
+class Rows8:
+    """[n, d] rows held in 8 bits: int8 codes with one power-of-two step per 32 values (see include/sae_hip.h, "Rows held in
+    8 bits").  `data` is uint8 [n, rows8_pitch(d)], one record per row: copying, slicing, indexing and saving those rows
+    copies, slices, indexes and saves the activations.  Made by `quantize_rows`; read by `gather_rows` / `restore_rows`,
+    `gemm_over_tokens`, `sparse_grad_rows`, `adam_step_sparse_rows` and `sparse_rows_grad_sq_nnz`."""
+
+    data: torch.Tensor
+    d: int
+
+    def __post_init__(self):
+        if self.d < 1:
+            raise ValueError(f"rows need at least one value, got d = {self.d}")
+        if self.data.dtype != torch.uint8 or self.data.ndim != 2 or self.data.shape[1] != rows8_pitch(self.d):
+            raise ValueError(f"records of {self.d} values are uint8 [n, {rows8_pitch(self.d)}], got {self.data.dtype} "
+                             f"{tuple(self.data.shape)}")
+
+    @property
+    def shape(self) -> Tuple[int, int]:
+        return (self.data.shape[0], self.d)
+
+    @property
+    def device(self) -> torch.device:
+        return self.data.device
+
+    def __len__(self) -> int:
+        return self.data.shape[0]
+
+    def record_stream(self, stream) -> None:
+        self.data.record_stream(stream)
+
+
+class _on_device:
+    """Makes a tensor's device the current one for a launch on it (a no-op where it is already)."""
+
+    def __init__(self, t: torch.Tensor):
+        self.index = t.device.index
+
+    def __enter__(self):
+        self.prev = torch.cuda.current_device()
+        if self.prev != self.index:
+            torch.cuda.set_device(self.index)
+        return self
+
+    def __exit__(self, *exc):
+        if self.prev != self.index:
+            torch.cuda.set_device(self.prev)
+        return False
+
+
+def _req_rows8(q: Rows8, name: str):
+    _req(q.data, name, torch.uint8, 2)
+    if q.data.data_ptr() % 16:
+        raise ValueError(f"{name} must start on a 16-byte boundary")
+
+
+def _req_dense(dense, name: str = "dense"):
+    """The gathered operand of the gradient-row entry points: [n, d] fp32 / bf16, or `Rows8`.  -> (pointer, dtype, label)"""
+    if isinstance(dense, Rows8):
+        _req_rows8(dense, name)
+        return dense.data.data_ptr(), SAE_ROWS8, "rows8"
+    _req(dense, name, ndim=2)
+    return dense.data_ptr(), _dt(dense), "bf16" if dense.dtype == torch.bfloat16 else "f32"
 
 
 # ---- element-wise ---------------------------------------------------------------------------
@@ -792,19 +866,24 @@ def build_feature_index(code: SparseCode) -> FeatureIndex:
 
 def sparse_grad_rows(fi: FeatureIndex, coef: torch.Tensor, dense: torch.Tensor, F: int, want_bias: bool = False,
                      out: Optional[torch.Tensor] = None):
-    """out[f, :] = sum over feature f's slots of coef[slot] * dense[token(slot), :]; optional bias_out[f] = sum coef."""
+    """out[f, :] = sum over feature f's slots of coef[slot] * dense[token(slot), :]; optional bias_out[f] = sum coef.
+    `dense`: [n, d] fp32 / bf16 (d a multiple of 4), or `Rows8` (any d)."""
     _req(coef, "coef", torch.float32, 1)
-    _req(dense, "dense", ndim=2)
+    dense_ptr, dense_dt, label = _req_dense(dense)
     d = dense.shape[1]
     dev = dense.device
+    if label == "rows8" and (fi.feat_ptr.numel() != F + 1 or fi.feat_slot.numel() != coef.numel()
+                             or fi.slot_tok.numel() != coef.numel()):
+        raise ValueError(f"a feature index of {fi.feat_ptr.numel() - 1} features and {fi.feat_slot.numel()} slots does not fit "
+                         f"{F} features and {coef.numel()} coefficients")
     if out is None:
         out = torch.empty(F, d, dtype=torch.float32, device=dev)
     bias = torch.empty(F, dtype=torch.float32, device=dev) if want_bias else None
-    with _timed("sparse_grad_rows[bf16 dense]" if dense.dtype == torch.bfloat16 else "sparse_grad_rows[f32 dense]"):
+    with _timed(f"sparse_grad_rows[{label} dense]"), _on_device(coef):
         check(
             _lib.load().sae_sparse_grad_rows(fi.feat_ptr.data_ptr(), fi.feat_slot.data_ptr(), fi.slot_tok.data_ptr(),
-                                             coef.data_ptr(), dense.data_ptr(), _dt(dense), out.data_ptr(), _ptr(bias), F, d,
-                                             _stream(dense)),
+                                             coef.data_ptr(), dense_ptr, dense_dt, out.data_ptr(), _ptr(bias), F, d,
+                                             _stream(coef)),
             "sparse_grad_rows",
         )
     return out, bias
@@ -862,7 +941,7 @@ def adam_step_sparse_rows(fi: FeatureIndex, coef: torch.Tensor, dense: torch.Ten
     `row_grad_coef` (fp32 [F]) adds row_grad_coef[f] * p[f, :] to row f's gradient (the gradient through the row norm);
     `grad_scale` (device float scalar) multiplies the gradient first (gradient clipping);
     `grad_sq_nnz_acc` (device double[2]) += (sum g^2, #non-zero g) of the gradient consumed;
-    `extra` adds a densely held block of gradient rows.  A bf16 `p` (with bf16 `m`, `v`) takes the low-precision
+    `extra` adds a densely held block of gradient rows.  `dense` may be `Rows8`.  A bf16 `p` (with bf16 `m`, `v`) takes the low-precision
     update (no shadow copy, no row coefficient)."""
     lowp = p.dtype == torch.bfloat16
     for name, t in (("p", p), ("m", m), ("v", v)):
@@ -874,7 +953,7 @@ def adam_step_sparse_rows(fi: FeatureIndex, coef: torch.Tensor, dense: torch.Ten
         if row_grad_coef.numel() != p.shape[0]:
             raise ValueError("row_grad_coef must have one entry per row")
     _req(coef, "coef", torch.float32, 1)
-    _req(dense, "dense", ndim=2)
+    dense_ptr, dense_dt, label = _req_dense(dense)
     F, d = p.shape
     if dense.shape[1] != d or m.shape != p.shape or v.shape != p.shape:
         raise ValueError("shape mismatch between p, m, v and the dense operand")
@@ -889,11 +968,11 @@ def adam_step_sparse_rows(fi: FeatureIndex, coef: torch.Tensor, dense: torch.Ten
         _req(grad_sq_nnz_acc, "grad_sq_nnz_acc", torch.float64, 1)
         ws_bytes = 16 * F
         ws = torch.empty(2 * F, dtype=torch.float64, device=p.device)
-    with _timed("adam_step_sparse_rows[bf16 dense]" if dense.dtype == torch.bfloat16 else "adam_step_sparse_rows[f32 dense]"):
+    with _timed(f"adam_step_sparse_rows[{label} dense]"):
         if lowp:
             check(
                 _lib.load().sae_adam_step_sparse_rows_lowp(fi.feat_ptr.data_ptr(), fi.feat_slot.data_ptr(), fi.slot_tok.data_ptr(),
-                                                           coef.data_ptr(), dense.data_ptr(), _dt(dense), p.data_ptr(),
+                                                           coef.data_ptr(), dense_ptr, dense_dt, p.data_ptr(),
                                                            m.data_ptr(), v.data_ptr(), F, d, lr, beta1, beta2, eps, int(step),
                                                            _ptr(row_norm_out), _ptr(bias_grad_out), _ptr(grad_scale),
                                                            _ptr(grad_sq_nnz_acc), _ptr(ws), ws_bytes, *_extra_ptrs(extra, F, d),
@@ -903,7 +982,7 @@ def adam_step_sparse_rows(fi: FeatureIndex, coef: torch.Tensor, dense: torch.Ten
             return
         check(
             _lib.load().sae_adam_step_sparse_rows(fi.feat_ptr.data_ptr(), fi.feat_slot.data_ptr(), fi.slot_tok.data_ptr(),
-                                                  coef.data_ptr(), dense.data_ptr(), _dt(dense), p.data_ptr(), m.data_ptr(),
+                                                  coef.data_ptr(), dense_ptr, dense_dt, p.data_ptr(), m.data_ptr(),
                                                   v.data_ptr(), F, d, lr, beta1, beta2, eps, int(step), _ptr(shadow_bf16),
                                                   _ptr(row_norm_out), _ptr(bias_grad_out), _ptr(grad_scale),
                                                   _ptr(grad_sq_nnz_acc), _ptr(ws), ws_bytes, *_extra_ptrs(extra, F, d),
@@ -939,7 +1018,7 @@ def sparse_rows_grad_sq_nnz(fi: FeatureIndex, coef: torch.Tensor, dense: torch.T
     """acc (device double[2]) += (sum of squares, number of non-zero entries) of the [F, d] gradient that
     (fi, coef, dense) stand for; optionally writes the per-feature bias gradient as well."""
     _req(coef, "coef", torch.float32, 1)
-    _req(dense, "dense", ndim=2)
+    dense_ptr, dense_dt, _ = _req_dense(dense)
     _req(acc, "acc", torch.float64, 1)
     F, d = fi.feat_ptr.numel() - 1, dense.shape[1]
     lib = _lib.load()
@@ -948,8 +1027,8 @@ def sparse_rows_grad_sq_nnz(fi: FeatureIndex, coef: torch.Tensor, dense: torch.T
     with _timed("sparse_rows_grad_sq_nnz"):
         check(
             lib.sae_sparse_rows_grad_sq_nnz(fi.feat_ptr.data_ptr(), fi.feat_slot.data_ptr(), fi.slot_tok.data_ptr(),
-                                            coef.data_ptr(), dense.data_ptr(), _dt(dense), F, d, acc.data_ptr(),
-                                            _ptr(bias_grad_out), ws.data_ptr(), nbytes, *_extra_ptrs(extra, F, d), _stream(dense)),
+                                            coef.data_ptr(), dense_ptr, dense_dt, F, d, acc.data_ptr(),
+                                            _ptr(bias_grad_out), ws.data_ptr(), nbytes, *_extra_ptrs(extra, F, d), _stream(coef)),
             "sparse_rows_grad_sq_nnz",
         )
 
@@ -1279,9 +1358,13 @@ def mfma_probe(device: torch.device, n_workgroups: int = 4096, iters: int = 4096
     return flop.value, start.elapsed_time(end)
 
 
-def gather_rows(src: torch.Tensor, row_idx: torch.Tensor, out_dtype: Optional[torch.dtype] = None, scale: float = 1.0,
+def gather_rows(src, row_idx: torch.Tensor, out_dtype: Optional[torch.dtype] = None, scale: float = 1.0,
                 out: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """out[i] = cast(scale * src[row_idx[i]]) for a [N, d] fp32 / bf16 buffer and int64 row indices."""
+    """out[i] = cast(scale * src[row_idx[i]]) for a [N, d] fp32 / bf16 buffer, or `Rows8` (read as bf16 unless `out_dtype`
+    says otherwise), and int64 row indices.  Of `Rows8`, an index outside the buffer gives a row of NaN."""
+    if isinstance(src, Rows8):
+        _req(row_idx, "row_idx", torch.int64, 1)
+        return _read_rows8(src, row_idx, out_dtype, scale, out)
     _req(src, "src", ndim=2)
     _req(row_idx, "row_idx", torch.int64, 1)
     out_dtype = out_dtype or src.dtype
@@ -1301,3 +1384,120 @@ def gather_rows(src: torch.Tensor, row_idx: torch.Tensor, out_dtype: Optional[to
             "gather_rows",
         )
     return out
+
+
+# ---- rows held in 8 bits ---------------------------------------------------------------------
+
+def quantize_rows(x: torch.Tensor, out: Optional[torch.Tensor] = None, bf16_copy: bool = False):
+    """`Rows8` of x [n, d] (fp32 / bf16; rows may lie any distance apart, their values side by side).  `out`: uint8
+    [n, rows8_pitch(d)] to write the records into (rows of a buffer).  With `bf16_copy` also returns bf16(x), the operand a
+    bf16 product reads, from the same pass: -> (Rows8, [n, d] bf16); of a contiguous bf16 x that is x itself."""
+    if not x.is_cuda:
+        raise RuntimeError(f"x must live on the GPU (got {x.device}); the HIP path has no CPU fallback")
+    if x.ndim != 2 or x.shape[1] < 1:
+        raise ValueError(f"x must be [n, d] with d >= 1, got {tuple(x.shape)}")
+    n, d = x.shape
+    dt = _dt(x)
+    if d > 1 and x.stride(1) != 1:
+        raise ValueError("the values of a row of x must lie side by side")
+    pitch = rows8_pitch(d)
+    if out is None:
+        out = torch.empty(n, pitch, dtype=torch.uint8, device=x.device)
+    elif out.device != x.device:
+        raise ValueError("out must be on x's device")
+    rows = Rows8(out, d)
+    _req_rows8(rows, "out")
+    if len(rows) != n:
+        raise ValueError(f"out has {len(rows)} records for {n} rows")
+    copy = None
+    if bf16_copy:
+        copy = x if x.dtype == torch.bfloat16 and x.is_contiguous() else torch.empty(n, d, dtype=torch.bfloat16, device=x.device)
+    if n:
+        with _timed("rows8_quantize"), _on_device(x):
+            check(_lib.load().sae_rows8_quantize(x.data_ptr(), dt, n, d, x.stride(0), out.data_ptr(),
+                                                 None if copy is x else _ptr(copy), _stream(x)), "rows8_quantize")
+    return (rows, copy) if bf16_copy else rows
+
+
+def _read_rows8(src: Rows8, row_idx: Optional[torch.Tensor], out_dtype: Optional[torch.dtype], scale: float,
+                out: Optional[torch.Tensor]) -> torch.Tensor:
+    _req_rows8(src, "src")
+    out_dtype = out_dtype or torch.bfloat16
+    n, d = len(src) if row_idx is None else row_idx.numel(), src.d
+    if row_idx is not None and row_idx.device != src.device:
+        raise ValueError("row_idx must be on the buffer's device")
+    if out is None:
+        out = torch.empty(n, d, dtype=out_dtype, device=src.device)
+    else:
+        _req(out, "out", out_dtype, 2)
+        if tuple(out.shape) != (n, d) or out.device != src.device:
+            raise ValueError(f"out must be {(n, d)} on the buffer's device")
+    dt = _dt(out)
+    if n == 0:
+        return out
+    if len(src) == 0:
+        raise ValueError("rows asked of an empty buffer")
+    with _timed("rows8_gather"), _on_device(src.data):
+        check(_lib.load().sae_rows8_gather(src.data.data_ptr(), _ptr(row_idx), len(src), n, d, out.data_ptr(), dt, float(scale),
+                                           _stream(src.data)), "rows8_gather")
+    return out
+
+
+def restore_rows(src: Rows8, out_dtype: torch.dtype = torch.bfloat16, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """[n, d] values of all rows, in order (every value is exact in bf16)."""
+    return _read_rows8(src, None, out_dtype, 1.0, out)
+
+
+def _transpose_padded(src, out_dtype: torch.dtype, pitch: int) -> torch.Tensor:
+    """[cols, pitch] = src^T (fp32, bf16 or `Rows8` [rows, cols]), zeros behind the rows-th."""
+    t = src.data if isinstance(src, Rows8) else src
+    rows, cols = src.shape
+    out = torch.empty(cols, pitch, dtype=out_dtype, device=t.device)
+    with _timed("transpose_padded"):
+        check(_lib.load().sae_transpose_padded(t.data_ptr(), SAE_ROWS8 if t is not src else _dt(t), rows, cols, out.data_ptr(),
+                                               _dt(out), pitch, _stream(t)), "transpose_padded")
+    return out
+
+
+def gemm_over_tokens(left, right, out_dtype: torch.dtype = torch.float32) -> torch.Tensor:
+    """left^T @ right -> [m, n] for left [tokens, m] and right [tokens, n], each bf16, fp32 or `Rows8`: a weight gradient
+    d(pre)^T x or acts^T d(recon) whose saved side is held in 8 bits.  Any number of tokens and any widths.  Operands held in 8
+    bits are exact in bf16; with an fp32 operand the product is an fp32 product (and so is `out_dtype`), otherwise a bf16
+    product with fp32 accumulation.
+
+    Rows held in 8 bits are read once, into a transposed bf16 (fp32) operand: their steps change along the contraction, so
+    the codes cannot enter the matrix cores as they are, and widening them inside the product's tiles would be done again for
+    every tile of the other side."""
+    for name, t in (("left", left), ("right", right)):
+        if isinstance(t, Rows8):
+            _req_rows8(t, name)
+        else:
+            _req(t, name, ndim=2)
+            _dt(t)
+    (T, m), (T2, n) = left.shape, right.shape
+    if T != T2 or left.device != right.device:
+        raise ValueError(f"operands must share their tokens and device: left {tuple(left.shape)} on {left.device}, "
+                         f"right {tuple(right.shape)} on {right.device}")
+    if m < 1 or n < 1:
+        raise ValueError("operands need at least one column")
+    wide = any(not isinstance(t, Rows8) and t.dtype == torch.float32 for t in (left, right))
+    if out_dtype not in ((torch.float32,) if wide else (torch.float32, torch.bfloat16)):
+        raise TypeError(f"out_dtype {out_dtype} of a product of {'fp32' if wide else 'bf16'} operands")
+    dev = left.device
+    if T == 0:
+        return torch.zeros(m, n, dtype=out_dtype, device=dev)
+    with _on_device(left.data):
+        if wide:
+            pitch = -(-T // 32) * 32
+            return encoder_gemm(_transpose_padded(left, torch.float32, pitch), _transpose_padded(right, torch.float32, pitch),
+                                torch.float32)
+        pitch = -(-T // 64) * 64
+
+        def operand(t):
+            """(operand, whether it is stored [tokens, columns])"""
+            if not isinstance(t, Rows8) and T == pitch and t.shape[1] % 8 == 0 and t.data_ptr() % 16 == 0:
+                return t, True
+            return _transpose_padded(t, torch.bfloat16, pitch), False
+
+        (a, a_k), (b, b_k) = operand(left), operand(right)
+        return gemm(a, b, out_dtype, a_k_major=a_k, b_k_major=b_k)
