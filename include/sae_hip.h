@@ -319,8 +319,7 @@ int sae_build_feature_index(const int32_t *idx, const int64_t *row_off, const in
 
 /* out[f, :] = sum_{s in segment f} coef[s] * dense[slot_tok[s], :]   for every f in [0, F)
  * (rows with an empty segment are written as zeros, so `out` needs no prior clearing);
- * optionally bias_out[f] = sum coef[s].  dense [B, d] in dense_dtype (SAE_F32, SAE_BF16 or SAE_ROWS8), out [F, d]
- * fp32.  d a multiple of 4 (any d for SAE_ROWS8).
+ * optionally bias_out[f] = sum coef[s].  dense [B, d] in dense_dtype, out [F, d] fp32.
  * With coef = val and dense = grad_recon this is dW_D; with coef = d(pre) and dense = x it
  * is dW_E^T and bias_out = db_E.
  * Replaces the sorted atomic-add SpMM (kernels/kernels.py:137-225) and the dense
@@ -354,7 +353,7 @@ int sae_adam_step(float *p, const void *g, int g_dtype, float *m, float *v, int6
  * consumed at once; no dense gradient is stored.  Same update rule, scalars and by-products
  * (shadow_bf16, row_norm_out) as sae_adam_step; bias_grad_out (nullable) receives
  * sum_{s in segment f} coef[s], the gradient of the per-feature bias.  Bit-identical to
- * sae_sparse_grad_rows followed by sae_adam_step.  grad_scale (nullable): device float[1]; the
+ * sae_sparse_grad_rows followed by sae_adam_step (for SAE_ROWS8: on the rows those records read as).  grad_scale (nullable): device float[1]; the
  * row gradient and bias_grad_out are multiplied by it before use, which is clip_grad_norm's
  * `grad.mul_(factor)` (optim.py:280-292) with the factor left on the device.
  * grad_sq_nnz_acc (nullable): device double[2]; sum g^2 and #(g != 0) of the gradient this call consumes are
@@ -520,6 +519,17 @@ int sae_rows8_gather(const void *rows, const int64_t *row_idx, int64_t n_src_row
  * (records of cols values), dst [cols, dst_pitch] in SAE_F32 or SAE_BF16 (fp32 to bf16 rounds to nearest even). */
 int sae_transpose_padded(const void *src, int src_dtype, int64_t rows, int64_t cols, void *dst, int dst_dtype, int64_t dst_pitch,
                          void *stream);
+
+/* sae_sparse_grad_rows for a dense operand held as records (any d): out[f, :] = sum over the slots s of feature f of
+ * coef[s] * values of record slot_tok[s]; rows without slots are written as zeros; bias_out (nullable) [F].  n_slots: the
+ * length of feat_slot (feat_ptr[F] of them are in use).  A feature's slots are added in ascending order, as
+ * sae_sparse_grad_rows adds them; where they cross a multiple of a fixed length in feat_slot the pieces are summed apart and
+ * then joined in order, so a feature that many tokens keep costs no more time than as many slots of rare ones.  workspace:
+ * sae_rows8_grad_rows_workspace_bytes(n_slots, d) bytes, 16-byte aligned. */
+int64_t sae_rows8_grad_rows_workspace_bytes(int64_t n_slots, int64_t d);
+int sae_rows8_grad_rows(const int32_t *feat_ptr, const int32_t *feat_slot, const int32_t *slot_tok, const float *coef,
+                        const void *rows, float *out, float *bias_out, int64_t F, int64_t d, int64_t n_slots, void *workspace,
+                        int64_t workspace_bytes, void *stream);
 
 /* ---- Training metrics from the sparse code ----------------------------------------------------------
  * The per-step quantities behind FrequencyMetric, MeanFeatureActMetric and L0Metric (metrics.py:102-127,

@@ -248,10 +248,6 @@ __global__ __launch_bounds__(FI_THREADS) void sparse_grad_rows_kernel(
   }
 }
 
-// the same for a dense operand held as rows8 (rows8.hip)
-int rows8_grad_rows(const int32_t *feat_ptr, const int32_t *feat_slot, const int32_t *slot_tok, const float *coef, const void *dense,
-                    float *out, float *bias_out, int64_t F, int64_t d, hipStream_t st);
-
 }  // namespace sae
 
 extern "C" int64_t sae_feature_index_workspace_bytes(int64_t B, int64_t F, int64_t n_slots) {
@@ -303,11 +299,10 @@ extern "C" int sae_sparse_grad_rows(const int32_t *feat_ptr, const int32_t *feat
   SAE_REQUIRE(feat_ptr && feat_slot && slot_tok && coef && dense && out, SAE_ERR_INVALID_ARG,
               "sparse_grad_rows: null pointer");
   SAE_REQUIRE(F > 0 && d > 0, SAE_ERR_INVALID_ARG, "sparse_grad_rows: F and d must be positive");
-  SAE_REQUIRE(dense_dtype == SAE_F32 || dense_dtype == SAE_BF16 || dense_dtype == SAE_ROWS8, SAE_ERR_INVALID_ARG, "sparse_grad_rows: bad dtype %d", dense_dtype);
-  SAE_REQUIRE(dense_dtype == SAE_ROWS8 || d % 4 == 0, SAE_ERR_UNSUPPORTED, "sparse_grad_rows: d_model=%lld must be a multiple of 4", (long long)d);
-  SAE_REQUIRE(F < (1LL << 31) && (dense_dtype != SAE_ROWS8 || d < (1LL << 30)), SAE_ERR_UNSUPPORTED, "sparse_grad_rows: F or d too large");
+  SAE_REQUIRE(dense_dtype == SAE_F32 || dense_dtype == SAE_BF16, SAE_ERR_INVALID_ARG, "sparse_grad_rows: bad dtype %d", dense_dtype);
+  SAE_REQUIRE(d % 4 == 0, SAE_ERR_UNSUPPORTED, "sparse_grad_rows: d_model=%lld must be a multiple of 4", (long long)d);
+  SAE_REQUIRE(F < (1LL << 31), SAE_ERR_UNSUPPORTED, "sparse_grad_rows: F too large");
   hipStream_t st = (hipStream_t)stream;
-  if (dense_dtype == SAE_ROWS8) return rows8_grad_rows(feat_ptr, feat_slot, slot_tok, coef, dense, out, bias_out, F, d, st);
   if (dense_dtype == SAE_BF16)
     hipLaunchKernelGGL(sparse_grad_rows_kernel<SAE_BF16>, dim3((unsigned)F), dim3(FI_THREADS), 0, st, feat_ptr, feat_slot,
                        slot_tok, coef, dense, out, bias_out, (int)d);

@@ -105,35 +105,168 @@ __global__ __launch_bounds__(256) void transpose_padded_kernel(const void *__res
   }
 }
 
-// out[f, :] = sum over feature f's slots, in the index's order, of coef[slot] * values of record slot_tok[slot]
-__global__ __launch_bounds__(256) void rows8_grad_rows_kernel(const int32_t *__restrict__ feat_ptr, const int32_t *__restrict__ feat_slot,
-                                                              const int32_t *__restrict__ slot_tok, const float *__restrict__ coef,
-                                                              const uint8_t *__restrict__ rows, float *__restrict__ out,
-                                                              float *__restrict__ bias_out, int64_t d) {
-  const int64_t f = blockIdx.x, codes = r8_blocks(d) * R8_BLOCK, pitch = r8_pitch(d);
+// ---- gradient rows ---------------------------------------------------------------------------------------------------
+// out[f, :] = sum over feature f's slots of coef * (values of the slot's record): a segmented sum over the feature index.
+// Some features are kept by most tokens and most by few, so work is cut by position in feat_slot, not by feature: a wave
+// owns a window of R8_WINDOW positions and 64 C columns.  A segment that lies inside a window goes straight to its row; one
+// that crosses leaves one partial row per window, joined in window order by a third launch.
+constexpr int R8_WINDOW = 128;
+
+// Per feature: the feature of each of its positions, a zero row where it has none, its coefficients' sum.
+__global__ __launch_bounds__(256) void rows8_grad_prepare_kernel(const int32_t *__restrict__ feat_ptr, const int32_t *__restrict__ feat_slot,
+                                                                 const float *__restrict__ coef, int32_t *__restrict__ pos_feat,
+                                                                 float *__restrict__ out, float *__restrict__ bias_out, int64_t F, int64_t d) {
+  const int64_t f = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63;
+  if (f >= F) return;
   const int lo = feat_ptr[f], hi = feat_ptr[f + 1];
-  if (bias_out && threadIdx.x < 64) {
+  for (int i = lo + lane; i < hi; i += 64) pos_feat[i] = (int32_t)f;
+  if (bias_out) {
     float s = 0.f;
-    for (int i = lo + (int)threadIdx.x; i < hi; i += 64) s += coef[feat_slot[i]];
+    for (int i = lo + lane; i < hi; i += 64) s += coef[feat_slot[i]];
     s = wave_sum(s);
-    if (threadIdx.x == 0) bias_out[f] = s;
+    if (lane == 0) bias_out[f] = s;
   }
-  for (int64_t j = threadIdx.x; j < d; j += 256) {
-    float acc = 0.f;
-    for (int i = lo; i < hi; ++i) {
-      const int sl = feat_slot[i];
-      acc = fmaf(coef[sl], r8_value(rows + (int64_t)slot_tok[sl] * pitch, codes, j), acc);
-    }
-    out[f * d + j] = acc;
+  if (lo < hi) return;
+  float *row = out + f * d;
+  if ((d & 3) == 0) {
+    for (int64_t j = lane; j < (d >> 2); j += 64) reinterpret_cast<float4 *>(row)[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+  } else {
+    for (int64_t j = lane; j < d; j += 64) row[j] = 0.f;
   }
 }
 
-// called by sae_sparse_grad_rows (feature_index.hip) for a dense operand held as rows8
-int rows8_grad_rows(const int32_t *feat_ptr, const int32_t *feat_slot, const int32_t *slot_tok, const float *coef, const void *dense,
-                    float *out, float *bias_out, int64_t F, int64_t d, hipStream_t st) {
-  hipLaunchKernelGGL(rows8_grad_rows_kernel, dim3((unsigned)F), dim3(256), 0, st, feat_ptr, feat_slot, slot_tok, coef,
-                     reinterpret_cast<const uint8_t *>(dense), out, bias_out, d);
-  return check_launch("sparse_grad_rows[rows8]");
+// C codes per lane as they lie in memory
+template <int C>
+struct R8Piece {
+  uint32_t w[C / 4];
+  uint32_t field;
+};
+
+template <int C>
+__global__ __launch_bounds__(256) void rows8_grad_window_kernel(const int32_t *__restrict__ feat_ptr, const int32_t *__restrict__ feat_slot,
+                                                                const int32_t *__restrict__ slot_tok, const float *__restrict__ coef,
+                                                                const uint8_t *__restrict__ rows, const int32_t *__restrict__ pos_feat,
+                                                                float *__restrict__ out, float *__restrict__ part, int64_t F, int64_t d,
+                                                                int64_t n_windows, int64_t n_tasks) {
+  constexpr int G = 32 / C * 2;   // records requested together: 16 of 4 codes, 8 of 8
+  const int lane = threadIdx.x & 63;
+  // tasks in chunk-major order, one contiguous eighth per XCD (workgroups go round the XCDs): what an XCD reads at a time
+  // is one chunk of columns of all records, which its L2 holds
+  const int64_t per_xcd = (n_tasks + 7) / 8;
+  const int64_t local = (int64_t)(blockIdx.x >> 3) * 4 + (threadIdx.x >> 6);
+  const int64_t task = (int64_t)(blockIdx.x & 7) * per_xcd + local;
+  if (local >= per_xcd || task >= n_tasks) return;
+  const int64_t chunk = task / n_windows, window = task % n_windows;
+  const int total = feat_ptr[F];
+  const int w0 = (int)(window * R8_WINDOW);
+  if (w0 >= total) return;
+  const int w1 = w0 + R8_WINDOW < total ? w0 + R8_WINDOW : total;
+  const int64_t codes = r8_blocks(d) * R8_BLOCK, pitch = r8_pitch(d);
+  const int64_t col = chunk * 64 * C + lane * C;
+  const bool on = col < codes;
+  const uint32_t code_at = on ? (uint32_t)col : 0u, field_at = (uint32_t)(codes + (on ? col >> 5 : 0));   // offsets in a record
+  const int before = w0 > 0 ? pos_feat[w0 - 1] : -1, after = w1 < total ? pos_feat[w1] : -1;
+
+  float acc[C];
+#pragma unroll
+  for (int e = 0; e < C; ++e) acc[e] = 0.f;
+  int current = -1;   // the feature being summed
+  auto flush = [&]() {
+    if (on && current >= 0) {
+      const bool head = current == before, tail = current == after;
+      if (head || tail) {
+        float *dst = part + (window * 2 + (head ? 0 : 1)) * codes + col;
+#pragma unroll
+        for (int e = 0; e < C; e += 4) *reinterpret_cast<float4 *>(dst + e) = make_float4(acc[e], acc[e + 1], acc[e + 2], acc[e + 3]);
+      } else {
+        float *dst = out + (int64_t)current * d + col;
+        if ((d & 3) == 0) {
+#pragma unroll
+          for (int e = 0; e < C; e += 4)
+            if (col + e < d) *reinterpret_cast<float4 *>(dst + e) = make_float4(acc[e], acc[e + 1], acc[e + 2], acc[e + 3]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < C; ++e)
+            if (col + e < d) dst[e] = acc[e];
+        }
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < C; ++e) acc[e] = 0.f;
+  };
+
+  for (int p0 = w0; p0 < w1; p0 += 64) {
+    const int n = w1 - p0 < 64 ? w1 - p0 : 64;
+    int tok = 0, feat = -1;
+    float c = 0.f;
+    if (lane < n) {
+      const int slot = feat_slot[p0 + lane];
+      tok = slot_tok[slot];
+      c = coef[slot];
+      feat = pos_feat[p0 + lane];
+    }
+    for (int j0 = 0; j0 < n; j0 += G) {
+      R8Piece<C> r[G];
+#pragma unroll
+      for (int j = 0; j < G; ++j) {
+        const int at = j0 + j < n ? j0 + j : n - 1;
+        const uint8_t *rec = rows + (int64_t)__builtin_amdgcn_readlane(tok, at) * pitch;   // the same for the whole wave
+        if constexpr (C == 4) {
+          r[j].w[0] = *reinterpret_cast<const uint32_t *>(rec + code_at);
+        } else {
+          const uint2 w = *reinterpret_cast<const uint2 *>(rec + code_at);
+          r[j].w[0] = w.x;
+          r[j].w[C / 4 - 1] = w.y;
+        }
+        r[j].field = rec[field_at];
+      }
+#pragma unroll
+      for (int j = 0; j < G; ++j) {
+        if (j0 + j < n) {
+          const int f = __builtin_amdgcn_readlane(feat, j0 + j);
+          if (f != current) {
+            flush();
+            current = f;
+          }
+          const float cc = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(c), j0 + j));
+          const float step = __uint_as_float(r[j].field << 23);
+#pragma unroll
+          for (int e = 0; e < C; ++e) acc[e] = fmaf(cc, (float)(int8_t)(r[j].w[e / 4] >> (8 * (e % 4))) * step, acc[e]);
+        }
+      }
+    }
+  }
+  flush();
+}
+
+// The segment that begins in this window and goes on behind it: its partial rows, added in window order.
+__global__ __launch_bounds__(256) void rows8_grad_join_kernel(const int32_t *__restrict__ feat_ptr, const int32_t *__restrict__ pos_feat,
+                                                              const float *__restrict__ part, float *__restrict__ out, int64_t F, int64_t d) {
+  const int64_t window = blockIdx.x;
+  const int total = feat_ptr[F];
+  const int64_t w0 = window * R8_WINDOW, w1 = w0 + R8_WINDOW;
+  if (w1 >= total) return;
+  const int f = pos_feat[w1];
+  if (pos_feat[w1 - 1] != f || (w0 > 0 && pos_feat[w0 - 1] == f)) return;
+  const int64_t last = (feat_ptr[f + 1] - 1) / R8_WINDOW, codes = r8_blocks(d) * R8_BLOCK;
+  const int64_t j = ((int64_t)blockIdx.y * 256 + threadIdx.x) * 4;
+  if (j >= d) return;
+  float4 s = *reinterpret_cast<const float4 *>(part + (window * 2 + 1) * codes + j);
+#pragma unroll 4
+  for (int64_t w = window + 1; w <= last; ++w) {
+    const float4 x = *reinterpret_cast<const float4 *>(part + w * 2 * codes + j);
+    s.x += x.x; s.y += x.y; s.z += x.z; s.w += x.w;
+  }
+  float *dst = out + (int64_t)f * d + j;
+  if ((d & 3) == 0) {
+    *reinterpret_cast<float4 *>(dst) = s;
+  } else {
+    const float v[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (j + e < d) dst[e] = v[e];
+  }
 }
 
 }  // namespace sae
@@ -199,4 +332,44 @@ extern "C" int sae_transpose_padded(const void *src, int src_dtype, int64_t rows
   }
 #undef SAE_TP
   return check_launch("transpose_padded");
+}
+
+namespace sae {
+static int64_t r8_windows(int64_t n_slots) { return (n_slots + R8_WINDOW - 1) / R8_WINDOW; }
+static int64_t r8_part_offset(int64_t n_slots) { return (n_slots * 4 + 15) & ~(int64_t)15; }
+}  // namespace sae
+
+extern "C" int64_t sae_rows8_grad_rows_workspace_bytes(int64_t n_slots, int64_t d) {
+  using namespace sae;
+  if (n_slots <= 0 || d <= 0) return 0;
+  // the feature of every position, and two partial rows per window
+  return r8_part_offset(n_slots) + r8_windows(n_slots) * 2 * r8_blocks(d) * R8_BLOCK * 4;
+}
+
+extern "C" int sae_rows8_grad_rows(const int32_t *feat_ptr, const int32_t *feat_slot, const int32_t *slot_tok, const float *coef,
+                                   const void *rows, float *out, float *bias_out, int64_t F, int64_t d, int64_t n_slots,
+                                   void *workspace, int64_t workspace_bytes, void *stream) {
+  using namespace sae;
+  SAE_REQUIRE(feat_ptr && feat_slot && slot_tok && coef && rows && out, SAE_ERR_INVALID_ARG, "rows8_grad_rows: null pointer");
+  SAE_REQUIRE(F > 0 && d > 0 && n_slots > 0, SAE_ERR_INVALID_ARG, "rows8_grad_rows: bad sizes");
+  SAE_REQUIRE(F < (1LL << 31) - 1 && d < (1LL << 30) && n_slots < (1LL << 31) - R8_WINDOW, SAE_ERR_UNSUPPORTED, "rows8_grad_rows: size too large");
+  SAE_REQUIRE((((uintptr_t)rows | (uintptr_t)out | (uintptr_t)workspace) & 15) == 0, SAE_ERR_INVALID_ARG,
+              "rows8_grad_rows: 16-byte alignment required");
+  SAE_REQUIRE(workspace && workspace_bytes >= sae_rows8_grad_rows_workspace_bytes(n_slots, d), SAE_ERR_WORKSPACE,
+              "rows8_grad_rows: workspace of %lld bytes needed", (long long)sae_rows8_grad_rows_workspace_bytes(n_slots, d));
+  hipStream_t st = (hipStream_t)stream;
+  int32_t *pos_feat = reinterpret_cast<int32_t *>(workspace);
+  float *part = reinterpret_cast<float *>(reinterpret_cast<char *>(workspace) + r8_part_offset(n_slots));
+  const uint8_t *rec = reinterpret_cast<const uint8_t *>(rows);
+  hipLaunchKernelGGL(rows8_grad_prepare_kernel, dim3((unsigned)((F + 3) / 4)), dim3(256), 0, st, feat_ptr, feat_slot, coef, pos_feat, out,
+                     bias_out, F, d);
+  constexpr int C = 4;
+  const int64_t windows = r8_windows(n_slots), chunks = (r8_blocks(d) * R8_BLOCK + 64 * C - 1) / (64 * C), tasks = windows * chunks;
+  const int64_t per_xcd = (tasks + 7) / 8, blocks = (per_xcd + 3) / 4 * 8;
+  SAE_REQUIRE(blocks < (1LL << 31), SAE_ERR_UNSUPPORTED, "rows8_grad_rows: size too large");
+  hipLaunchKernelGGL(rows8_grad_window_kernel<C>, dim3((unsigned)blocks), dim3(256), 0, st, feat_ptr, feat_slot, slot_tok, coef, rec, pos_feat,
+                     out, part, F, d, windows, tasks);
+  hipLaunchKernelGGL(rows8_grad_join_kernel, dim3((unsigned)windows, (unsigned)((d + 1023) / 1024)), dim3(256), 0, st, feat_ptr, pos_feat, part,
+                     out, F, d);
+  return check_launch("rows8_grad_rows");
 }

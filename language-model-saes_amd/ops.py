@@ -872,18 +872,17 @@ def sparse_grad_rows(fi: FeatureIndex, coef: torch.Tensor, dense: torch.Tensor, 
     dense_ptr, dense_dt, label = _req_dense(dense)
     d = dense.shape[1]
     dev = dense.device
-    if label == "rows8" and (fi.feat_ptr.numel() != F + 1 or fi.feat_slot.numel() != coef.numel()
-                             or fi.slot_tok.numel() != coef.numel()):
-        raise ValueError(f"a feature index of {fi.feat_ptr.numel() - 1} features and {fi.feat_slot.numel()} slots does not fit "
-                         f"{F} features and {coef.numel()} coefficients")
     if out is None:
         out = torch.empty(F, d, dtype=torch.float32, device=dev)
     bias = torch.empty(F, dtype=torch.float32, device=dev) if want_bias else None
-    with _timed(f"sparse_grad_rows[{label} dense]"), _on_device(coef):
+    if label == "rows8":
+        _rows8_grad_rows(fi, coef, dense, F, out, bias)
+        return out, bias
+    with _timed("sparse_grad_rows[bf16 dense]" if dense.dtype == torch.bfloat16 else "sparse_grad_rows[f32 dense]"):
         check(
             _lib.load().sae_sparse_grad_rows(fi.feat_ptr.data_ptr(), fi.feat_slot.data_ptr(), fi.slot_tok.data_ptr(),
-                                             coef.data_ptr(), dense_ptr, dense_dt, out.data_ptr(), _ptr(bias), F, d,
-                                             _stream(coef)),
+                                             coef.data_ptr(), dense.data_ptr(), _dt(dense), out.data_ptr(), _ptr(bias), F, d,
+                                             _stream(dense)),
             "sparse_grad_rows",
         )
     return out, bias
@@ -1441,6 +1440,30 @@ def _read_rows8(src: Rows8, row_idx: Optional[torch.Tensor], out_dtype: Optional
         check(_lib.load().sae_rows8_gather(src.data.data_ptr(), _ptr(row_idx), len(src), n, d, out.data_ptr(), dt, float(scale),
                                            _stream(src.data)), "rows8_gather")
     return out
+
+
+def _rows8_grad_rows(fi: FeatureIndex, coef: torch.Tensor, rows: Rows8, F: int, out: torch.Tensor, bias: Optional[torch.Tensor]):
+    _req(out, "out", torch.float32, 2)
+    n_slots, d = coef.numel(), rows.d
+    if tuple(out.shape) != (F, d):
+        raise ValueError(f"out must be {(F, d)}, got {tuple(out.shape)}")
+    if fi.feat_ptr.numel() != F + 1 or fi.feat_slot.numel() != n_slots or fi.slot_tok.numel() != n_slots:
+        raise ValueError(f"a feature index of {fi.feat_ptr.numel() - 1} features and {fi.feat_slot.numel()} slots does not fit "
+                         f"{F} features and {n_slots} coefficients")
+    if any(t.device != rows.device for t in (coef, out, fi.feat_ptr, fi.feat_slot, fi.slot_tok)):
+        raise ValueError("the index, the coefficients, the rows and out must be on one device")
+    if F == 0 or n_slots == 0:
+        out.zero_()
+        if bias is not None:
+            bias.zero_()
+        return
+    lib = _lib.load()
+    nbytes = lib.sae_rows8_grad_rows_workspace_bytes(n_slots, d)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=rows.device)
+    with _timed("sparse_grad_rows[rows8 dense]"), _on_device(coef):
+        check(lib.sae_rows8_grad_rows(fi.feat_ptr.data_ptr(), fi.feat_slot.data_ptr(), fi.slot_tok.data_ptr(), coef.data_ptr(),
+                                      rows.data.data_ptr(), out.data_ptr(), _ptr(bias), F, d, n_slots, ws.data_ptr(), nbytes,
+                                      _stream(coef)), "rows8_grad_rows")
 
 
 def restore_rows(src: Rows8, out_dtype: torch.dtype = torch.bfloat16, out: Optional[torch.Tensor] = None) -> torch.Tensor:

@@ -50,5 +50,9 @@ def test_entry_points_refuse_before_any_launch(pkg):
     tr = lambda src=P, dt=2, r=4, c=40, dst=P, odt=1, pitch=64: lib.sae_transpose_padded(src, dt, r, c, dst, odt, pitch, None)  # noqa: E731
     assert tr(src=None) == -1 and tr(dst=None) == -1 and tr(r=0) == -1 and tr(pitch=3) == -1 and tr(dt=3) == -1 and tr(odt=2) == -1
     assert tr(pitch=1 << 30) == -2
-    rows = lambda dt, d: lib.sae_sparse_grad_rows(P, P, P, P, P, dt, P, None, 4, d, None)  # noqa: E731
-    assert rows(3, 40) == -1 and rows(1, 42) == -2 and rows(2, 1 << 30) == -2
+    need = lib.sae_rows8_grad_rows_workspace_bytes(100, 40)
+    assert need >= 100 * 4 and lib.sae_rows8_grad_rows_workspace_bytes(0, 40) == 0
+    rows = lambda r=P, out=P, F=4, d=40, n=100, ws=P, b=need: lib.sae_rows8_grad_rows(P, P, P, P, r, out, None, F, d, n, ws, b, None)  # noqa: E731
+    assert rows(r=None) == -1 and rows(out=None) == -1 and rows(F=0) == -1 and rows(d=0) == -1 and rows(n=0) == -1
+    assert rows(r=P + 8) == -1 and rows(ws=None) == -4 and rows(b=need - 1) == -4 and rows(d=1 << 30) == -2 and rows(n=(1 << 31) - 1) == -2
+    assert lib.sae_sparse_grad_rows(P, P, P, P, P, 2, P, None, 4, 40, None) == -1      # records have their own entry point
