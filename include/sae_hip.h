@@ -505,7 +505,8 @@ int sae_gather_rows(const void *src, int src_dtype, const int64_t *row_idx, int6
 int64_t sae_rows8_pitch(int64_t d);
 
 /* rows[i] = record of src[i, :], i < n.  src: SAE_F32 or SAE_BF16, row i at element i * src_stride (unit stride inside a
- * row).  bf16_copy (nullable): bf16 [n, d], the rounded source itself, what a bf16 product reads, from the same pass. */
+ * row).  bf16_copy (nullable, for an fp32 source): bf16 [n, d], the source rounded to what a bf16 product reads, from the
+ * same pass. */
 int sae_rows8_quantize(const void *src, int src_dtype, int64_t n, int64_t d, int64_t src_stride, void *rows, void *bf16_copy,
                        void *stream);
 

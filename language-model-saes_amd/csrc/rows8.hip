@@ -13,21 +13,28 @@
 namespace sae {
 
 // field of a block whose largest magnitude has these bits: the smallest step that brings it to 127 after rounding, i.e.
-// 2^(floor(log2 amax) - 6), and twice that where amax / step would round to 128 (mantissa from 127.5 / 64 on; the tie is
-// even at 128).  In the last binade there is no larger step whose codes stay finite: codes stop at 127 there.
+// 2^(floor(log2 amax) - 6), and twice that where amax / step would round to 128 (mantissa from 127.5 / 64 on, the tie going
+// to the even 128: the addition carries into the exponent there).  In the last binade no larger step is left whose values
+// stay finite: codes stop at 127 there.
 __device__ __forceinline__ uint32_t r8_field(uint32_t amax_bits) {
-  const uint32_t e = amax_bits >> 23;
-  if (amax_bits == 0u) return 0u;
-  if (e == 255u) return 255u;
-  if (e < 7u) return 1u;
-  return e - 6u + ((e < 254u && (amax_bits & 0x7fffffu) >= 0x7f0000u) ? 1u : 0u);
+  const uint32_t e = (amax_bits + 0x10000u) >> 23;
+  uint32_t f = (e > 7u ? e : 7u) - 6u;
+  f = f < 248u ? f : 248u;
+  f = amax_bits == 0u ? 0u : f;
+  return amax_bits >= 0x7f800000u ? 255u : f;
 }
 
-// one float -> its code under a block's field
-__device__ __forceinline__ int r8_code(float x, uint32_t field) {
-  if (field == 0u || field == 255u) return 0;
-  const float inv = __uint_as_float((254u - field) << 23);
-  return (int)fminf(fmaxf(rintf(x * inv), -127.f), 127.f);
+// Four floats -> their codes under a block's field, packed.  x / step is exact (a power of two); adding 1.5 * 2^23 rounds it to
+// nearest even and leaves the code in the sum's low byte.
+__device__ __forceinline__ uint32_t r8_codes(const float *x, uint32_t field) {
+  const bool bad = field == 255u;   // an infinity or a NaN in the block: no codes
+  const float inv = __uint_as_float((254u - field) << 23);   // field 0: all x are 0
+  uint32_t b[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    b[e] = __float_as_uint(__builtin_amdgcn_fmed3f((bad ? 0.f : x[e]) * (bad ? 0.f : inv), -127.f, 127.f) + 12582912.f);
+  const uint32_t lo = __builtin_amdgcn_perm(b[1], b[0], 0x0c0c0400u), hi = __builtin_amdgcn_perm(b[3], b[2], 0x04000c0cu);
+  return lo | hi;
 }
 
 template <int DT>
@@ -47,38 +54,169 @@ __device__ __forceinline__ float r8_value(const uint8_t *rec, int64_t codes, int
   return (float)(int8_t)rec[j] * step;
 }
 
-// One workgroup per row; half a wave owns a block, one value per lane.
-template <int DT>
-__global__ __launch_bounds__(256) void rows8_quantize_kernel(const void *__restrict__ src, int64_t stride, int64_t d, uint8_t *__restrict__ dst,
-                                                             uint16_t *__restrict__ copy) {
-  const int64_t row = blockIdx.x, nb = r8_blocks(d), codes = nb * R8_BLOCK, pitch = r8_pitch(d);
-  uint8_t *rec = dst + row * pitch;
-  for (int64_t j = threadIdx.x; j < codes; j += 256) {
-    const float x = j < d ? r8_load<DT>(src, row * stride + j) : 0.f;
-    uint32_t top = __float_as_uint(x) & 0x7fffffffu;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      const uint32_t other = __shfl_xor(top, o, 64);
-      top = other > top ? other : top;
-    }
-    const uint32_t field = r8_field(top);
-    rec[j] = (uint8_t)(int8_t)r8_code(x, field);
-    if ((j & 31) == 0) rec[codes + (j >> 5)] = (uint8_t)field;
-    if (copy && j < d) copy[row * d + j] = f32_to_bf16_bits(x);
+// Row and piece of a flat task number: tasks run over the pieces of one row, then the next.  t / per_row as a product with a
+// 32-bit reciprocal, exact for t < 2^31 (multiplier = ceil(2^(31 + s) / per_row) with per_row <= 2^s).
+struct R8Split {
+  uint32_t per_row, mul;
+  int shift;
+  explicit R8Split(int64_t n) : per_row((uint32_t)n), mul(0), shift(0) {   // n >= 2
+    while ((1LL << shift) < n) ++shift;
+    mul = (uint32_t)(((1ULL << (31 + shift)) + (uint64_t)n - 1) / (uint64_t)n);
   }
-  for (int64_t j = codes + nb + threadIdx.x; j < pitch; j += 256) rec[j] = 0;
+  __device__ __forceinline__ uint32_t row(uint32_t t) const { return __umulhi(t, mul) >> (shift - 1); }
+};
+
+// 16 bytes at any element's address: rows may start anywhere, and the memory instructions take any alignment
+template <int ALIGN>
+struct __attribute__((packed, aligned(ALIGN))) R8Bytes16 {
+  uint32_t w[4];
+};
+template <int ALIGN>
+struct __attribute__((packed, aligned(ALIGN))) R8Bytes8 {
+  uint32_t w[2];
+};
+
+// largest of the 4 (8) neighbouring lanes that hold a block: lane permutations inside the vector unit, no LDS
+template <int LANES>
+__device__ __forceinline__ uint32_t r8_block_max(uint32_t x) {
+  auto with = [&](uint32_t y) { x = y > x ? y : x; };
+  with(__builtin_amdgcn_update_dpp(0, x, 0xB1, 0xf, 0xf, false));   // quad_perm [1, 0, 3, 2]
+  with(__builtin_amdgcn_update_dpp(0, x, 0x4E, 0xf, 0xf, false));   // quad_perm [2, 3, 0, 1]
+  if constexpr (LANES == 8) with(__builtin_amdgcn_update_dpp(0, x, 0x141, 0xf, 0xf, false));   // row_half_mirror
+  return x;
 }
 
-// dst[i, :] = cast(scale * values of record row_idx[i]); a row index outside the buffer gives a row of NaN.
-template <int DT>
+// A thread takes pieces of 16 source bytes (8 bf16 or 4 fp32 values), 4 or 8 neighbouring lanes a block of 32.  All loads are
+// requested before the first is used: none stands behind a branch (WHOLE: d is a multiple of the piece, so no piece crosses
+// the row's end; a piece past the task list or the row's end reads one that is inside and drops it).
+template <int DT, bool WHOLE>
+__global__ __launch_bounds__(256) void rows8_quantize_kernel(const void *__restrict__ src, int64_t stride, int64_t d, uint8_t *__restrict__ dst,
+                                                             uint16_t *__restrict__ copy, R8Split split, uint32_t n_tasks) {
+  constexpr int W = DT == SAE_BF16 ? 8 : 4, LANES = R8_BLOCK / W, U = 4, ES = DT == SAE_BF16 ? 2 : 4;
+  const int64_t nb = r8_blocks(d), codes = nb * R8_BLOCK, pitch = r8_pitch(d);
+  const uint32_t first = blockIdx.x * (256 * U) + threadIdx.x;
+  float x[U][W];
+  uint32_t row[U], col[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const uint32_t t = first + u * 256 < n_tasks ? first + u * 256 : n_tasks - 1;
+    row[u] = split.row(t);
+    col[u] = (t - row[u] * split.per_row) * W;
+    const char *at = reinterpret_cast<const char *>(src) + ((int64_t)row[u] * stride + (col[u] < d ? col[u] : 0)) * ES;
+    if (WHOLE || col[u] >= d || col[u] + W <= d) {
+      if (WHOLE || col[u] < d) {
+        const R8Bytes16<ES> q = *reinterpret_cast<const R8Bytes16<ES> *>(at);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if constexpr (DT == SAE_BF16) {
+            x[u][2 * e] = __uint_as_float(q.w[e] << 16);
+            x[u][2 * e + 1] = __uint_as_float(q.w[e] & 0xffff0000u);
+          } else {
+            x[u][e] = __uint_as_float(q.w[e]);
+          }
+        }
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < W; ++e) x[u][e] = col[u] + e < d ? r8_load<DT>(at, e) : 0.f;
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    uint32_t top = 0u;
+#pragma unroll
+    for (int e = 0; e < W; ++e) {
+      x[u][e] = col[u] < d ? x[u][e] : 0.f;
+      const uint32_t m = __float_as_uint(x[u][e]) & 0x7fffffffu;
+      top = m > top ? m : top;
+    }
+    const uint32_t field = r8_field(r8_block_max<LANES>(top));
+    if (first + u * 256 >= n_tasks) continue;
+    uint8_t *rec = dst + (int64_t)row[u] * pitch;
+    uint32_t packed[W / 4];
+#pragma unroll
+    for (int e = 0; e < W; e += 4) packed[e / 4] = r8_codes(&x[u][e], field);
+    if constexpr (W == 8) *reinterpret_cast<uint2 *>(rec + col[u]) = make_uint2(packed[0], packed[W / 4 - 1]);
+    else *reinterpret_cast<uint32_t *>(rec + col[u]) = packed[0];
+    const int in_block = (int)(col[u] & 31) / W;
+    if (in_block == 0) rec[codes + (col[u] >> 5)] = (uint8_t)field;
+    if (col[u] >= codes - R8_BLOCK)   // the last block's lanes fill the record up
+      for (int64_t j = codes + nb + in_block; j < pitch; j += LANES) rec[j] = 0;
+    if constexpr (DT == SAE_F32) {
+      if (copy) {
+        uint16_t *c = copy + (int64_t)row[u] * d + col[u];
+        if (WHOLE ? col[u] < d : col[u] + 4 <= d) {
+          R8Bytes8<2> o;
+          o.w[0] = pack_bf16x2(x[u][0], x[u][1]);
+          o.w[1] = pack_bf16x2(x[u][2], x[u][3]);
+          *reinterpret_cast<R8Bytes8<2> *>(c) = o;
+        } else if constexpr (!WHOLE) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (col[u] + e < d) c[e] = f32_to_bf16_bits(x[u][e]);
+        }
+      }
+    }
+  }
+}
+
+// dst[i, :] = cast(scale * values of record row_idx[i]); a row index outside the buffer gives a row of NaN.  A thread takes
+// pieces of 16 bytes of the output (8 bf16 or 4 fp32 values); loads as above (WHOLE, and nothing behind a branch: a thread
+// past the task list reads the last piece again, an index outside the buffer reads row 0, and both drop what they read).
+template <int DT, bool IDX, bool WHOLE>
 __global__ __launch_bounds__(256) void rows8_gather_kernel(const uint8_t *__restrict__ rows, const int64_t *__restrict__ row_idx,
-                                                           int64_t n_src, int64_t d, float scale, void *__restrict__ dst) {
-  const int64_t i = blockIdx.x, r = row_idx ? row_idx[i] : i, codes = r8_blocks(d) * R8_BLOCK;
-  const bool ok = r >= 0 && r < n_src;
-  const uint8_t *rec = rows + (ok ? r : 0) * r8_pitch(d);
-  for (int64_t j = threadIdx.x; j < d; j += 256) {
-    const float x = ok ? r8_value(rec, codes, j) : __uint_as_float(0x7fc00000u);
-    r8_store<DT>(dst, i * d + j, x * scale);
+                                                           int64_t n_src, int64_t d, float scale, void *__restrict__ dst, R8Split split,
+                                                           uint32_t n_tasks) {
+  constexpr int W = DT == SAE_BF16 ? 8 : 4, U = 4, ES = DT == SAE_BF16 ? 2 : 4;
+  const int64_t codes = r8_blocks(d) * R8_BLOCK, pitch = r8_pitch(d);
+  const uint32_t first = blockIdx.x * (256 * U) + threadIdx.x;
+  uint32_t row[U], col[U], packed[U][W / 4], field[U];
+  int64_t r[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const uint32_t t = first + u * 256 < n_tasks ? first + u * 256 : n_tasks - 1;
+    row[u] = split.row(t);
+    col[u] = (t - row[u] * split.per_row) * W;
+    r[u] = IDX ? row_idx[row[u]] : (int64_t)row[u];
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const bool inside = r[u] >= 0 && r[u] < n_src;
+    const uint8_t *rec = rows + (inside ? r[u] : 0) * pitch;
+    if constexpr (W == 8) {
+      const uint2 q = *reinterpret_cast<const uint2 *>(rec + col[u]);
+      packed[u][0] = inside ? q.x : 0u;
+      packed[u][W / 4 - 1] = inside ? q.y : 0u;
+    } else {
+      const uint32_t q = *reinterpret_cast<const uint32_t *>(rec + col[u]);
+      packed[u][0] = inside ? q : 0u;
+    }
+    const uint32_t q = rec[codes + (col[u] >> 5)];
+    field[u] = inside ? q : 255u;   // 0 * inf: NaN
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u) asm volatile("" : "+v"(packed[u][0]));   // the loads stay up here, before the branches
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    if (first + u * 256 >= n_tasks || col[u] >= d) continue;
+    const float step = __uint_as_float(field[u] << 23);
+    float x[W];
+#pragma unroll
+    for (int e = 0; e < W; ++e) x[e] = (float)(int8_t)(packed[u][e / 4] >> (8 * (e % 4))) * step * scale;
+    char *at = reinterpret_cast<char *>(dst) + ((int64_t)row[u] * d + col[u]) * ES;
+    if (WHOLE || col[u] + W <= d) {
+      R8Bytes16<ES> o;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if constexpr (DT == SAE_BF16) o.w[e] = pack_bf16x2(x[2 * e], x[2 * e + 1]);
+        else o.w[e] = __float_as_uint(x[e]);
+      }
+      *reinterpret_cast<R8Bytes16<ES> *>(at) = o;
+    } else {
+#pragma unroll
+      for (int e = 0; e < W; ++e)
+        if (col[u] + e < d) r8_store<DT>(at, e, x[e]);
+    }
   }
 }
 
@@ -279,15 +417,25 @@ extern "C" int sae_rows8_quantize(const void *src, int src_dtype, int64_t n, int
   SAE_REQUIRE(src && rows, SAE_ERR_INVALID_ARG, "rows8_quantize: null pointer");
   SAE_REQUIRE(n > 0 && d > 0 && src_stride >= 0, SAE_ERR_INVALID_ARG, "rows8_quantize: bad sizes");
   SAE_REQUIRE(src_dtype == SAE_F32 || src_dtype == SAE_BF16, SAE_ERR_INVALID_ARG, "rows8_quantize: bad dtype %d", src_dtype);
+  SAE_REQUIRE(!bf16_copy || src_dtype == SAE_F32, SAE_ERR_INVALID_ARG, "rows8_quantize: a bf16 source is its own copy");
   SAE_REQUIRE(n < (1LL << 31) && d < (1LL << 30), SAE_ERR_UNSUPPORTED, "rows8_quantize: size too large");
   SAE_REQUIRE(((uintptr_t)rows & 15) == 0, SAE_ERR_INVALID_ARG, "rows8_quantize: rows must be 16-byte aligned");
-  hipStream_t st = (hipStream_t)stream;
-  uint8_t *out = reinterpret_cast<uint8_t *>(rows);
-  uint16_t *copy = reinterpret_cast<uint16_t *>(bf16_copy);
-  if (src_dtype == SAE_BF16)
-    hipLaunchKernelGGL(rows8_quantize_kernel<SAE_BF16>, dim3((unsigned)n), dim3(256), 0, st, src, src_stride, d, out, copy);
-  else
-    hipLaunchKernelGGL(rows8_quantize_kernel<SAE_F32>, dim3((unsigned)n), dim3(256), 0, st, src, src_stride, d, out, copy);
+  const int width = src_dtype == SAE_BF16 ? 8 : 4, size = src_dtype == SAE_BF16 ? 2 : 4;
+  const R8Split split(r8_blocks(d) * (R8_BLOCK / width));
+  const int64_t rows_per_launch = (1LL << 30) / split.per_row;   // task numbers stay below 2^31
+  for (int64_t r0 = 0; r0 < n; r0 += rows_per_launch) {
+    const int64_t m = n - r0 < rows_per_launch ? n - r0 : rows_per_launch, tasks = m * split.per_row;
+    const dim3 grid((unsigned)((tasks + 1023) / 1024));
+    const void *in = reinterpret_cast<const char *>(src) + r0 * src_stride * size;
+    uint8_t *out = reinterpret_cast<uint8_t *>(rows) + r0 * r8_pitch(d);
+    uint16_t *copy = bf16_copy ? reinterpret_cast<uint16_t *>(bf16_copy) + r0 * d : nullptr;
+#define SAE_R8_QUANTIZE(DT, WHOLE)                                                                                              \
+  hipLaunchKernelGGL((rows8_quantize_kernel<DT, WHOLE>), grid, dim3(256), 0, (hipStream_t)stream, in, src_stride, d, out, copy, split, \
+                     (uint32_t)tasks)
+    if (src_dtype == SAE_BF16) { if (d % width == 0) SAE_R8_QUANTIZE(SAE_BF16, true); else SAE_R8_QUANTIZE(SAE_BF16, false); }
+    else { if (d % width == 0) SAE_R8_QUANTIZE(SAE_F32, true); else SAE_R8_QUANTIZE(SAE_F32, false); }
+#undef SAE_R8_QUANTIZE
+  }
   return check_launch("rows8_quantize");
 }
 
@@ -300,12 +448,25 @@ extern "C" int sae_rows8_gather(const void *rows, const int64_t *row_idx, int64_
   SAE_REQUIRE(dst_dtype == SAE_F32 || dst_dtype == SAE_BF16, SAE_ERR_INVALID_ARG, "rows8_gather: bad dtype %d", dst_dtype);
   SAE_REQUIRE(n_rows < (1LL << 31) && d < (1LL << 30), SAE_ERR_UNSUPPORTED, "rows8_gather: size too large");
   SAE_REQUIRE(((uintptr_t)rows & 15) == 0, SAE_ERR_INVALID_ARG, "rows8_gather: rows must be 16-byte aligned");
-  hipStream_t st = (hipStream_t)stream;
-  const uint8_t *in = reinterpret_cast<const uint8_t *>(rows);
-  if (dst_dtype == SAE_BF16)
-    hipLaunchKernelGGL(rows8_gather_kernel<SAE_BF16>, dim3((unsigned)n_rows), dim3(256), 0, st, in, row_idx, n_src_rows, d, (float)scale, dst);
-  else
-    hipLaunchKernelGGL(rows8_gather_kernel<SAE_F32>, dim3((unsigned)n_rows), dim3(256), 0, st, in, row_idx, n_src_rows, d, (float)scale, dst);
+  const int width = dst_dtype == SAE_BF16 ? 8 : 4, size = dst_dtype == SAE_BF16 ? 2 : 4;
+  const R8Split split(r8_blocks(d) * (R8_BLOCK / width));
+  const int64_t rows_per_launch = (1LL << 30) / split.per_row;   // task numbers stay below 2^31
+  for (int64_t r0 = 0; r0 < n_rows; r0 += rows_per_launch) {
+    const int64_t m = n_rows - r0 < rows_per_launch ? n_rows - r0 : rows_per_launch, tasks = m * split.per_row;
+    const dim3 grid((unsigned)((tasks + 1023) / 1024));
+    const uint8_t *in = reinterpret_cast<const uint8_t *>(rows) + (row_idx ? 0 : r0 * r8_pitch(d));
+    const int64_t *idx = row_idx ? row_idx + r0 : nullptr;
+    void *out = reinterpret_cast<char *>(dst) + r0 * d * size;
+#define SAE_R8_GATHER(DT, IDX, WHOLE)                                                                                         \
+  hipLaunchKernelGGL((rows8_gather_kernel<DT, IDX, WHOLE>), grid, dim3(256), 0, (hipStream_t)stream, in, idx, IDX ? n_src_rows : m, d, \
+                     (float)scale, out, split, (uint32_t)tasks)
+#define SAE_R8_GATHER_TYPE(DT)                                                                        \
+  if (idx) { if (d % width == 0) SAE_R8_GATHER(DT, true, true); else SAE_R8_GATHER(DT, true, false); } \
+  else { if (d % width == 0) SAE_R8_GATHER(DT, false, true); else SAE_R8_GATHER(DT, false, false); }
+    if (dst_dtype == SAE_BF16) { SAE_R8_GATHER_TYPE(SAE_BF16) } else { SAE_R8_GATHER_TYPE(SAE_F32) }
+#undef SAE_R8_GATHER_TYPE
+#undef SAE_R8_GATHER
+  }
   return check_launch("rows8_gather");
 }
 

@@ -1390,7 +1390,7 @@ def gather_rows(src, row_idx: torch.Tensor, out_dtype: Optional[torch.dtype] = N
 def quantize_rows(x: torch.Tensor, out: Optional[torch.Tensor] = None, bf16_copy: bool = False):
     """`Rows8` of x [n, d] (fp32 / bf16; rows may lie any distance apart, their values side by side).  `out`: uint8
     [n, rows8_pitch(d)] to write the records into (rows of a buffer).  With `bf16_copy` also returns bf16(x), the operand a
-    bf16 product reads, from the same pass: -> (Rows8, [n, d] bf16); of a contiguous bf16 x that is x itself."""
+    bf16 product reads, from the same pass: -> (Rows8, [n, d] bf16); of a bf16 x that is x itself, made contiguous."""
     if not x.is_cuda:
         raise RuntimeError(f"x must live on the GPU (got {x.device}); the HIP path has no CPU fallback")
     if x.ndim != 2 or x.shape[1] < 1:
@@ -1410,11 +1410,11 @@ def quantize_rows(x: torch.Tensor, out: Optional[torch.Tensor] = None, bf16_copy
         raise ValueError(f"out has {len(rows)} records for {n} rows")
     copy = None
     if bf16_copy:
-        copy = x if x.dtype == torch.bfloat16 and x.is_contiguous() else torch.empty(n, d, dtype=torch.bfloat16, device=x.device)
+        copy = x.contiguous() if x.dtype == torch.bfloat16 else torch.empty(n, d, dtype=torch.bfloat16, device=x.device)
     if n:
         with _timed("rows8_quantize"), _on_device(x):
             check(_lib.load().sae_rows8_quantize(x.data_ptr(), dt, n, d, x.stride(0), out.data_ptr(),
-                                                 None if copy is x else _ptr(copy), _stream(x)), "rows8_quantize")
+                                                 _ptr(copy) if dt == SAE_F32 else None, _stream(x)), "rows8_quantize")
     return (rows, copy) if bf16_copy else rows
 
 

@@ -43,7 +43,7 @@ def test_entry_points_refuse_before_any_launch(pkg):
     P = 1 << 20
     quant = lambda src=P, dt=0, n=4, d=40, stride=40, rows=P, copy=None: lib.sae_rows8_quantize(src, dt, n, d, stride, rows, copy, None)  # noqa: E731
     assert quant(src=None) == -1 and quant(rows=None) == -1 and quant(n=0) == -1 and quant(d=0) == -1 and quant(stride=-1) == -1
-    assert quant(dt=2) == -1 and quant(rows=P + 8) == -1 and quant(n=1 << 31) == -2 and quant(d=1 << 30) == -2
+    assert quant(dt=2) == -1 and quant(dt=1, copy=P) == -1 and quant(rows=P + 8) == -1 and quant(n=1 << 31) == -2 and quant(d=1 << 30) == -2
     gather = lambda rows=P, idx=P, ns=4, n=4, d=40, dst=P, dt=0: lib.sae_rows8_gather(rows, idx, ns, n, d, dst, dt, 1.0, None)  # noqa: E731
     assert gather(rows=None) == -1 and gather(dst=None) == -1 and gather(ns=0) == -1 and gather(n=0) == -1 and gather(d=-1) == -1
     assert gather(idx=None, n=5) == -1 and gather(dt=2) == -1 and gather(rows=P + 1) == -1 and gather(n=1 << 31) == -2
