@@ -515,11 +515,19 @@ int sae_rows8_quantize(const void *src, int src_dtype, int64_t n, int64_t d, int
 int sae_rows8_gather(const void *rows, const int64_t *row_idx, int64_t n_src_rows, int64_t n_rows, int64_t d, void *dst,
                      int dst_dtype, double scale, void *stream);
 
-/* dst[c, r] = src[r, c] for r < rows and 0 for rows <= r < dst_pitch: an operand whose token axis has become the contiguous
- * one, filled up to the contraction lengths the GEMM entry points take.  src [rows, cols] in SAE_F32, SAE_BF16 or SAE_ROWS8
- * (records of cols values), dst [cols, dst_pitch] in SAE_F32 or SAE_BF16 (fp32 to bf16 rounds to nearest even). */
-int sae_transpose_padded(const void *src, int src_dtype, int64_t rows, int64_t cols, void *dst, int dst_dtype, int64_t dst_pitch,
-                         void *stream);
+/* dst[c, r] = src[r, c] for r < rows and 0 for rows <= r < dst_pitch (a multiple of 8): an operand whose token axis has become
+ * the contiguous one, filled up to a contraction length the GEMM entry points take.  src [rows, cols] in SAE_BF16 or SAE_ROWS8
+ * (records of cols values), dst bf16 [cols, dst_pitch]. */
+int sae_transpose_padded(const void *src, int src_dtype, int64_t rows, int64_t cols, void *dst, int64_t dst_pitch, void *stream);
+
+/* out[i, j] = sum_t left[t, i] right[t, j] for left [tokens, m] and right [tokens, n], each in SAE_F32, SAE_BF16 or SAE_ROWS8: a
+ * weight gradient over the token axis (dW = d(pre)^T x, acts^T d(recon)) whose saved side may be held in records.  Any widths
+ * and token counts; records enter exactly.  With an fp32 operand fp32 products are formed and out is SAE_F32; otherwise bf16
+ * products with fp32 sums, out in SAE_F32 or SAE_BF16.  n_slices > 1 cuts the tokens (slabs of 64, or 32 with an fp32 operand;
+ * at most one slice per slab) for products with few outputs: partials is then fp32 [n_slices, m, n], summed in token order.
+ * Made for products that are small or that no slab divides; sae_gemm_bf16 runs large ones faster. */
+int sae_gemm_over_tokens(const void *left, int left_dtype, const void *right, int right_dtype, int64_t tokens, int64_t m, int64_t n,
+                         void *out, int out_dtype, int64_t n_slices, float *partials, void *stream);
 
 /* sae_sparse_grad_rows for a dense operand held as records (any d): out[f, :] = sum over the slots s of feature f of
  * coef[s] * values of record slot_tok[s]; rows without slots are written as zeros; bias_out (nullable) [F].  n_slots: the

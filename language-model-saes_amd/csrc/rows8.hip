@@ -48,12 +48,6 @@ __device__ __forceinline__ void r8_store(void *dst, int64_t i, float x) {
   else reinterpret_cast<float *>(dst)[i] = x;
 }
 
-// element j of a record
-__device__ __forceinline__ float r8_value(const uint8_t *rec, int64_t codes, int64_t j) {
-  const float step = __uint_as_float((uint32_t)rec[codes + (j >> 5)] << 23);
-  return (float)(int8_t)rec[j] * step;
-}
-
 // Row and piece of a flat task number: tasks run over the pieces of one row, then the next.  t / per_row as a product with a
 // 32-bit reciprocal, exact for t < 2^31 (multiplier = ceil(2^(31 + s) / per_row) with per_row <= 2^s).
 struct R8Split {
@@ -220,26 +214,78 @@ __global__ __launch_bounds__(256) void rows8_gather_kernel(const uint8_t *__rest
   }
 }
 
-// dst[c, r] = src[r, c] for r < rows, 0 for rows <= r < dst_pitch, through a 64 x 64 tile.
-template <int SRC, int DT>
-__global__ __launch_bounds__(256) void transpose_padded_kernel(const void *__restrict__ src, int64_t rows, int64_t cols, void *__restrict__ dst,
+// dst[c, r] = bf16(src[r, c]) for r < rows, 0 for rows <= r < dst_pitch: 128 rows x 64 columns per workgroup.  A thread takes 8
+// columns of two rows at a time and writes them to LDS as pairs of rows, column by column (33-word columns: a wave's words
+// fall on 64 banks), so that an output row leaves in whole 16-byte stores of 8 tokens.
+template <int SRC>
+__global__ __launch_bounds__(256) void transpose_padded_kernel(const void *__restrict__ src, int64_t rows, int64_t cols, uint16_t *__restrict__ dst,
                                                                int64_t dst_pitch) {
-  __shared__ float tile[64][65];
-  const int64_t r0 = (int64_t)blockIdx.y * 64, c0 = (int64_t)blockIdx.x * 64;
-  const int tx = threadIdx.x & 63, ty = threadIdx.x >> 6;
-  for (int i = ty; i < 64; i += 4) {
-    const int64_t r = r0 + i, c = c0 + tx;
-    float x = 0.f;
-    if (r < rows && c < cols) {
-      if constexpr (SRC == SAE_ROWS8) x = r8_value(reinterpret_cast<const uint8_t *>(src) + r * r8_pitch(cols), r8_blocks(cols) * R8_BLOCK, c);
-      else x = r8_load<SRC>(src, r * cols + c);
+  __shared__ uint32_t tile[2][64 * 33];
+  const int64_t r0 = (int64_t)blockIdx.y * 128, c0 = (int64_t)blockIdx.x * 64;
+  const int group = threadIdx.x & 7, pair = threadIdx.x >> 3;   // 8 columns, and 32 pairs of rows
+  const int64_t col = c0 + group * 8, end = SRC == SAE_ROWS8 ? r8_blocks(cols) * R8_BLOCK : cols;
+  const size_t pitch = dense_row_bytes<SRC>(cols);
+  const uint8_t *base = reinterpret_cast<const uint8_t *>(src);
+  u32x4 q[2][2];
+  uint32_t field[2][2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int64_t r = r0 + h * 64 + pair * 2 + i;
+      const uint8_t *row = base + (size_t)(r < rows ? r : rows - 1) * pitch;
+      const bool in = r < rows && col < end;
+      if constexpr (SRC == SAE_ROWS8) {
+        const uint2 w = *reinterpret_cast<const uint2 *>(row + (col < end ? col : 0));
+        field[h][i] = in ? (uint32_t)row[end + ((col < end ? col : 0) >> 5)] : 0u;
+        q[h][i] = in ? u32x4{w.x, w.y, 0u, 0u} : u32x4{0u, 0u, 0u, 0u};
+      } else {
+        q[h][i] = u32x4{0u, 0u, 0u, 0u};
+        if (in) {
+          if (col + 8 <= cols) {
+            const R8Bytes16<2> w = *reinterpret_cast<const R8Bytes16<2> *>(row + col * 2);
+            q[h][i] = u32x4{w.w[0], w.w[1], w.w[2], w.w[3]};
+          } else {
+            uint32_t e[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) e[j] = col + j < cols ? (uint32_t)reinterpret_cast<const uint16_t *>(row)[col + j] : 0u;
+            q[h][i] = u32x4{e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16};
+          }
+        }
+      }
     }
-    tile[i][tx] = x;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    uint32_t even[4], odd[4];   // the two rows' 8 values as bf16 pairs of columns
+    if constexpr (SRC == SAE_ROWS8) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const float step = __uint_as_float(field[h][i] << 23);
+        const uint32_t w[2] = {q[h][i].x, q[h][i].y};
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          (i ? odd : even)[j] = pack_bf16x2((float)(int8_t)(w[j >> 1] >> (16 * (j & 1))) * step, (float)(int8_t)(w[j >> 1] >> (16 * (j & 1) + 8)) * step);
+      }
+    } else {
+      even[0] = q[h][0].x; even[1] = q[h][0].y; even[2] = q[h][0].z; even[3] = q[h][0].w;
+      odd[0] = q[h][1].x; odd[1] = q[h][1].y; odd[2] = q[h][1].z; odd[3] = q[h][1].w;
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      tile[h][(group * 8 + 2 * j) * 33 + pair] = (even[j] & 0xffffu) | (odd[j] << 16);
+      tile[h][(group * 8 + 2 * j + 1) * 33 + pair] = (even[j] >> 16) | (odd[j] & 0xffff0000u);
+    }
   }
   __syncthreads();
-  for (int i = ty; i < 64; i += 4) {
-    const int64_t c = c0 + i, r = r0 + tx;
-    if (c < cols && r < dst_pitch) r8_store<DT>(dst, c * dst_pitch + r, tile[tx][i]);
+  const int part = threadIdx.x & 15, first = threadIdx.x >> 4;   // 16 threads write the 128 tokens of one column
+  const int64_t r = r0 + part * 8;
+  if (r >= dst_pitch) return;   // the pitch is a multiple of 8
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const int c = first + 16 * k;
+    if (c0 + c >= cols) break;
+    const uint32_t *w = &tile[part >> 3][c * 33 + (part & 7) * 4];
+    *reinterpret_cast<u32x4 *>(dst + (c0 + c) * dst_pitch + r) = u32x4{w[0], w[1], w[2], w[3]};
   }
 }
 
@@ -470,28 +516,21 @@ extern "C" int sae_rows8_gather(const void *rows, const int64_t *row_idx, int64_
   return check_launch("rows8_gather");
 }
 
-extern "C" int sae_transpose_padded(const void *src, int src_dtype, int64_t rows, int64_t cols, void *dst, int dst_dtype, int64_t dst_pitch,
-                                    void *stream) {
+extern "C" int sae_transpose_padded(const void *src, int src_dtype, int64_t rows, int64_t cols, void *dst, int64_t dst_pitch, void *stream) {
   using namespace sae;
   SAE_REQUIRE(src && dst, SAE_ERR_INVALID_ARG, "transpose_padded: null pointer");
-  SAE_REQUIRE(rows > 0 && cols > 0 && dst_pitch >= rows, SAE_ERR_INVALID_ARG, "transpose_padded: bad sizes");
-  SAE_REQUIRE(src_dtype == SAE_F32 || src_dtype == SAE_BF16 || src_dtype == SAE_ROWS8, SAE_ERR_INVALID_ARG, "transpose_padded: bad dtype %d", src_dtype);
-  SAE_REQUIRE(dst_dtype == SAE_F32 || dst_dtype == SAE_BF16, SAE_ERR_INVALID_ARG, "transpose_padded: bad dtype %d", dst_dtype);
-  const int64_t gy = (dst_pitch + 63) / 64, gx = (cols + 63) / 64;
-  SAE_REQUIRE(gy <= 65535 && gx < (1LL << 31), SAE_ERR_UNSUPPORTED, "transpose_padded: %lld rows, at most %d", (long long)dst_pitch, 65535 * 64);
-  hipStream_t st = (hipStream_t)stream;
+  SAE_REQUIRE(rows > 0 && cols > 0 && dst_pitch >= rows && dst_pitch % 8 == 0, SAE_ERR_INVALID_ARG, "transpose_padded: bad sizes");
+  SAE_REQUIRE(src_dtype == SAE_BF16 || src_dtype == SAE_ROWS8, SAE_ERR_INVALID_ARG, "transpose_padded: bad dtype %d", src_dtype);
+  SAE_REQUIRE(((uintptr_t)dst & 15) == 0 && (src_dtype != SAE_ROWS8 || ((uintptr_t)src & 15) == 0), SAE_ERR_INVALID_ARG,
+              "transpose_padded: 16-byte alignment required");
+  const int64_t gy = (dst_pitch + 127) / 128, gx = (cols + 63) / 64;
+  SAE_REQUIRE(gy <= 65535 && cols < (1LL << 30), SAE_ERR_UNSUPPORTED, "transpose_padded: %lld rows, at most %d", (long long)dst_pitch, 65535 * 128);
   const dim3 grid((unsigned)gx, (unsigned)gy);
-#define SAE_TP(S, D) hipLaunchKernelGGL((transpose_padded_kernel<S, D>), grid, dim3(256), 0, st, src, rows, cols, dst, dst_pitch)
-  if (dst_dtype == SAE_BF16) {
-    if (src_dtype == SAE_ROWS8) SAE_TP(SAE_ROWS8, SAE_BF16);
-    else if (src_dtype == SAE_BF16) SAE_TP(SAE_BF16, SAE_BF16);
-    else SAE_TP(SAE_F32, SAE_BF16);
-  } else {
-    if (src_dtype == SAE_ROWS8) SAE_TP(SAE_ROWS8, SAE_F32);
-    else if (src_dtype == SAE_BF16) SAE_TP(SAE_BF16, SAE_F32);
-    else SAE_TP(SAE_F32, SAE_F32);
-  }
-#undef SAE_TP
+  uint16_t *out = reinterpret_cast<uint16_t *>(dst);
+  if (src_dtype == SAE_ROWS8)
+    hipLaunchKernelGGL(transpose_padded_kernel<SAE_ROWS8>, grid, dim3(256), 0, (hipStream_t)stream, src, rows, cols, out, dst_pitch);
+  else
+    hipLaunchKernelGGL(transpose_padded_kernel<SAE_BF16>, grid, dim3(256), 0, (hipStream_t)stream, src, rows, cols, out, dst_pitch);
   return check_launch("transpose_padded");
 }
 

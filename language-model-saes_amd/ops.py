@@ -15,6 +15,10 @@ from . import _lib
 from ._lib import SAE_BF16, SAE_F32, SAE_ROWS8, check
 
 
+# handle of a device's current stream; a build of torch without a GPU side has none to hand out
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
 def _stream(t: torch.Tensor) -> int:
     return torch.cuda.current_stream(t.device).cuda_stream
 
@@ -190,6 +194,20 @@ class _on_device:
         if self.prev != self.index:
             torch.cuda.set_device(self.prev)
         return False
+
+
+def _launch(name: str, t: torch.Tensor, fn, *args) -> None:
+    """One library call on `t`'s device and that device's current stream (appended as the last argument).  Small calls are
+    as long as their host side: with no timer installed and the device current already, nothing stands around the call, and
+    the stream's handle is taken without a Stream object around it (1 us of 8)."""
+    index = t.device.index
+    if _timer is None and torch.cuda.current_device() == index:
+        rc = fn(*args, _raw_stream(index))
+    else:
+        with _on_device(t), _timed(name):
+            rc = fn(*args, _raw_stream(index))
+    if rc:
+        check(rc, name)
 
 
 def _req_rows8(q: Rows8, name: str):
@@ -1412,9 +1430,8 @@ def quantize_rows(x: torch.Tensor, out: Optional[torch.Tensor] = None, bf16_copy
     if bf16_copy:
         copy = x.contiguous() if x.dtype == torch.bfloat16 else torch.empty(n, d, dtype=torch.bfloat16, device=x.device)
     if n:
-        with _timed("rows8_quantize"), _on_device(x):
-            check(_lib.load().sae_rows8_quantize(x.data_ptr(), dt, n, d, x.stride(0), out.data_ptr(),
-                                                 _ptr(copy) if dt == SAE_F32 else None, _stream(x)), "rows8_quantize")
+        _launch("rows8_quantize", x, _lib.load().sae_rows8_quantize, x.data_ptr(), dt, n, d, x.stride(0), out.data_ptr(),
+                _ptr(copy) if dt == SAE_F32 else None)
     return (rows, copy) if bf16_copy else rows
 
 
@@ -1436,9 +1453,8 @@ def _read_rows8(src: Rows8, row_idx: Optional[torch.Tensor], out_dtype: Optional
         return out
     if len(src) == 0:
         raise ValueError("rows asked of an empty buffer")
-    with _timed("rows8_gather"), _on_device(src.data):
-        check(_lib.load().sae_rows8_gather(src.data.data_ptr(), _ptr(row_idx), len(src), n, d, out.data_ptr(), dt, float(scale),
-                                           _stream(src.data)), "rows8_gather")
+    _launch("rows8_gather", src.data, _lib.load().sae_rows8_gather, src.data.data_ptr(), _ptr(row_idx), len(src), n, d,
+            out.data_ptr(), dt, float(scale))
     return out
 
 
@@ -1460,10 +1476,9 @@ def _rows8_grad_rows(fi: FeatureIndex, coef: torch.Tensor, rows: Rows8, F: int, 
     lib = _lib.load()
     nbytes = lib.sae_rows8_grad_rows_workspace_bytes(n_slots, d)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=rows.device)
-    with _timed("sparse_grad_rows[rows8 dense]"), _on_device(coef):
-        check(lib.sae_rows8_grad_rows(fi.feat_ptr.data_ptr(), fi.feat_slot.data_ptr(), fi.slot_tok.data_ptr(), coef.data_ptr(),
-                                      rows.data.data_ptr(), out.data_ptr(), _ptr(bias), F, d, n_slots, ws.data_ptr(), nbytes,
-                                      _stream(coef)), "rows8_grad_rows")
+    _launch("sparse_grad_rows[rows8 dense]", coef, lib.sae_rows8_grad_rows, fi.feat_ptr.data_ptr(), fi.feat_slot.data_ptr(),
+            fi.slot_tok.data_ptr(), coef.data_ptr(), rows.data.data_ptr(), out.data_ptr(), _ptr(bias), F, d, n_slots,
+            ws.data_ptr(), nbytes)
 
 
 def restore_rows(src: Rows8, out_dtype: torch.dtype = torch.bfloat16, out: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -1471,15 +1486,35 @@ def restore_rows(src: Rows8, out_dtype: torch.dtype = torch.bfloat16, out: Optio
     return _read_rows8(src, None, out_dtype, 1.0, out)
 
 
-def _transpose_padded(src, out_dtype: torch.dtype, pitch: int) -> torch.Tensor:
-    """[cols, pitch] = src^T (fp32, bf16 or `Rows8` [rows, cols]), zeros behind the rows-th."""
+def _transpose_padded(src, pitch: int) -> torch.Tensor:
+    """bf16 [cols, pitch] = src^T (bf16 or `Rows8` [rows, cols]), zeros behind the rows-th."""
     t = src.data if isinstance(src, Rows8) else src
     rows, cols = src.shape
-    out = torch.empty(cols, pitch, dtype=out_dtype, device=t.device)
-    with _timed("transpose_padded"):
-        check(_lib.load().sae_transpose_padded(t.data_ptr(), SAE_ROWS8 if t is not src else _dt(t), rows, cols, out.data_ptr(),
-                                               _dt(out), pitch, _stream(t)), "transpose_padded")
+    out = torch.empty(cols, pitch, dtype=torch.bfloat16, device=t.device)
+    _launch("transpose_padded", t, _lib.load().sae_transpose_padded, t.data_ptr(), _operand_dt(src), rows, cols, out.data_ptr(), pitch)
     return out
+
+
+def _operand_dt(t) -> int:
+    return SAE_ROWS8 if isinstance(t, Rows8) else _dt(t)
+
+
+OVER_TOKENS_FLOP = 3.4e10
+
+
+def _over_tokens_slices(tokens: int, m: int, n: int, wide: bool) -> int:
+    """Into how many slices of the tokens the product of 64 x 64 tiles is cut: the least estimated time.  A slab (64 tokens, 32
+    in fp32) takes a workgroup about 1 us, longer once more than two of them share every CU; joining costs a launch of 4 us,
+    0.3 us per slice and 8 bytes per output and slice at 4 TB/s.  Measured at 4096 x 1024 x 768 (192 tiles): 46 us uncut, 28 in
+    4 slices, 39 in 16; 8192 x 64 x 64 (one tile): 73 us uncut, 15 in 16 slices, 17 in 32; 1000 x 1003 x 521: 24 uncut, 17 in
+    4; 2048 x 2048 x 768: 29 uncut, 30 in two; fp32 4096 x 1024 x 768: 153 uncut, 77 in 4, 85 in 16."""
+    slabs, tiles = -(-tokens // (32 if wide else 64)), -(-m // 64) * -(-n // 64)
+    best, best_us = 1, slabs * max(1.0, tiles / 512)
+    for s in (2, 4, 8, 16, 32):
+        us = -(-slabs // s) * max(1.0, tiles * s / 512) + 4.0 + s * (m * n * 2e-6 + 0.3)
+        if s <= slabs and us < best_us:
+            best, best_us = s, us
+    return best
 
 
 def gemm_over_tokens(left, right, out_dtype: torch.dtype = torch.float32) -> torch.Tensor:
@@ -1488,9 +1523,12 @@ def gemm_over_tokens(left, right, out_dtype: torch.dtype = torch.float32) -> tor
     bits are exact in bf16; with an fp32 operand the product is an fp32 product (and so is `out_dtype`), otherwise a bf16
     product with fp32 accumulation.
 
-    Rows held in 8 bits are read once, into a transposed bf16 (fp32) operand: their steps change along the contraction, so
-    the codes cannot enter the matrix cores as they are, and widening them inside the product's tiles would be done again for
-    every tile of the other side."""
+    Products of up to 34 GFLOP, and all fp32 ones, run on a kernel of 64 x 64 tiles that reads every operand as it lies; larger
+    ones on the GEMM kernel's 256 x 256 tiles, for which rows held in 8 bits (and operands that its slabs do not divide) are
+    first copied into a transposed bf16 operand: their steps change along the contraction, so codes cannot enter the matrix
+    cores as they are, and widening them inside that product's tiles would be done again for every tile of the other side.
+    Measured: 4096 x 2048 x 2048 (34 GFLOP) 89 us against 91, 4096 x 4096 x 768 68 against 86, 8192 x 2048 x 2048 169 against
+    112; fp32 4096 x 4096 x 768 0.26 ms against 1.04."""
     for name, t in (("left", left), ("right", right)):
         if isinstance(t, Rows8):
             _req_rows8(t, name)
@@ -1503,24 +1541,29 @@ def gemm_over_tokens(left, right, out_dtype: torch.dtype = torch.float32) -> tor
                          f"right {tuple(right.shape)} on {right.device}")
     if m < 1 or n < 1:
         raise ValueError("operands need at least one column")
-    wide = any(not isinstance(t, Rows8) and t.dtype == torch.float32 for t in (left, right))
+    left_dt, right_dt = _operand_dt(left), _operand_dt(right)
+    wide = SAE_F32 in (left_dt, right_dt)
     if out_dtype not in ((torch.float32,) if wide else (torch.float32, torch.bfloat16)):
         raise TypeError(f"out_dtype {out_dtype} of a product of {'fp32' if wide else 'bf16'} operands")
     dev = left.device
     if T == 0:
         return torch.zeros(m, n, dtype=out_dtype, device=dev)
+    if wide or 2.0 * T * m * n <= OVER_TOKENS_FLOP:
+        slices = _over_tokens_slices(T, m, n, wide)
+        out = torch.empty(m, n, dtype=out_dtype, device=dev)
+        part = torch.empty(slices * m * n, dtype=torch.float32, device=dev) if slices > 1 else None
+        lt, rt = left.data, right.data
+        _launch("gemm_over_tokens", lt, _lib.load().sae_gemm_over_tokens, lt.data_ptr(), left_dt, rt.data_ptr(), right_dt, T, m, n,
+                out.data_ptr(), _dt(out), slices, _ptr(part))
+        return out
+    pitch = -(-T // 64) * 64
+
+    def operand(t):
+        """(operand, whether it is stored [tokens, columns])"""
+        if not isinstance(t, Rows8) and T == pitch and t.shape[1] % 8 == 0 and t.data_ptr() % 16 == 0:
+            return t, True
+        return _transpose_padded(t, pitch), False
+
     with _on_device(left.data):
-        if wide:
-            pitch = -(-T // 32) * 32
-            return encoder_gemm(_transpose_padded(left, torch.float32, pitch), _transpose_padded(right, torch.float32, pitch),
-                                torch.float32)
-        pitch = -(-T // 64) * 64
-
-        def operand(t):
-            """(operand, whether it is stored [tokens, columns])"""
-            if not isinstance(t, Rows8) and T == pitch and t.shape[1] % 8 == 0 and t.data_ptr() % 16 == 0:
-                return t, True
-            return _transpose_padded(t, torch.bfloat16, pitch), False
-
         (a, a_k), (b, b_k) = operand(left), operand(right)
         return gemm(a, b, out_dtype, a_k_major=a_k, b_k_major=b_k)

@@ -221,13 +221,57 @@ def test_gemm_over_tokens(pkg, dev, T, m, n, left_kind):
         assert (np.abs(low - want) <= bound(lv, r, T) + 2.0**-8 * np.abs(want) + 1e-38).all()
 
 
-def test_gemm_over_tokens_of_float_operands_is_the_same_product(pkg, dev):
-    """Rows that 8 bits hold exactly: the product of the float rows, bit for bit."""
+@pytest.mark.parametrize("T,m,n", [(2049, 4100, 2055), (2112, 4096, 2048), (2500, 2056, 3600)])
+@pytest.mark.parametrize("left_kind", ["bf16", "rows8"])
+def test_large_products(pkg, dev, T, m, n, left_kind):
+    """Past the size that the 64 x 64 tiles take: tokens and widths that the GEMM kernel's slabs divide, or do not."""
     ops = pkg.ops
-    q = ops.quantize_rows(activations(256, 96, 11))
-    g = activations(256, 160, 12, torch.bfloat16)
-    assert torch.equal(ops.gemm_over_tokens(g, q), ops.gemm(g, ops.restore_rows(q), torch.float32, True, True))
-    assert torch.equal(ops.gemm_over_tokens(g, ops.restore_rows(q)), ops.gemm_over_tokens(g, q))
+    assert 2.0 * T * m * n > ops.OVER_TOKENS_FLOP
+    left, right = activations(T, m, 9, torch.bfloat16), ops.quantize_rows(activations(T, n, 10))
+    left = ops.quantize_rows(left) if left_kind == "rows8" else left
+    lv = (ops.restore_rows(left, torch.float32) if left_kind == "rows8" else left).double()
+    r = ops.restore_rows(right, torch.float32).double()
+    limit = 2.0 * T * 2.0**-24 * (lv.abs().t() @ r.abs()) + 1e-40
+    assert ((ops.gemm_over_tokens(left, right).double() - lv.t() @ r).abs() <= limit).all()
+    assert ((ops.gemm_over_tokens(right, left).double() - r.t() @ lv).abs() <= limit.t()).all()
+
+
+@pytest.mark.parametrize("wide", [False, True])
+@pytest.mark.parametrize("slices", [1, 2, 3, 7])
+def test_slices_of_the_tokens(pkg, dev, slices, wide):
+    """Any number of slices of whole slabs, the last one short, adds up to the same product."""
+    ops, lib = pkg.ops, pkg._lib.load()
+    T, m, n = 450, 70, 45
+    left = activations(T, m, 11, torch.float32 if wide else torch.bfloat16)
+    right = ops.quantize_rows(activations(T, n, 12))
+    out, part = torch.full((m, n), float("nan"), device=dev), torch.full((slices, m, n), float("nan"), device=dev)
+    pkg._lib.check(lib.sae_gemm_over_tokens(left.data_ptr(), 0 if wide else 1, right.data.data_ptr(), 2, T, m, n, out.data_ptr(), 0, slices,
+                                            part.data_ptr(), torch.cuda.current_stream().cuda_stream))
+    lv, r = doubles(left), doubles(ops.restore_rows(right, torch.float32))
+    assert (np.abs(doubles(out) - lv.T @ r) <= bound(lv, r, T)).all()
+
+
+def test_gemm_over_tokens_of_float_operands(pkg, dev):
+    """Any two operand types; rows that 8 bits hold exactly give the product of the float rows, bit for bit."""
+    ops = pkg.ops
+    left, right = ops.quantize_rows(activations(300, 76, 11)), ops.quantize_rows(activations(300, 100, 12))
+    forms = lambda q: (q, ops.restore_rows(q), ops.restore_rows(q, torch.float32))  # noqa: E731
+    low = [ops.gemm_over_tokens(a, b) for a in forms(left)[:2] for b in forms(right)[:2]]
+    wide = [ops.gemm_over_tokens(a, b) for a in forms(left) for b in forms(right) if torch.float32 in (getattr(a, "dtype", 0), getattr(b, "dtype", 0))]
+    assert len(low) == 4 and len(wide) == 5
+    for group in (low, wide):
+        for g in group[1:]:
+            assert torch.equal(g, group[0])
+
+
+def test_the_two_tilings_agree(pkg, dev, monkeypatch):
+    ops = pkg.ops
+    left, right = activations(256, 160, 13, torch.bfloat16), ops.quantize_rows(activations(256, 96, 14))
+    small = doubles(ops.gemm_over_tokens(left, right))
+    monkeypatch.setattr(ops, "OVER_TOKENS_FLOP", 0.0)
+    large = ops.gemm_over_tokens(left, right)
+    assert torch.equal(large, ops.gemm(left, ops.restore_rows(right), torch.float32, True, True))
+    assert (np.abs(small - doubles(large)) <= bound(doubles(left), doubles(ops.restore_rows(right, torch.float32)), 256)).all()
 
 
 def test_no_tokens(pkg, dev):

@@ -14,6 +14,14 @@ def test_pitch_of_nothing(pkg):
     assert lib.sae_rows8_pitch(0) == 0 and lib.sae_rows8_pitch(-4) == 0
 
 
+@pytest.mark.parametrize("tokens", [1, 64, 100, 4096, 131072])
+@pytest.mark.parametrize("m,n", [(1, 1), (64, 64), (1003, 521), (8192, 2048)])
+@pytest.mark.parametrize("wide", [False, True])
+def test_a_slice_holds_a_slab(pkg, tokens, m, n, wide):
+    s = pkg.ops._over_tokens_slices(tokens, m, n, wide)
+    assert 1 <= s <= -(-tokens // (32 if wide else 64))
+
+
 def test_rows8_holds_whole_records(pkg):
     R = pkg.Rows8
     ok = R(torch.zeros(3, 80, dtype=torch.uint8), 40)
@@ -47,9 +55,14 @@ def test_entry_points_refuse_before_any_launch(pkg):
     gather = lambda rows=P, idx=P, ns=4, n=4, d=40, dst=P, dt=0: lib.sae_rows8_gather(rows, idx, ns, n, d, dst, dt, 1.0, None)  # noqa: E731
     assert gather(rows=None) == -1 and gather(dst=None) == -1 and gather(ns=0) == -1 and gather(n=0) == -1 and gather(d=-1) == -1
     assert gather(idx=None, n=5) == -1 and gather(dt=2) == -1 and gather(rows=P + 1) == -1 and gather(n=1 << 31) == -2
-    tr = lambda src=P, dt=2, r=4, c=40, dst=P, odt=1, pitch=64: lib.sae_transpose_padded(src, dt, r, c, dst, odt, pitch, None)  # noqa: E731
-    assert tr(src=None) == -1 and tr(dst=None) == -1 and tr(r=0) == -1 and tr(pitch=3) == -1 and tr(dt=3) == -1 and tr(odt=2) == -1
-    assert tr(pitch=1 << 30) == -2
+    tr = lambda src=P, dt=2, r=4, c=40, dst=P, pitch=64: lib.sae_transpose_padded(src, dt, r, c, dst, pitch, None)  # noqa: E731
+    assert tr(src=None) == -1 and tr(dst=None) == -1 and tr(r=0) == -1 and tr(pitch=3) == -1 and tr(pitch=60) == -1 and tr(dt=0) == -1
+    assert tr(dst=P + 2) == -1 and tr(src=P + 8) == -1 and tr(pitch=1 << 30) == -2
+    ot = lambda l=P, ldt=1, r=P, rdt=2, T=100, m=8, n=8, out=P, odt=0, s=1, part=None: lib.sae_gemm_over_tokens(  # noqa: E731
+        l, ldt, r, rdt, T, m, n, out, odt, s, part, None)
+    assert ot(l=None) == -1 and ot(r=None) == -1 and ot(out=None) == -1 and ot(T=0) == -1 and ot(m=0) == -1 and ot(n=-1) == -1
+    assert ot(ldt=3) == -1 and ot(rdt=-1) == -1 and ot(odt=2) == -1 and ot(ldt=0, odt=1) == -1 and ot(r=P + 8) == -1
+    assert ot(s=0) == -1 and ot(s=2) == -1 and ot(s=3, part=P) == -1 and ot(n=1 << 22) == -2 and ot(m=1 << 29) == -2
     need = lib.sae_rows8_grad_rows_workspace_bytes(100, 40)
     assert need >= 100 * 4 and lib.sae_rows8_grad_rows_workspace_bytes(0, 40) == 0
     rows = lambda r=P, out=P, F=4, d=40, n=100, ws=P, b=need: lib.sae_rows8_grad_rows(P, P, P, P, r, out, None, F, d, n, ws, b, None)  # noqa: E731
