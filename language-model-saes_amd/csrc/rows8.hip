@@ -296,17 +296,37 @@ __global__ __launch_bounds__(256) void transpose_padded_kernel(const void *__res
 // that crosses leaves one partial row per window, joined in window order by a third launch.
 constexpr int R8_WINDOW = 128;
 
-// Per feature: the feature of each of its positions, a zero row where it has none, its coefficients' sum.
+// The first launch.  Workgroups below feat_blocks, a wave per feature: the feature of each of its positions, a zero row where
+// it has none, its coefficients' sum.  The others, a thread per position: token and coefficient in index order, so that the
+// waves of the second launch, one per window and chunk of columns, read them in line (by slot they would touch a cache line
+// per entry, once for every chunk).  Positions behind the last, up to a whole window, get feature -1.
 __global__ __launch_bounds__(256) void rows8_grad_prepare_kernel(const int32_t *__restrict__ feat_ptr, const int32_t *__restrict__ feat_slot,
-                                                                 const float *__restrict__ coef, int32_t *__restrict__ pos_feat,
-                                                                 float *__restrict__ out, float *__restrict__ bias_out, int64_t F, int64_t d) {
-  const int64_t f = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+                                                                 const int32_t *__restrict__ slot_tok, const float *__restrict__ coef,
+                                                                 int32_t *__restrict__ pos_feat, int32_t *__restrict__ pos_tok,
+                                                                 float *__restrict__ pos_coef, float *__restrict__ out,
+                                                                 float *__restrict__ bias_out, int64_t F, int64_t d, uint32_t feat_blocks) {
+  if (blockIdx.x >= feat_blocks) {
+    const int64_t i = (int64_t)(blockIdx.x - feat_blocks) * 256 + threadIdx.x;
+    const int total = feat_ptr[F];
+    if (i < total) {
+      const int slot = feat_slot[i];
+      pos_tok[i] = slot_tok[slot];
+      pos_coef[i] = coef[slot];
+    } else if (i < ((int64_t)total + R8_WINDOW - 1) / R8_WINDOW * R8_WINDOW) {
+      pos_feat[i] = -1;
+      pos_tok[i] = 0;
+      pos_coef[i] = 0.f;
+    }
+    return;
+  }
+  const int64_t f = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lane = threadIdx.x & 63;
   if (f >= F) return;
   const int lo = feat_ptr[f], hi = feat_ptr[f + 1];
   for (int i = lo + lane; i < hi; i += 64) pos_feat[i] = (int32_t)f;
   if (bias_out) {
     float s = 0.f;
+#pragma unroll 4
     for (int i = lo + lane; i < hi; i += 64) s += coef[feat_slot[i]];
     s = wave_sum(s);
     if (lane == 0) bias_out[f] = s;
@@ -314,7 +334,7 @@ __global__ __launch_bounds__(256) void rows8_grad_prepare_kernel(const int32_t *
   if (lo < hi) return;
   float *row = out + f * d;
   if ((d & 3) == 0) {
-    for (int64_t j = lane; j < (d >> 2); j += 64) reinterpret_cast<float4 *>(row)[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int64_t j = lane; j < (d >> 2); j += 64) store_stream(row, j, make_float4(0.f, 0.f, 0.f, 0.f));
   } else {
     for (int64_t j = lane; j < d; j += 64) row[j] = 0.f;
   }
@@ -327,29 +347,31 @@ struct R8Piece {
   uint32_t field;
 };
 
+// The second launch: a wave per window and chunk.  What says which record is read is the same for the whole wave and stays in
+// scalar registers.
 template <int C>
-__global__ __launch_bounds__(256) void rows8_grad_window_kernel(const int32_t *__restrict__ feat_ptr, const int32_t *__restrict__ feat_slot,
-                                                                const int32_t *__restrict__ slot_tok, const float *__restrict__ coef,
-                                                                const uint8_t *__restrict__ rows, const int32_t *__restrict__ pos_feat,
-                                                                float *__restrict__ out, float *__restrict__ part, int64_t F, int64_t d,
-                                                                int64_t n_windows, int64_t n_tasks) {
-  constexpr int G = 32 / C * 2;   // records requested together: 16 of 4 codes, 8 of 8
+__global__ __launch_bounds__(256) void rows8_grad_window_kernel(const int32_t *__restrict__ feat_ptr, const int32_t *__restrict__ pos_feat,
+                                                                const int32_t *__restrict__ pos_tok, const float *__restrict__ pos_coef,
+                                                                const uint8_t *__restrict__ rows, float *__restrict__ out,
+                                                                float *__restrict__ part, int64_t F, int64_t d, int64_t n_windows,
+                                                                int64_t n_tasks) {
+  constexpr int G = 16;   // records requested together
   const int lane = threadIdx.x & 63;
   // tasks in chunk-major order, one contiguous eighth per XCD (workgroups go round the XCDs): what an XCD reads at a time
   // is one chunk of columns of all records, which its L2 holds
   const int64_t per_xcd = (n_tasks + 7) / 8;
-  const int64_t local = (int64_t)(blockIdx.x >> 3) * 4 + (threadIdx.x >> 6);
+  const int64_t local = (int64_t)(blockIdx.x >> 3) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t task = (int64_t)(blockIdx.x & 7) * per_xcd + local;
   if (local >= per_xcd || task >= n_tasks) return;
   const int64_t chunk = task / n_windows, window = task % n_windows;
   const int total = feat_ptr[F];
-  const int w0 = (int)(window * R8_WINDOW);
+  const int w0 = (int)(window * R8_WINDOW), w1 = w0 + R8_WINDOW;
   if (w0 >= total) return;
-  const int w1 = w0 + R8_WINDOW < total ? w0 + R8_WINDOW : total;
-  const int64_t codes = r8_blocks(d) * R8_BLOCK, pitch = r8_pitch(d);
+  const int64_t codes = r8_blocks(d) * R8_BLOCK;
+  const uint32_t pitch = (uint32_t)r8_pitch(d);
   const int64_t col = chunk * 64 * C + lane * C;
   const bool on = col < codes;
-  const uint32_t code_at = on ? (uint32_t)col : 0u, field_at = (uint32_t)(codes + (on ? col >> 5 : 0));   // offsets in a record
+  const uint32_t code_off = on ? (uint32_t)col : 0u, field_off = (uint32_t)(codes + (on ? col >> 5 : 0));   // in a record
   const int before = w0 > 0 ? pos_feat[w0 - 1] : -1, after = w1 < total ? pos_feat[w1] : -1;
 
   float acc[C];
@@ -368,7 +390,7 @@ __global__ __launch_bounds__(256) void rows8_grad_window_kernel(const int32_t *_
         if ((d & 3) == 0) {
 #pragma unroll
           for (int e = 0; e < C; e += 4)
-            if (col + e < d) *reinterpret_cast<float4 *>(dst + e) = make_float4(acc[e], acc[e + 1], acc[e + 2], acc[e + 3]);
+            if (col + e < d) store_stream(dst + e, 0, make_float4(acc[e], acc[e + 1], acc[e + 2], acc[e + 3]));
         } else {
 #pragma unroll
           for (int e = 0; e < C; ++e)
@@ -380,45 +402,39 @@ __global__ __launch_bounds__(256) void rows8_grad_window_kernel(const int32_t *_
     for (int e = 0; e < C; ++e) acc[e] = 0.f;
   };
 
-  for (int p0 = w0; p0 < w1; p0 += 64) {
-    const int n = w1 - p0 < 64 ? w1 - p0 : 64;
-    int tok = 0, feat = -1;
-    float c = 0.f;
-    if (lane < n) {
-      const int slot = feat_slot[p0 + lane];
-      tok = slot_tok[slot];
-      c = coef[slot];
-      feat = pos_feat[p0 + lane];
+  for (int p = w0; p < w1; p += G) {
+    R8Piece<C> r[G];
+    int feat[G];
+    float coef[G];
+    // 32-bit offsets that the compiler cannot widen ahead of the loop: the loads then add them to a scalar base themselves
+    uint32_t code_at = code_off, field_at = field_off;
+    asm("" : "+v"(code_at), "+v"(field_at));
+#pragma unroll
+    for (int j = 0; j < G; ++j) {
+      feat[j] = pos_feat[p + j];
+      coef[j] = pos_coef[p + j];
     }
-    for (int j0 = 0; j0 < n; j0 += G) {
-      R8Piece<C> r[G];
 #pragma unroll
-      for (int j = 0; j < G; ++j) {
-        const int at = j0 + j < n ? j0 + j : n - 1;
-        const uint8_t *rec = rows + (int64_t)__builtin_amdgcn_readlane(tok, at) * pitch;   // the same for the whole wave
-        if constexpr (C == 4) {
-          r[j].w[0] = *reinterpret_cast<const uint32_t *>(rec + code_at);
-        } else {
-          const uint2 w = *reinterpret_cast<const uint2 *>(rec + code_at);
-          r[j].w[0] = w.x;
-          r[j].w[C / 4 - 1] = w.y;
-        }
-        r[j].field = rec[field_at];
+    for (int j = 0; j < G; ++j) {
+      const uint8_t *rec = rows + (uint64_t)(uint32_t)pos_tok[p + j] * pitch;
+      if constexpr (C == 4) {
+        r[j].w[0] = *reinterpret_cast<const uint32_t *>(rec + code_at);
+      } else {
+        const uint2 w = *reinterpret_cast<const uint2 *>(rec + code_at);
+        r[j].w[0] = w.x;
+        r[j].w[C / 4 - 1] = w.y;
       }
+      r[j].field = rec[field_at];
+    }
 #pragma unroll
-      for (int j = 0; j < G; ++j) {
-        if (j0 + j < n) {
-          const int f = __builtin_amdgcn_readlane(feat, j0 + j);
-          if (f != current) {
-            flush();
-            current = f;
-          }
-          const float cc = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(c), j0 + j));
-          const float step = __uint_as_float(r[j].field << 23);
-#pragma unroll
-          for (int e = 0; e < C; ++e) acc[e] = fmaf(cc, (float)(int8_t)(r[j].w[e / 4] >> (8 * (e % 4))) * step, acc[e]);
-        }
+    for (int j = 0; j < G; ++j) {
+      if (feat[j] != current) {
+        flush();
+        current = feat[j];
       }
+      const float step = __uint_as_float(r[j].field << 23);
+#pragma unroll
+      for (int e = 0; e < C; ++e) acc[e] = fmaf(coef[j], (float)(int8_t)(r[j].w[e / 4] >> (8 * (e % 4))) * step, acc[e]);
     }
   }
   flush();
@@ -444,7 +460,7 @@ __global__ __launch_bounds__(256) void rows8_grad_join_kernel(const int32_t *__r
   }
   float *dst = out + (int64_t)f * d + j;
   if ((d & 3) == 0) {
-    *reinterpret_cast<float4 *>(dst) = s;
+    store_stream(dst, 0, s);
   } else {
     const float v[4] = {s.x, s.y, s.z, s.w};
 #pragma unroll
@@ -536,14 +552,14 @@ extern "C" int sae_transpose_padded(const void *src, int src_dtype, int64_t rows
 
 namespace sae {
 static int64_t r8_windows(int64_t n_slots) { return (n_slots + R8_WINDOW - 1) / R8_WINDOW; }
-static int64_t r8_part_offset(int64_t n_slots) { return (n_slots * 4 + 15) & ~(int64_t)15; }
+static int64_t r8_positions(int64_t n_slots) { return r8_windows(n_slots) * R8_WINDOW; }
 }  // namespace sae
 
 extern "C" int64_t sae_rows8_grad_rows_workspace_bytes(int64_t n_slots, int64_t d) {
   using namespace sae;
   if (n_slots <= 0 || d <= 0) return 0;
-  // the feature of every position, and two partial rows per window
-  return r8_part_offset(n_slots) + r8_windows(n_slots) * 2 * r8_blocks(d) * R8_BLOCK * 4;
+  // feature, token and coefficient of every position, and two partial rows per window
+  return r8_positions(n_slots) * 12 + r8_windows(n_slots) * 2 * r8_blocks(d) * R8_BLOCK * 4;
 }
 
 extern "C" int sae_rows8_grad_rows(const int32_t *feat_ptr, const int32_t *feat_slot, const int32_t *slot_tok, const float *coef,
@@ -558,17 +574,19 @@ extern "C" int sae_rows8_grad_rows(const int32_t *feat_ptr, const int32_t *feat_
   SAE_REQUIRE(workspace && workspace_bytes >= sae_rows8_grad_rows_workspace_bytes(n_slots, d), SAE_ERR_WORKSPACE,
               "rows8_grad_rows: workspace of %lld bytes needed", (long long)sae_rows8_grad_rows_workspace_bytes(n_slots, d));
   hipStream_t st = (hipStream_t)stream;
-  int32_t *pos_feat = reinterpret_cast<int32_t *>(workspace);
-  float *part = reinterpret_cast<float *>(reinterpret_cast<char *>(workspace) + r8_part_offset(n_slots));
+  const int64_t positions = r8_positions(n_slots), windows = r8_windows(n_slots);
+  int32_t *pos_feat = reinterpret_cast<int32_t *>(workspace), *pos_tok = pos_feat + positions;
+  float *pos_coef = reinterpret_cast<float *>(pos_tok + positions), *part = pos_coef + positions;
   const uint8_t *rec = reinterpret_cast<const uint8_t *>(rows);
-  hipLaunchKernelGGL(rows8_grad_prepare_kernel, dim3((unsigned)((F + 3) / 4)), dim3(256), 0, st, feat_ptr, feat_slot, coef, pos_feat, out,
-                     bias_out, F, d);
+  const int64_t feat_blocks = (F + 3) / 4;
   constexpr int C = 4;
-  const int64_t windows = r8_windows(n_slots), chunks = (r8_blocks(d) * R8_BLOCK + 64 * C - 1) / (64 * C), tasks = windows * chunks;
+  const int64_t chunks = (r8_blocks(d) * R8_BLOCK + 64 * C - 1) / (64 * C), tasks = windows * chunks;
   const int64_t per_xcd = (tasks + 7) / 8, blocks = (per_xcd + 3) / 4 * 8;
   SAE_REQUIRE(blocks < (1LL << 31), SAE_ERR_UNSUPPORTED, "rows8_grad_rows: size too large");
-  hipLaunchKernelGGL(rows8_grad_window_kernel<C>, dim3((unsigned)blocks), dim3(256), 0, st, feat_ptr, feat_slot, slot_tok, coef, rec, pos_feat,
-                     out, part, F, d, windows, tasks);
+  hipLaunchKernelGGL(rows8_grad_prepare_kernel, dim3((unsigned)(feat_blocks + (positions + 255) / 256)), dim3(256), 0, st, feat_ptr, feat_slot,
+                     slot_tok, coef, pos_feat, pos_tok, pos_coef, out, bias_out, F, d, (uint32_t)feat_blocks);
+  hipLaunchKernelGGL(rows8_grad_window_kernel<C>, dim3((unsigned)blocks), dim3(256), 0, st, feat_ptr, pos_feat, pos_tok, pos_coef, rec, out, part,
+                     F, d, windows, tasks);
   hipLaunchKernelGGL(rows8_grad_join_kernel, dim3((unsigned)windows, (unsigned)((d + 1023) / 1024)), dim3(256), 0, st, feat_ptr, pos_feat, part,
                      out, F, d);
   return check_launch("rows8_grad_rows");
