@@ -292,9 +292,22 @@ __global__ __launch_bounds__(256) void transpose_padded_kernel(const void *__res
 // ---- gradient rows ---------------------------------------------------------------------------------------------------
 // out[f, :] = sum over feature f's slots of coef * (values of the slot's record): a segmented sum over the feature index.
 // Some features are kept by most tokens and most by few, so work is cut by position in feat_slot, not by feature: a wave
-// owns a window of R8_WINDOW positions and 64 C columns.  A segment that lies inside a window goes straight to its row; one
-// that crosses leaves one partial row per window, joined in window order by a third launch.
-constexpr int R8_WINDOW = 128;
+// owns a window of positions and 256 columns.  A segment that lies inside a window goes straight to its row; one that crosses
+// leaves one partial row per window, joined in window order by a third launch.
+// (8192 tokens, 64 of 32768 features, d = 2048: 142 us; a workgroup per feature takes 33 ms there, the most frequent feature's
+// 8000 records one after the other.  292 MB have to move, 42 us at the rate of a large fill; the second launch's vector
+// instructions alone are 90 us: 13 per record and four columns.)
+constexpr int R8_COLS = 256;   // columns of a chunk: four per lane (eight per lane: 196 us instead of 184, before the streaming
+                               // stores)
+
+// Positions per window.  Long windows leave fewer partial rows, short ones more waves: with few waves per CU a window's
+// records, read one group after the other, are what takes the time.  us at 32 / 64 / 128 positions: 36 / 30 / 32 at 4096
+// tokens, k = 32, d = 768 (3072 tasks of 128 positions), 194 / 167 / 161 at 8192, 64, 2048 (32768 tasks), 16 / 18 / 24 at 1000,
+// 32, 512 (500 tasks), 12 / 15 / 22 at 300, 16, 260 (76 tasks).
+static int r8_window(int64_t n_slots, int64_t d) {
+  const int64_t tasks = (n_slots + 127) / 128 * ((d + R8_COLS - 1) / R8_COLS);
+  return tasks < 1024 ? 32 : tasks < 8192 ? 64 : 128;
+}
 
 // The first launch.  Workgroups below feat_blocks, a wave per feature: the feature of each of its positions, a zero row where
 // it has none, its coefficients' sum.  The others, a thread per position: token and coefficient in index order, so that the
@@ -304,7 +317,8 @@ __global__ __launch_bounds__(256) void rows8_grad_prepare_kernel(const int32_t *
                                                                  const int32_t *__restrict__ slot_tok, const float *__restrict__ coef,
                                                                  int32_t *__restrict__ pos_feat, int32_t *__restrict__ pos_tok,
                                                                  float *__restrict__ pos_coef, float *__restrict__ out,
-                                                                 float *__restrict__ bias_out, int64_t F, int64_t d, uint32_t feat_blocks) {
+                                                                 float *__restrict__ bias_out, int64_t F, int64_t d, uint32_t feat_blocks,
+                                                                 int window) {
   if (blockIdx.x >= feat_blocks) {
     const int64_t i = (int64_t)(blockIdx.x - feat_blocks) * 256 + threadIdx.x;
     const int total = feat_ptr[F];
@@ -312,7 +326,7 @@ __global__ __launch_bounds__(256) void rows8_grad_prepare_kernel(const int32_t *
       const int slot = feat_slot[i];
       pos_tok[i] = slot_tok[slot];
       pos_coef[i] = coef[slot];
-    } else if (i < ((int64_t)total + R8_WINDOW - 1) / R8_WINDOW * R8_WINDOW) {
+    } else if (i < ((int64_t)total + window - 1) / window * window) {
       pos_feat[i] = -1;
       pos_tok[i] = 0;
       pos_coef[i] = 0.f;
@@ -340,16 +354,9 @@ __global__ __launch_bounds__(256) void rows8_grad_prepare_kernel(const int32_t *
   }
 }
 
-// C codes per lane as they lie in memory
-template <int C>
-struct R8Piece {
-  uint32_t w[C / 4];
-  uint32_t field;
-};
-
 // The second launch: a wave per window and chunk.  What says which record is read is the same for the whole wave and stays in
 // scalar registers.
-template <int C>
+template <int WINDOW>
 __global__ __launch_bounds__(256) void rows8_grad_window_kernel(const int32_t *__restrict__ feat_ptr, const int32_t *__restrict__ pos_feat,
                                                                 const int32_t *__restrict__ pos_tok, const float *__restrict__ pos_coef,
                                                                 const uint8_t *__restrict__ rows, float *__restrict__ out,
@@ -365,45 +372,40 @@ __global__ __launch_bounds__(256) void rows8_grad_window_kernel(const int32_t *_
   if (local >= per_xcd || task >= n_tasks) return;
   const int64_t chunk = task / n_windows, window = task % n_windows;
   const int total = feat_ptr[F];
-  const int w0 = (int)(window * R8_WINDOW), w1 = w0 + R8_WINDOW;
+  const int w0 = (int)(window * WINDOW), w1 = w0 + WINDOW;
   if (w0 >= total) return;
   const int64_t codes = r8_blocks(d) * R8_BLOCK;
   const uint32_t pitch = (uint32_t)r8_pitch(d);
-  const int64_t col = chunk * 64 * C + lane * C;
+  const int64_t col = chunk * R8_COLS + lane * 4;
   const bool on = col < codes;
   const uint32_t code_off = on ? (uint32_t)col : 0u, field_off = (uint32_t)(codes + (on ? col >> 5 : 0));   // in a record
   const int before = w0 > 0 ? pos_feat[w0 - 1] : -1, after = w1 < total ? pos_feat[w1] : -1;
 
-  float acc[C];
-#pragma unroll
-  for (int e = 0; e < C; ++e) acc[e] = 0.f;
+  float acc[4] = {0.f, 0.f, 0.f, 0.f};
   int current = -1;   // the feature being summed
   auto flush = [&]() {
     if (on && current >= 0) {
+      const float4 sum = make_float4(acc[0], acc[1], acc[2], acc[3]);
       const bool head = current == before, tail = current == after;
       if (head || tail) {
-        float *dst = part + (window * 2 + (head ? 0 : 1)) * codes + col;
-#pragma unroll
-        for (int e = 0; e < C; e += 4) *reinterpret_cast<float4 *>(dst + e) = make_float4(acc[e], acc[e + 1], acc[e + 2], acc[e + 3]);
+        *reinterpret_cast<float4 *>(part + (window * 2 + (head ? 0 : 1)) * codes + col) = sum;
       } else {
-        float *dst = out + (int64_t)current * d + col;
+        float *dst = out + (int64_t)current * d + col;   // written once, read by no one here: it need not displace records
         if ((d & 3) == 0) {
-#pragma unroll
-          for (int e = 0; e < C; e += 4)
-            if (col + e < d) store_stream(dst + e, 0, make_float4(acc[e], acc[e + 1], acc[e + 2], acc[e + 3]));
+          if (col < d) store_stream(dst, 0, sum);
         } else {
 #pragma unroll
-          for (int e = 0; e < C; ++e)
+          for (int e = 0; e < 4; ++e)
             if (col + e < d) dst[e] = acc[e];
         }
       }
     }
 #pragma unroll
-    for (int e = 0; e < C; ++e) acc[e] = 0.f;
+    for (int e = 0; e < 4; ++e) acc[e] = 0.f;
   };
 
   for (int p = w0; p < w1; p += G) {
-    R8Piece<C> r[G];
+    uint32_t codes4[G], field[G];
     int feat[G];
     float coef[G];
     // 32-bit offsets that the compiler cannot widen ahead of the loop: the loads then add them to a scalar base themselves
@@ -417,14 +419,8 @@ __global__ __launch_bounds__(256) void rows8_grad_window_kernel(const int32_t *_
 #pragma unroll
     for (int j = 0; j < G; ++j) {
       const uint8_t *rec = rows + (uint64_t)(uint32_t)pos_tok[p + j] * pitch;
-      if constexpr (C == 4) {
-        r[j].w[0] = *reinterpret_cast<const uint32_t *>(rec + code_at);
-      } else {
-        const uint2 w = *reinterpret_cast<const uint2 *>(rec + code_at);
-        r[j].w[0] = w.x;
-        r[j].w[C / 4 - 1] = w.y;
-      }
-      r[j].field = rec[field_at];
+      codes4[j] = *reinterpret_cast<const uint32_t *>(rec + code_at);
+      field[j] = rec[field_at];
     }
 #pragma unroll
     for (int j = 0; j < G; ++j) {
@@ -432,9 +428,9 @@ __global__ __launch_bounds__(256) void rows8_grad_window_kernel(const int32_t *_
         flush();
         current = feat[j];
       }
-      const float step = __uint_as_float(r[j].field << 23);
+      const float step = __uint_as_float(field[j] << 23);
 #pragma unroll
-      for (int e = 0; e < C; ++e) acc[e] = fmaf(coef[j], (float)(int8_t)(r[j].w[e / 4] >> (8 * (e % 4))) * step, acc[e]);
+      for (int e = 0; e < 4; ++e) acc[e] = fmaf(coef[j], (float)(int8_t)(codes4[j] >> (8 * e)) * step, acc[e]);
     }
   }
   flush();
@@ -442,14 +438,15 @@ __global__ __launch_bounds__(256) void rows8_grad_window_kernel(const int32_t *_
 
 // The segment that begins in this window and goes on behind it: its partial rows, added in window order.
 __global__ __launch_bounds__(256) void rows8_grad_join_kernel(const int32_t *__restrict__ feat_ptr, const int32_t *__restrict__ pos_feat,
-                                                              const float *__restrict__ part, float *__restrict__ out, int64_t F, int64_t d) {
+                                                              const float *__restrict__ part, float *__restrict__ out, int64_t F, int64_t d,
+                                                             int length) {
   const int64_t window = blockIdx.x;
   const int total = feat_ptr[F];
-  const int64_t w0 = window * R8_WINDOW, w1 = w0 + R8_WINDOW;
+  const int64_t w0 = window * length, w1 = w0 + length;
   if (w1 >= total) return;
   const int f = pos_feat[w1];
   if (pos_feat[w1 - 1] != f || (w0 > 0 && pos_feat[w0 - 1] == f)) return;
-  const int64_t last = (feat_ptr[f + 1] - 1) / R8_WINDOW, codes = r8_blocks(d) * R8_BLOCK;
+  const int64_t last = (feat_ptr[f + 1] - 1) / length, codes = r8_blocks(d) * R8_BLOCK;
   const int64_t j = ((int64_t)blockIdx.y * 256 + threadIdx.x) * 4;
   if (j >= d) return;
   float4 s = *reinterpret_cast<const float4 *>(part + (window * 2 + 1) * codes + j);
@@ -550,16 +547,12 @@ extern "C" int sae_transpose_padded(const void *src, int src_dtype, int64_t rows
   return check_launch("transpose_padded");
 }
 
-namespace sae {
-static int64_t r8_windows(int64_t n_slots) { return (n_slots + R8_WINDOW - 1) / R8_WINDOW; }
-static int64_t r8_positions(int64_t n_slots) { return r8_windows(n_slots) * R8_WINDOW; }
-}  // namespace sae
-
 extern "C" int64_t sae_rows8_grad_rows_workspace_bytes(int64_t n_slots, int64_t d) {
   using namespace sae;
   if (n_slots <= 0 || d <= 0) return 0;
+  const int64_t length = r8_window(n_slots, d), windows = (n_slots + length - 1) / length;
   // feature, token and coefficient of every position, and two partial rows per window
-  return r8_positions(n_slots) * 12 + r8_windows(n_slots) * 2 * r8_blocks(d) * R8_BLOCK * 4;
+  return windows * length * 12 + windows * 2 * r8_blocks(d) * R8_BLOCK * 4;
 }
 
 extern "C" int sae_rows8_grad_rows(const int32_t *feat_ptr, const int32_t *feat_slot, const int32_t *slot_tok, const float *coef,
@@ -568,26 +561,30 @@ extern "C" int sae_rows8_grad_rows(const int32_t *feat_ptr, const int32_t *feat_
   using namespace sae;
   SAE_REQUIRE(feat_ptr && feat_slot && slot_tok && coef && rows && out, SAE_ERR_INVALID_ARG, "rows8_grad_rows: null pointer");
   SAE_REQUIRE(F > 0 && d > 0 && n_slots > 0, SAE_ERR_INVALID_ARG, "rows8_grad_rows: bad sizes");
-  SAE_REQUIRE(F < (1LL << 31) - 1 && d < (1LL << 30) && n_slots < (1LL << 31) - R8_WINDOW, SAE_ERR_UNSUPPORTED, "rows8_grad_rows: size too large");
+  SAE_REQUIRE(F < (1LL << 31) - 1 && d < (1LL << 30) && n_slots < (1LL << 31) - 128, SAE_ERR_UNSUPPORTED, "rows8_grad_rows: size too large");
   SAE_REQUIRE((((uintptr_t)rows | (uintptr_t)out | (uintptr_t)workspace) & 15) == 0, SAE_ERR_INVALID_ARG,
               "rows8_grad_rows: 16-byte alignment required");
   SAE_REQUIRE(workspace && workspace_bytes >= sae_rows8_grad_rows_workspace_bytes(n_slots, d), SAE_ERR_WORKSPACE,
               "rows8_grad_rows: workspace of %lld bytes needed", (long long)sae_rows8_grad_rows_workspace_bytes(n_slots, d));
   hipStream_t st = (hipStream_t)stream;
-  const int64_t positions = r8_positions(n_slots), windows = r8_windows(n_slots);
+  const int length = r8_window(n_slots, d);
+  const int64_t windows = (n_slots + length - 1) / length, positions = windows * length;
   int32_t *pos_feat = reinterpret_cast<int32_t *>(workspace), *pos_tok = pos_feat + positions;
   float *pos_coef = reinterpret_cast<float *>(pos_tok + positions), *part = pos_coef + positions;
   const uint8_t *rec = reinterpret_cast<const uint8_t *>(rows);
-  const int64_t feat_blocks = (F + 3) / 4;
-  constexpr int C = 4;
-  const int64_t chunks = (r8_blocks(d) * R8_BLOCK + 64 * C - 1) / (64 * C), tasks = windows * chunks;
+  const int64_t feat_blocks = (F + 3) / 4, chunks = (r8_blocks(d) * R8_BLOCK + R8_COLS - 1) / R8_COLS, tasks = windows * chunks;
   const int64_t per_xcd = (tasks + 7) / 8, blocks = (per_xcd + 3) / 4 * 8;
   SAE_REQUIRE(blocks < (1LL << 31), SAE_ERR_UNSUPPORTED, "rows8_grad_rows: size too large");
   hipLaunchKernelGGL(rows8_grad_prepare_kernel, dim3((unsigned)(feat_blocks + (positions + 255) / 256)), dim3(256), 0, st, feat_ptr, feat_slot,
-                     slot_tok, coef, pos_feat, pos_tok, pos_coef, out, bias_out, F, d, (uint32_t)feat_blocks);
-  hipLaunchKernelGGL(rows8_grad_window_kernel<C>, dim3((unsigned)blocks), dim3(256), 0, st, feat_ptr, pos_feat, pos_tok, pos_coef, rec, out, part,
-                     F, d, windows, tasks);
+                     slot_tok, coef, pos_feat, pos_tok, pos_coef, out, bias_out, F, d, (uint32_t)feat_blocks, length);
+#define SAE_R8_GRAD(W)                                                                                                              \
+  hipLaunchKernelGGL(rows8_grad_window_kernel<W>, dim3((unsigned)blocks), dim3(256), 0, st, feat_ptr, pos_feat, pos_tok, pos_coef, rec, out, \
+                     part, F, d, windows, tasks)
+  if (length == 32) SAE_R8_GRAD(32);
+  else if (length == 64) SAE_R8_GRAD(64);
+  else SAE_R8_GRAD(128);
+#undef SAE_R8_GRAD
   hipLaunchKernelGGL(rows8_grad_join_kernel, dim3((unsigned)windows, (unsigned)((d + 1023) / 1024)), dim3(256), 0, st, feat_ptr, pos_feat, part,
-                     out, F, d);
+                     out, F, d, length);
   return check_launch("rows8_grad_rows");
 }

@@ -305,7 +305,8 @@ def sparse_code(ops, T, F, k, seed, dev, heavy=False):
 
 
 CODES = [(1, 5, 1, 40), (7, 30, 4, 33), (64, 100, 8, 768), (300, 17, 5, 1037), (513, 64, 12, 520), (1500, 12, 3, 2052), (40, 9, 2, 4100),
-         (33, 50, 6, 1), (128, 5, 1, 64), (2000, 400, 16, 260), (640, 8, 5, 36), (4096, 3, 1, 300)]
+         (33, 50, 6, 1), (128, 5, 1, 64), (2000, 400, 16, 260), (640, 8, 5, 36), (4096, 3, 1, 300),
+         (4100, 60, 32, 1500), (9000, 300, 48, 516)]
 
 
 @pytest.mark.parametrize("heavy", [False, True])
@@ -323,8 +324,8 @@ def test_gradient_rows(pkg, dev, T, F, k, d, heavy):
     assert (np.abs(doubles(bias) - dense.sum(0)) <= 2.0**-23 * per_feature[:, 0] * np.abs(dense).sum(0) + 1e-40).all()
     assert not out[(dense == 0).all(0)].any()               # features that no token kept
     if d % 4 == 0:                                          # the same rows held in floats: the same bits, but for features whose
-        ptr = fi.feat_ptr.long()                            # slots cross a multiple of 64, which may be summed in pieces
-        whole = (ptr[:-1] // 64 == (ptr[1:] - 1).clamp_min(0) // 64) | (ptr[:-1] == ptr[1:])
+        ptr = fi.feat_ptr.long()                            # slots cross a multiple of 32, which may be summed in pieces
+        whole = (ptr[:-1] // 32 == (ptr[1:] - 1).clamp_min(0) // 32) | (ptr[:-1] == ptr[1:])
         floats = ops.restore_rows(q)
         want, _ = ops.sparse_grad_rows(fi, code.val, floats, F)
         assert torch.equal(out[whole], want[whole])
