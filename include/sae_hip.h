@@ -531,7 +531,8 @@ int sae_gemm_over_tokens(const void *left, int left_dtype, const void *right, in
 
 /* sae_sparse_grad_rows for a dense operand held as records (any d): out[f, :] = sum over the slots s of feature f of
  * coef[s] * values of record slot_tok[s]; rows without slots are written as zeros; bias_out (nullable) [F].  n_slots: the
- * length of feat_slot (feat_ptr[F] of them are in use).  A feature's slots are added in ascending order, as
+ * length of feat_slot (positions feat_ptr[0] .. feat_ptr[F] of it are in use: the index may be a stretch of a longer one's
+ * features).  A feature's slots are added in ascending order, as
  * sae_sparse_grad_rows adds them; where they cross a multiple of 32, 64 or 128 (by n_slots and d) in feat_slot the pieces are summed apart and
  * then joined in order, so a feature that many tokens keep costs no more time than as many slots of rare ones.  workspace:
  * sae_rows8_grad_rows_workspace_bytes(n_slots, d) bytes, 16-byte aligned. */

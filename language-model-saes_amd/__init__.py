@@ -32,10 +32,10 @@ __all__ += ["CrosscoderConfig", "CLTConfig", "LorsaConfig", "Crosscoder", "Cross
 from . import kernels, metrics  # noqa: E402,F401
 from .activation import (  # noqa: E402,F401
     ActivationBatchler, ActivationTransformer, ActivationWriter, ActivationWriterConfig, BufferShuffleConfig,
-    CachedActivationLoader, ChunkInfo, cached_activation_stream,
+    CachedActivationLoader, ChunkInfo, cached_activation_stream, rows8_pack, rows8_unpack,
 )
 from .initializer import Initializer, InitializerConfig, calculate_activation_norm  # noqa: E402,F401
 
 __all__ += ["metrics", "ActivationBatchler", "ActivationTransformer", "ActivationWriter", "ActivationWriterConfig",
-            "BufferShuffleConfig", "CachedActivationLoader", "ChunkInfo", "cached_activation_stream", "Initializer",
+            "BufferShuffleConfig", "CachedActivationLoader", "ChunkInfo", "cached_activation_stream", "rows8_pack", "rows8_unpack", "Initializer",
             "InitializerConfig", "calculate_activation_norm"]

@@ -9,6 +9,11 @@ File layout and processor semantics are the reference's
     <cache_dir>/<hook_point>/chunk-00000000.meta.json              (optional)
     <cache_dir>/<hook_point>/shard-3-chunk-00000007.pt             the sharded / torch.save variants
 
+With `row_format="rows8"` the writer's activation rows are records of 8-bit values (`ops.Rows8`; about a quarter of fp32 rows'
+bytes, half of bf16 ones): the file's `activation` is then uint8 [..., record bytes], and `activation_width` holds the width
+and the float type of the rows.  The loader gives float rows back unless it is asked to keep the records, and the batchler
+keeps records in its buffer, arriving as such or made there from float rows; a batch is one gather that reads them.
+
 What differs is where the bytes live.  The reference's `ActivationBuffer` re-concatenates and permutes the
 whole shuffle buffer for every refill and every batch; here the buffer is a fixed slab per key (in HBM when
 the stream is on the GPU), a shuffle permutes row indices on the host, and a batch is one gather kernel
@@ -34,6 +39,53 @@ from pydantic import BaseModel
 from . import ops
 
 
+# ---- rows held in 8 bits ----------------------------------------------------------------------------------
+
+_FLOAT_CODES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+def rows8_pack(x: torch.Tensor) -> torch.Tensor:
+    """uint8 [..., rows8_pitch(d)] records of float rows [..., d]: on the GPU the kernel, on the CPU (files written and read
+    without one) the same bits from tensor operations."""
+    lead, d = x.shape[:-1], x.shape[-1]
+    if x.dtype not in _FLOAT_CODES or d < 1:
+        raise ValueError(f"rows held in 8 bits are made of fp32, bf16 or fp16 rows [..., d], got {x.dtype} {tuple(x.shape)}")
+    pitch = ops.rows8_pitch(d)
+    rows = x.reshape(-1, d) if x.dtype == torch.bfloat16 else x.reshape(-1, d).float()
+    if rows.is_cuda:
+        return ops.quantize_rows(rows).data.view(*lead, pitch)
+    nb = -(-d // ops.ROWS8_BLOCK)
+    full = torch.zeros(rows.shape[0], nb * ops.ROWS8_BLOCK)
+    full[:, :d] = rows
+    blocks = full.view(-1, nb, ops.ROWS8_BLOCK)
+    bits = blocks.abs().contiguous().view(torch.int32).amax(2)      # of a magnitude: in the order of the magnitudes, NaN last
+    field = torch.clamp(((bits + 0x10000) >> 23).clamp_min(7) - 6, max=248)
+    field = torch.where(bits == 0, torch.zeros_like(field), field)
+    bad = bits >= 0x7F800000
+    inv = torch.clamp(254 - field, 1, 254).bitwise_left_shift(23).view(torch.float32)
+    codes = torch.where(bad[..., None], torch.zeros_like(blocks), blocks * inv[..., None]).round().clamp(-127, 127).to(torch.int8)
+    out = torch.zeros(rows.shape[0], pitch, dtype=torch.uint8)
+    out[:, : nb * ops.ROWS8_BLOCK] = codes.view(rows.shape[0], -1).view(torch.uint8)
+    out[:, nb * ops.ROWS8_BLOCK : nb * ops.ROWS8_BLOCK + nb] = torch.where(bad, torch.full_like(field, 255), field).to(torch.uint8)
+    return out.view(*lead, pitch)
+
+
+def rows8_unpack(data: torch.Tensor, d: int, dtype: torch.dtype, scale: float = 1.0) -> torch.Tensor:
+    """cast(scale * values) [..., d] of records [..., rows8_pitch(d)]."""
+    lead = data.shape[:-1]
+    rows = ops.Rows8(data.reshape(-1, data.shape[-1]), d)
+    if data.is_cuda:
+        direct = dtype if dtype in (torch.float32, torch.bfloat16) else torch.float32
+        out = ops.restore_rows(ops.Rows8(rows.data.contiguous(), d), direct, scale)
+    else:
+        nb = -(-d // ops.ROWS8_BLOCK)
+        codes = rows.data[:, : nb * ops.ROWS8_BLOCK].contiguous().view(torch.int8).float().view(-1, nb, ops.ROWS8_BLOCK)
+        field = rows.data[:, nb * ops.ROWS8_BLOCK : nb * ops.ROWS8_BLOCK + nb].to(torch.int32)
+        out = (codes * field.bitwise_left_shift(23).view(torch.float32)[..., None]).view(-1, nb * ops.ROWS8_BLOCK)[:, :d]
+        out = (out * scale if scale != 1.0 else out).contiguous()
+    return out.to(dtype).view(*lead, d)
+
+
 # ---- writer (activation/writer.py) ----------------------------------------------------------------
 
 class ActivationWriterConfig(BaseModel):
@@ -42,6 +94,7 @@ class ActivationWriterConfig(BaseModel):
     n_samples_per_chunk: Optional[int] = None
     cache_dir: str = "activations"
     format: str = "safetensors"      # "pt" | "safetensors"; anything else is rejected when a chunk is written
+    row_format: Literal["float", "rows8"] = "float"     # "rows8": activation rows as records of 8-bit values
     num_workers: Optional[int] = None
 
 
@@ -99,7 +152,11 @@ class ActivationWriter:
                 assert all(k in chunk for k in self.cfg.hook_points), f"All samples must have the hook points: {self.cfg.hook_points}"
                 name = f"chunk-{chunk_id:08d}" if start_shard is None else f"shard-{start_shard}-chunk-{chunk_id:08d}"
                 for hp in self.cfg.hook_points:
-                    payload = {"activation": chunk[hp]} | {k: v for k, v in chunk.items() if k not in ["meta", *self.cfg.hook_points]}
+                    act = {"activation": chunk[hp]}
+                    if self.cfg.row_format == "rows8":
+                        act = {"activation": rows8_pack(chunk[hp]),
+                               "activation_width": torch.tensor([chunk[hp].shape[-1], _FLOAT_CODES[chunk[hp].dtype]])}
+                    payload = act | {k: v for k, v in chunk.items() if k not in ["meta", *self.cfg.hook_points]}
                     if pool is None:
                         self._write_chunk(hp, payload, name, chunk.get("meta"))
                     else:
@@ -140,11 +197,16 @@ _REQUIRED = ("activation", "tokens", "mask", "attention_mask")
 class CachedActivationLoader:
     """Streams cached chunks in (shard, chunk) order; one output dict per chunk index with every hook point's
     activation under its name plus tokens / mask / attention_mask / meta, leading sample dims flattened
-    until `tokens` is at most 2-D (cached_activation.py:318-420).  With a GPU `device`, chunk i + 1 is read
+    until `tokens` is at most 2-D (cached_activation.py:318-420).  Rows held in 8 bits come out as the float rows they stand for
+    (`dtype`, or the type they were written from), read back on `device`; with `keep_rows8` as they are, uint8 records, whose
+    widths `rows8_widths` then names by hook point.  With a GPU `device`, chunk i + 1 is read
     from disk by a worker thread into pinned memory and copied on a side stream while chunk i is in use."""
 
     def __init__(self, cache_dirs: Mapping[str, str | Path], device: str = "cpu", dtype: Optional[torch.dtype] = None,
-                 prefetch: int = 2):
+                 prefetch: int = 2, keep_rows8: bool = False):
+        self.keep_rows8 = bool(keep_rows8)
+        self.rows8_widths: dict[str, int] = {}                     # hook points whose files hold 8-bit rows -> width
+        self._rows8_types: dict[str, torch.dtype] = {}
         self.cache_dirs = {k: Path(v) for k, v in cache_dirs.items()}
         self.device = torch.device(device)
         self.dtype = dtype
@@ -188,6 +250,18 @@ class CachedActivationLoader:
             elif not torch.equal(data["tokens"], out["tokens"]):
                 raise AssertionError(f"Loading cached activation error: tokens mismatch for chunk {i}")
             act = data["activation"]
+            if "activation_width" in data:
+                d, code = (int(v) for v in data["activation_width"])
+                if act.dtype != torch.uint8 or d < 1 or act.shape[-1] != ops.rows8_pitch(d) or code not in _FLOAT_CODES.values():
+                    raise ValueError(f"Loading cached activation {path} error: {act.dtype} {tuple(act.shape)} does not hold "
+                                     f"8-bit rows of width {d}, type {code}")
+                if self.rows8_widths.setdefault(hp, d) != d:
+                    raise ValueError(f"Loading cached activation {path} error: rows of width {d} after {self.rows8_widths[hp]}")
+                self._rows8_types[hp] = next(t for t, c in _FLOAT_CODES.items() if c == code)
+                out[hp] = act
+                continue
+            if hp in self.rows8_widths:
+                raise ValueError(f"Loading cached activation {path} error: float rows after 8-bit ones")
             out[hp] = act.to(self.dtype) if self.dtype is not None else act
         while out["tokens"].ndim >= 3:
             out = {k: (v.flatten(0, 1) if isinstance(v, torch.Tensor) else ([a for b in v for a in b] if v is not None else None))
@@ -231,6 +305,13 @@ class CachedActivationLoader:
                 v.record_stream(consumer)
         return staged
 
+    def _floats(self, chunk: dict[str, Any]) -> dict[str, Any]:
+        """The chunk with its 8-bit rows read back, unless they are to be kept."""
+        if self.keep_rows8 or not self.rows8_widths:
+            return chunk
+        return {k: rows8_unpack(v, self.rows8_widths[k], self.dtype or self._rows8_types[k]) if k in self.rows8_widths else v
+                for k, v in chunk.items()}
+
     def process(self, data: None = None, **kwargs) -> Iterator[dict[str, Any]]:
         hook_chunks = {hp: self._get_sorted_chunks(hp) for hp in self.cache_dirs}
         counts = {hp: len(c) for hp, c in hook_chunks.items()}
@@ -240,7 +321,7 @@ class CachedActivationLoader:
         n = next(iter(counts.values()))
         if self.device.type != "cuda":
             for i in range(n):
-                yield self._read_chunk_index(i, hook_chunks)
+                yield self._floats(self._read_chunk_index(i, hook_chunks))
             return
 
         q: Queue = Queue(maxsize=self.prefetch)
@@ -268,7 +349,7 @@ class CachedActivationLoader:
                 nxt = self._to_device(payload, copy_stream) if kind == "chunk" else None
                 if pending is not None:
                     staged, (done, _host) = pending
-                    yield self._hand_over(staged, done, torch.cuda.current_stream(self.device))
+                    yield self._floats(self._hand_over(staged, done, torch.cuda.current_stream(self.device)))
                 pending = nxt
                 if kind == "end":
                     break
@@ -307,10 +388,18 @@ class BufferShuffleConfig(BaseModel):
 
 
 class _RowStore:
-    """Rows of one key in a fixed slab; logical order is kept by the batchler as a list of slab rows."""
+    """Rows of one key in a fixed slab; logical order is kept by the batchler as a list of slab rows.  With `width` the
+    slab holds 8-bit records of that many values: rows arrive as records, or as float rows and are written as records."""
 
-    def __init__(self, like: torch.Tensor, capacity: int):
-        self.data = torch.empty((capacity, *like.shape[1:]), dtype=like.dtype, device=like.device)
+    def __init__(self, like: torch.Tensor, capacity: int, width: Optional[int] = None):
+        self.width, shape, dtype = width, like.shape[1:], like.dtype
+        self.float_dtype = like.dtype if like.is_floating_point() else torch.bfloat16   # of a batch, unless it is overridden
+        if width is not None:
+            packed = like.dtype == torch.uint8
+            if like.ndim != 2 or like.shape[1] != (ops.rows8_pitch(width) if packed else width) or not (packed or like.is_floating_point()):
+                raise ValueError(f"{like.dtype} rows {tuple(like.shape)} are neither records nor float rows of {width} values")
+            shape, dtype = (ops.rows8_pitch(width),), torch.uint8
+        self.data = torch.empty((capacity, *shape), dtype=dtype, device=like.device)
 
     def grow(self, capacity: int) -> None:
         if capacity > self.data.shape[0]:
@@ -321,6 +410,14 @@ class _RowStore:
     def put(self, rows: torch.Tensor, slots_host: torch.Tensor) -> None:
         n = rows.shape[0]
         first = int(slots_host[0])
+        if self.width is not None:
+            if rows.ndim != 2 or rows.shape[1] != (self.width if rows.dtype != torch.uint8 else self.data.shape[1]):
+                raise ValueError(f"{rows.dtype} rows {tuple(rows.shape)} in a buffer of 8-bit rows of {self.width} values")
+        if self.width is not None and rows.dtype != torch.uint8:
+            if rows.is_cuda and rows.dtype in (torch.float32, torch.bfloat16) and int(slots_host[-1]) - first == n - 1:
+                ops.quantize_rows(rows, out=self.data[first:first + n])
+                return
+            rows = rows8_pack(rows)
         if int(slots_host[-1]) - first == n - 1:      # slots are handed out ascending: contiguous means a plain slice
             self.data[first:first + n] = rows
         else:
@@ -328,6 +425,11 @@ class _RowStore:
 
     def take(self, idx_host: torch.Tensor, out_dtype: Optional[torch.dtype], scale: float) -> torch.Tensor:
         d = self.data
+        if self.width is not None:
+            to = out_dtype or self.float_dtype
+            if d.is_cuda and to in (torch.float32, torch.bfloat16):
+                return ops.gather_rows(ops.Rows8(d, self.width), idx_host.to(d.device), out_dtype=to, scale=scale)
+            return rows8_unpack(d.index_select(0, idx_host.to(d.device)), self.width, to, scale)
         floaty = d.ndim == 2 and d.dtype in (torch.float32, torch.bfloat16)
         if d.is_cuda and floaty:
             return ops.gather_rows(d, idx_host.to(d.device), out_dtype=out_dtype or d.dtype, scale=scale)
@@ -344,11 +446,16 @@ class ActivationBatchler:
     """Batches (and optionally shuffles) token rows exactly as the reference's `ActivationBatchler`:
     with `buffer_size`, rows accumulate until the buffer holds that many, the buffer is shuffled, and batches
     are drawn until it is half empty; without, full batches are cut in arrival order; the tail is flushed in
-    batches at the end.  `override_dtype` / `scale` apply to floating-point rows on the way out."""
+    batches at the end.  `override_dtype` / `scale` apply to floating-point rows on the way out.
+
+    `rows8`: what to hold in 8 bits, a key's width by key (a mapping that may be filled until the key's first rows arrive).
+    Rows of such a key arrive as float rows of that width or as records (uint8), and leave as floats: `override_dtype`, or the
+    type they arrived in (bf16, in which every value is exact, for records)."""
 
     def __init__(self, batch_size: int, buffer_size: Optional[int] = None,
                  buffer_shuffle_config: Optional[BufferShuffleConfig] = None, override_dtype: Optional[torch.dtype] = None,
-                 scale: float = 1.0):
+                 scale: float = 1.0, rows8: Optional[Mapping[str, int]] = None):
+        self.rows8 = {} if rows8 is None else rows8
         self.batch_size = batch_size
         self.buffer_size = buffer_size
         self.override_dtype = override_dtype
@@ -399,7 +506,7 @@ class ActivationBatchler:
                 tensors = {k: v for k, v in d.items() if isinstance(v, torch.Tensor)}
                 for k, v in tensors.items():
                     if k not in stores:
-                        stores[k] = _RowStore(v, capacity)
+                        stores[k] = _RowStore(v, capacity, self.rows8.get(k))
                 slots = alloc(n)
                 for k, v in tensors.items():
                     stores[k].put(v, slots)
@@ -424,9 +531,13 @@ class ActivationBatchler:
 def cached_activation_stream(cache_dir: str | Path, hook_points: Sequence[str], *, batch_size: int,
                              buffer_size: Optional[int] = None, buffer_shuffle_config: Optional[BufferShuffleConfig] = None,
                              device: str = "cuda", dtype: Optional[torch.dtype] = None,
-                             override_dtype: Optional[torch.dtype] = None) -> Iterator[dict[str, torch.Tensor]]:
+                             override_dtype: Optional[torch.dtype] = None,
+                             rows8: bool = False) -> Iterator[dict[str, torch.Tensor]]:
     """Loader -> mask filter -> batchler, the chain the reference's ActivationFactory builds for a cached
-    source with a batch size (activation/factory.py:246-345): yields `{hook: [batch, d], tokens: [batch], ...}`."""
-    loader = CachedActivationLoader({hp: os.path.join(str(cache_dir), hp) for hp in hook_points}, device=device, dtype=dtype)
-    batchler = ActivationBatchler(batch_size, buffer_size, buffer_shuffle_config, override_dtype=override_dtype)
+    source with a batch size (activation/factory.py:246-345): yields `{hook: [batch, d], tokens: [batch], ...}`.
+    With `rows8` files of 8-bit rows stay records up to the batch: half the bytes of bf16 over the bus and in the buffer."""
+    loader = CachedActivationLoader({hp: os.path.join(str(cache_dir), hp) for hp in hook_points}, device=device, dtype=dtype,
+                                    keep_rows8=rows8)
+    batchler = ActivationBatchler(batch_size, buffer_size, buffer_shuffle_config, override_dtype=override_dtype or (dtype if rows8 else None),
+                                  rows8=loader.rows8_widths)
     return batchler.process(ActivationTransformer().process(loader.process()))

@@ -158,7 +158,9 @@ class _FusedCLTStep(torch.autograd.Function):
                 recon_out=recon[j], loss_out=loss_toks[j], dval_acc=dval, grad_out=grads[j])
         loss = loss_toks.sum()
         holder.update(code=cat, pres=pres, norms=norms, layer_cnt=layer_cnt)
-        ctx.cat, ctx.grads, ctx.dval, ctx.x_op, ctx.w_enc_op = cat, grads, dval, x_op, w_enc_op
+        ctx.cat, ctx.grads, ctx.dval, ctx.w_enc_op = cat, grads, dval, w_enc_op
+        ctx.x_rows = ([ops.Rows8(rows, d) for rows in ops.quantize_rows(x_op.reshape(L * B, d)).data.view(L, B, -1)]
+                      if m.rows8_checkpoint else x_op)                     # per layer: what the encoders' gradient rows gather
         ctx.shape = (B, L, d, F)
         ctx.amp = bool(amp)
         ctx.defer_to = m if holder.get("defer") else None
@@ -187,12 +189,12 @@ class _FusedCLTStep(torch.autograd.Function):
             if defer:
                 # the optimiser rebuilds the rows where it consumes them; nothing dense is written here
                 dec_params[j]._sparse_grad = SparseRowGrad(fi_j, coef_dec, gd_all[j], (j + 1) * F)
-                enc_pieces.append((j * F, SparseRowGrad(fi_l, coef_enc, ctx.x_op[j], F)))
+                enc_pieces.append((j * F, SparseRowGrad(fi_l, coef_enc, ctx.x_rows[j], F)))
                 dW_D.append(None)
                 continue
             rows, _ = ops.sparse_grad_rows(fi_j, coef_dec, ctx.grads[j], (j + 1) * F)
             dW_D.append(rows.view(j + 1, F, d))
-            rows_e, bias_e = ops.sparse_grad_rows(fi_l, coef_enc, ctx.x_op[j], F, want_bias=True)
+            rows_e, bias_e = ops.sparse_grad_rows(fi_l, coef_enc, ctx.x_rows[j], F, want_bias=True)
             dW_E.append(rows_e); db_E.append(bias_e)
         if defer:
             m.W_E._sparse_grad = SparseRowGradPieces(enc_pieces, L * F, bias_param=m.b_E)
@@ -221,7 +223,7 @@ class _LayerEncoderGemm(torch.autograd.Function):
     d(pre)^T x as a product over the token axis on the same kernel."""
 
     @staticmethod
-    def forward(ctx, x, W_E, w_op, amp):
+    def forward(ctx, x, W_E, w_op, amp, keep8=False):
         B, L, d = x.shape
         F = w_op.shape[1]
         x_l = x.permute(1, 0, 2).contiguous()                                    # [L, B, d]
@@ -233,7 +235,8 @@ class _LayerEncoderGemm(torch.autograd.Function):
         pre = torch.empty(L, B, F, dtype=out_dtype, device=x.device)
         for l in range(L):
             ops.encoder_gemm(x_op[l], w_op[l], out_dtype, out=pre[l])
-        ctx.save_for_backward(x_op, w_op)
+        ctx.rows8_d = d if keep8 else None                                       # x is held in 8 bits for the weight gradient
+        ctx.save_for_backward(ops.quantize_rows(x_op.reshape(L * B, d)).data.view(L, B, -1) if keep8 else x_op, w_op)
         ctx.x_dtype, ctx.w_dtype = x.dtype, W_E.dtype
         return pre.permute(1, 0, 2)
 
@@ -241,14 +244,15 @@ class _LayerEncoderGemm(torch.autograd.Function):
     def backward(ctx, g):
         x_op, w_op = ctx.saved_tensors
         L = x_op.shape[0]
+        x_rows = x_op if ctx.rows8_d is None else [ops.Rows8(x_op[l], ctx.rows8_d) for l in range(L)]
         gl = g.permute(1, 0, 2).to(w_op.dtype).contiguous()                     # [L, B, F]
         dx = dW = None
         if ctx.needs_input_grad[0]:   # rare (activations carry no gradient in training): library products
             dx = torch.stack([gl[l] @ w_op[l] for l in range(L)], dim=1).to(ctx.x_dtype)
         if ctx.needs_input_grad[1]:
-            rows = torch.stack([_rows_over_tokens(gl[l], x_op[l], w_op.dtype) for l in range(L)])      # [L, F, d]
+            rows = torch.stack([_rows_over_tokens(gl[l], x_rows[l], w_op.dtype) for l in range(L)])      # [L, F, d]
             dW = rows.permute(0, 2, 1).to(ctx.w_dtype)
-        return dx, dW, None, None
+        return dx, dW, None, None, None
 
 
 class _PrefixDecode(torch.autograd.Function):
@@ -478,7 +482,8 @@ class CrossLayerTranscoder(SparseDictionary):
         if (x.is_cuda and self.W_E.is_cuda and tuple(x.shape[-2:]) == (L, d) and self.W_E.dtype in (torch.float32, torch.bfloat16)
                 and _gemm_k_ok(d, torch.bfloat16 if low else torch.float32)):
             lead = x.shape[:-2]
-            pre = _LayerEncoderGemm.apply(x.reshape(-1, L, d).to(self.W_E.dtype), self.W_E, self._w_enc_operand(amp), low)
+            pre = _LayerEncoderGemm.apply(x.reshape(-1, L, d).to(self.W_E.dtype), self.W_E, self._w_enc_operand(amp), low,
+                                          self._keep_rows8())
             return pre.reshape(*lead, L, F)
         return torch.einsum("...ld,lds->...ls", x, self.W_E)
 
@@ -568,7 +573,8 @@ class CrossLayerTranscoder(SparseDictionary):
 
         L, d, F = self.cfg.n_layers, self.cfg.d_model, self.cfg.d_sae
         amp = _autocast_dtype("cuda") == torch.bfloat16
-        pre = _LayerEncoderGemm.apply(x.to(self.W_E.dtype), self.W_E, self._w_enc_operand(amp), amp).permute(1, 0, 2)   # [L, B, F]
+        pre = _LayerEncoderGemm.apply(x.to(self.W_E.dtype), self.W_E, self._w_enc_operand(amp), amp,
+                                      self._keep_rows8()).permute(1, 0, 2)                     # [L, B, F]
         scaled = bool(self.cfg.sparsity_include_decoder_norm)
         norms = self._norm_per_feature_nograd() if (scaled or want_tanh) else None
         if self.cfg.act_fn.lower() == "jumprelu":

@@ -25,7 +25,7 @@ from torch import nn
 
 from . import ops
 from .config import CrosscoderConfig, register_sae_model
-from .sae import SparseRowGrad, _autocast_dtype
+from .sae import SparseRowGrad, _autocast_dtype, _input_operand
 from .sparse_dictionary import LazyDict, SparseDictionary
 
 
@@ -46,12 +46,8 @@ class _FusedCrosscoderStep(torch.autograd.Function):
         F = m.cfg.d_sae
         w_enc_op = m._w_enc_operand(amp)                              # [F, H*d]
         x_cat = x.reshape(B, H * d)
-        if amp:
-            x_op = x_cat if x_cat.dtype == torch.bfloat16 else ops.cast_bf16(x_cat.contiguous())
-            pre = ops.encoder_gemm(x_op, w_enc_op, torch.bfloat16)
-        else:
-            x_op = x_cat.contiguous()
-            pre = ops.encoder_gemm(x_op, w_enc_op, torch.float32)
+        x_op, x_kept = _input_operand(x_cat, amp, m.rows8_checkpoint)
+        pre = ops.encoder_gemm(x_op, w_enc_op, torch.bfloat16 if amp else torch.float32)
         norms = m._decoder_norm_nograd()                              # [H, F]
         w_dec_op = m._w_dec_operand(amp)                              # [H, F, d]
         b_sum = b_E.detach().sum(dim=0)
@@ -87,7 +83,7 @@ class _FusedCrosscoderStep(torch.autograd.Function):
         loss = loss_toks.sum()
         recon = recons.transpose(0, 1)                                   # [B, H, d]
         holder["codes"], holder["pre"], holder["norms"], holder["b_sum"] = codes, pre, norms, b_sum
-        ctx.codes, ctx.grads, ctx.dvals, ctx.x_op, ctx.w_enc_op = codes, grads, dvals, x_op, w_enc_op
+        ctx.codes, ctx.grads, ctx.dvals, ctx.x_rows, ctx.w_enc_op = codes, grads, dvals, x_kept, w_enc_op
         ctx.stacked = stacked
         ctx.amp = bool(amp)
         ctx.shape = (B, H, d, F)
@@ -128,7 +124,7 @@ class _FusedCrosscoderStep(torch.autograd.Function):
             idx_cat = torch.cat([c.idx + h * F for h, c in enumerate(ctx.codes)])
             cat_code = dataclasses.replace(stacked, idx=idx_cat, d_sae=H * F)
             m.W_D._sparse_grad = SparseRowGrad(ops.build_feature_index(cat_code), stacked.val * g, gd, H * F)
-            m.W_E._sparse_grad = SparseRowGrad(fi, coef, ctx.x_op, F)
+            m.W_E._sparse_grad = SparseRowGrad(fi, coef, ctx.x_rows, F)
             db_sum, _ = ops.feature_segment_sums(fi, coef)
             dW_E = dW_D = None
         else:
@@ -138,7 +134,7 @@ class _FusedCrosscoderStep(torch.autograd.Function):
                 rows, _ = ops.sparse_grad_rows(fi_h, ctx.codes[h].val * g, gd[h * B:(h + 1) * B], F)
                 dW_D.append(rows)
             dW_D = torch.stack(dW_D)
-            dW_Et, db_sum = ops.sparse_grad_rows(fi, coef, ctx.x_op, F, want_bias=True)                # [F, H*d], [F]
+            dW_Et, db_sum = ops.sparse_grad_rows(fi, coef, ctx.x_rows, F, want_bias=True)              # [F, H*d], [F]
             dW_E = dW_Et.view(F, H, d).permute(1, 2, 0)
         db_E = db_sum.unsqueeze(0).expand(H, F)
         dx = dlabel = None
@@ -269,7 +265,7 @@ class Crosscoder(SparseDictionary):
 
             lead = x.shape[:-2]
             pre = _EncoderGemm.apply(x.reshape(-1, H * d).to(self.W_E.dtype), self.W_E, self._w_enc_operand(amp), low, False, None,
-                                     lambda rows: rows.view(F, H, d).permute(1, 2, 0))
+                                     lambda rows: rows.view(F, H, d).permute(1, 2, 0), self._keep_rows8())
             return pre.view(*lead, F) + self.b_E.sum(dim=0)
         return (torch.einsum("...hd,hdf->...hf", x, self.W_E) + self.b_E).sum(dim=-2)
 

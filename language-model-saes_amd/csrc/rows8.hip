@@ -320,7 +320,8 @@ static int r8_window(int64_t n_slots, int64_t d) {
 // The first launch.  Workgroups below feat_blocks, a wave per feature: the feature of each of its positions, a zero row where
 // it has none, its coefficients' sum.  The others, a thread per position: token and coefficient in index order, so that the
 // waves of the second launch, one per window and chunk of columns, read them in line (by slot they would touch a cache line
-// per entry, once for every chunk).  Positions behind the last, up to a whole window, get feature -1.
+// per entry, once for every chunk).  Positions in front of the first feature's and behind the last's, up to a whole window, get
+// feature -1.
 __global__ __launch_bounds__(256) void rows8_grad_prepare_kernel(const int32_t *__restrict__ feat_ptr, const int32_t *__restrict__ feat_slot,
                                                                  const int32_t *__restrict__ slot_tok, const float *__restrict__ coef,
                                                                  int32_t *__restrict__ pos_feat, int32_t *__restrict__ pos_tok,
@@ -329,12 +330,12 @@ __global__ __launch_bounds__(256) void rows8_grad_prepare_kernel(const int32_t *
                                                                  int window) {
   if (blockIdx.x >= feat_blocks) {
     const int64_t i = (int64_t)(blockIdx.x - feat_blocks) * 256 + threadIdx.x;
-    const int total = feat_ptr[F];
-    if (i < total) {
+    const int first = feat_ptr[0], total = feat_ptr[F];   // the index may be a stretch of a longer one's features
+    if (i >= first && i < total) {
       const int slot = feat_slot[i];
       pos_tok[i] = slot_tok[slot];
       pos_coef[i] = coef[slot];
-    } else if (i < ((int64_t)total + window - 1) / window * window) {
+    } else if (i < first || i < ((int64_t)total + window - 1) / window * window) {
       pos_feat[i] = -1;
       pos_tok[i] = 0;
       pos_coef[i] = 0.f;
@@ -381,7 +382,7 @@ __global__ __launch_bounds__(256) void rows8_grad_window_kernel(const int32_t *_
   const int64_t chunk = task / n_windows, window = task % n_windows;
   const int total = feat_ptr[F];
   const int w0 = (int)(window * WINDOW), w1 = w0 + WINDOW;
-  if (w0 >= total) return;
+  if (w0 >= total || w1 <= feat_ptr[0]) return;
   const int64_t codes = r8_blocks(d) * R8_BLOCK;
   const uint32_t pitch = (uint32_t)r8_pitch(d);
   const int64_t col = chunk * R8_COLS + lane * 4;
@@ -453,7 +454,7 @@ __global__ __launch_bounds__(256) void rows8_grad_join_kernel(const int32_t *__r
   const int64_t w0 = window * length, w1 = w0 + length;
   if (w1 >= total) return;
   const int f = pos_feat[w1];
-  if (pos_feat[w1 - 1] != f || (w0 > 0 && pos_feat[w0 - 1] == f)) return;
+  if (f < 0 || pos_feat[w1 - 1] != f || (w0 > 0 && pos_feat[w0 - 1] == f)) return;
   const int64_t last = (feat_ptr[f + 1] - 1) / length, codes = r8_blocks(d) * R8_BLOCK;
   const int64_t j = ((int64_t)blockIdx.y * 256 + threadIdx.x) * 4;
   if (j >= d) return;

@@ -1481,9 +1481,10 @@ def _rows8_grad_rows(fi: FeatureIndex, coef: torch.Tensor, rows: Rows8, F: int, 
             ws.data_ptr(), nbytes)
 
 
-def restore_rows(src: Rows8, out_dtype: torch.dtype = torch.bfloat16, out: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """[n, d] values of all rows, in order (every value is exact in bf16)."""
-    return _read_rows8(src, None, out_dtype, 1.0, out)
+def restore_rows(src: Rows8, out_dtype: torch.dtype = torch.bfloat16, scale: float = 1.0,
+                 out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """[n, d] values of all rows, in order, times `scale` (every value is exact in bf16)."""
+    return _read_rows8(src, None, out_dtype, scale, out)
 
 
 def _transpose_padded(src, pitch: int) -> torch.Tensor:

@@ -51,9 +51,10 @@ class SparseRowGrad:
     """Gradient of a feature-major [F, d] weight in factored form:
     g[f, :] = sum over feature f's slots of coef[slot] * dense[token(slot), :].
     Produced by the fused backward when the optimiser can consume it directly (HipAdam), so the
-    dense gradient never has to be written to HBM.  `dense()` materialises it on demand."""
+    dense gradient never has to be written to HBM.  `dense()` materialises it on demand.
+    `dense_operand`: [tokens, d] fp32 / bf16, or rows held in 8 bits (`ops.Rows8`)."""
 
-    def __init__(self, fi: ops.FeatureIndex, coef: torch.Tensor, dense_operand: torch.Tensor, n_features: int,
+    def __init__(self, fi: ops.FeatureIndex, coef: torch.Tensor, dense_operand, n_features: int,
                  bias_param: Optional[torch.Tensor] = None, extra: Optional[ops.DenseRowBlock] = None):
         self.fi, self.coef, self.dense_operand, self.n_features, self.bias_param = fi, coef, dense_operand, n_features, bias_param
         self.extra = extra    # gradient rows held densely for some features (added to the factored part)
@@ -232,6 +233,19 @@ def _aux_dense_grads(blk, g_aux, x_op, amp: bool):
             "db_E": db_E[:nd].contiguous(), "dpre": dpre, "dA": dA, "A": A, "W_Et": blk["W_Et"]}
 
 
+def _input_operand(x: torch.Tensor, low: bool, keep8: bool):
+    """(x as the encoder's product reads it, x as the backward pass is to read it): bf16 under autocast and for bf16 weights,
+    fp32 otherwise; with `keep8` the second is held in 8 bits, written by the pass that rounds fp32 rows to bf16."""
+    if low and x.dtype != torch.bfloat16:
+        if keep8:
+            kept, x_op = ops.quantize_rows(x.float(), bf16_copy=True)
+            return x_op, kept
+        x_op = ops.cast_bf16(x.float().contiguous())
+    else:
+        x_op = x if low else x.float().contiguous()
+    return x_op, (ops.quantize_rows(x_op) if keep8 else x_op)
+
+
 class _FusedSparseStep(torch.autograd.Function):
     """encode -> TopK / BatchTopK -> decode -> masked-mean squared error (+ aux-k), forward and backward,
     in kernels.
@@ -269,17 +283,15 @@ class _FusedSparseStep(torch.autograd.Function):
                    and (ops.granule_route_supported(x.shape[1], w_enc_op.shape[0], int(k)) if not batch_wide
                         else x.shape[1] % 64 == 0 and w_enc_op.shape[0] % 256 == 0))
         gmax = None
+        x_op, x_kept = _input_operand(x, amp, sae.rows8_checkpoint)
         if granule:
-            x_op = x if x.dtype == torch.bfloat16 else ops.cast_bf16(x.contiguous())
             scale = sae._decoder_norm_nograd() if sae.cfg.sparsity_include_decoder_norm else None
             if lowp and scale is not None:
                 scale = scale.bfloat16().float()   # decoder_norm() of bf16 weights is a bf16 tensor
             pre, gmax = ops.encoder_gemm_granule_max(x_op, w_enc_op, b_E, scale, lowp=lowp)
         elif amp:
-            x_op = x if x.dtype == torch.bfloat16 else ops.cast_bf16(x.contiguous())
             pre = ops.encoder_gemm(x_op, w_enc_op, torch.bfloat16)
         else:
-            x_op = x.contiguous()
             pre = ops.encoder_gemm(x_op, w_enc_op, torch.float32)
         if not granule:
             # decoder-side operands are fetched after the GEMM is enqueued: an overlapped decoder update of the
@@ -298,7 +310,7 @@ class _FusedSparseStep(torch.autograd.Function):
             recon, loss_tok, grad_recon, dval = ops.sparse_decode_mse_fused(code, w_dec_op, b_D, label, tok_w)
             loss = loss_tok.sum()
             l_aux = None
-            grad_code, grad_dense_D, grad_coef_E, x_rows = code, grad_recon, dval, x_op
+            grad_code, grad_dense_D, grad_coef_E, x_rows = code, grad_recon, dval, x_kept
             ctx.aux_dense = None
         else:
             dead = aux["is_dead"](code)                       # bool [F], from the caller's dead statistics
@@ -328,7 +340,7 @@ class _FusedSparseStep(torch.autograd.Function):
                 dval = ops.sparse_decode_bwd_dval(code, grad_recon, w_dec_op)
                 if g_aux is not None:
                     ctx.aux_dense = _aux_dense_grads(blk, g_aux, x_op, amp)
-                grad_code, grad_dense_D, grad_coef_E, x_rows = code, grad_recon, dval, x_op
+                grad_code, grad_dense_D, grad_coef_E, x_rows = code, grad_recon, dval, x_kept
                 holder.aux_code = blk["code"]
             else:
                 dead_f = dead.to(torch.float32)
@@ -357,7 +369,8 @@ class _FusedSparseStep(torch.autograd.Function):
                 grad_code = ops.stack_codes(code, aux_code)
                 grad_dense_D = torch.cat([grad_recon, g_aux])
                 grad_coef_E = torch.cat([dval, dval_aux])
-                x_rows = torch.cat([x_op, x_op])
+                x_rows = (ops.Rows8(torch.cat([x_kept.data, x_kept.data]), x_kept.d) if isinstance(x_kept, ops.Rows8)
+                          else torch.cat([x_kept, x_kept]))
                 holder.aux_code = aux_code
         if amp:
             # the decoder's weight gradient pairs the activations with the bf16-rounded output gradient, as the
@@ -447,7 +460,7 @@ class _GluSparseStep(torch.autograd.Function):
     def forward(ctx, x, label, tok_w, W_E, b_E, W_G, b_G, W_D, b_D, k, amp, holder):
         sae = holder.model
         w_enc_op, w_glu_op = sae._w_enc_operand(amp), sae._w_glu_operand(amp)
-        x_op = (x if x.dtype == torch.bfloat16 else ops.cast_bf16(x.contiguous())) if amp else x.contiguous()
+        x_op, x_kept = _input_operand(x, amp, sae.rows8_checkpoint)
         out_dtype = torch.bfloat16 if amp else torch.float32
         pre, pre_g = ops.encoder_gemm(x_op, w_enc_op, out_dtype), ops.encoder_gemm(x_op, w_glu_op, out_dtype)
         lin = pre.float() + b_E
@@ -465,7 +478,7 @@ class _GluSparseStep(torch.autograd.Function):
         zero = torch.zeros((), dtype=torch.float32, device=x.device)
         ctx.lin = torch.where(valid, lin.flatten()[cell], zero)                    # per kept entry
         ctx.gate = torch.where(valid, gate.flatten()[cell], zero)
-        ctx.code, ctx.x_op, ctx.grad_recon, ctx.dval, ctx.w_enc_op, ctx.w_glu_op = code, x_op, grad_recon, dval, w_enc_op, w_glu_op
+        ctx.code, ctx.x_rows, ctx.grad_recon, ctx.dval, ctx.w_enc_op, ctx.w_glu_op = code, x_kept, grad_recon, dval, w_enc_op, w_glu_op
         ctx.amp, ctx.has_b_D = bool(amp), b_D is not None
         holder.code, holder.hidden, holder.scale = code, hidden, scale
         ctx.mark_non_differentiable(recon)
@@ -485,8 +498,8 @@ class _GluSparseStep(torch.autograd.Function):
         dW_D, _ = ops.sparse_grad_rows(fi, code.val * g, gd, F)
         d_hidden = ctx.dval * g                     # kept entries are positive and the norm's two terms cancel
         c_enc, c_glu = d_hidden * ctx.gate, d_hidden * ctx.lin * ctx.gate * (1.0 - ctx.gate)
-        dW_Et, db_E = ops.sparse_grad_rows(fi, c_enc, ctx.x_op, F, want_bias=True)
-        dW_Gt, db_G = ops.sparse_grad_rows(fi, c_glu, ctx.x_op, F, want_bias=True)
+        dW_Et, db_E = ops.sparse_grad_rows(fi, c_enc, ctx.x_rows, F, want_bias=True)
+        dW_Gt, db_G = ops.sparse_grad_rows(fi, c_glu, ctx.x_rows, F, want_bias=True)
         db_D = ops.col_sum(ctx.grad_recon) * g if ctx.has_b_D else None
         dx = None
         if ctx.needs_input_grad[0]:
@@ -508,10 +521,12 @@ def _gemm_k_ok(k: int, dtype: torch.dtype) -> bool:
     return k % (64 if dtype == torch.bfloat16 else 32) == 0
 
 
-def _rows_over_tokens(left: torch.Tensor, right: torch.Tensor, out_dtype: torch.dtype) -> torch.Tensor:
+def _rows_over_tokens(left, right, out_dtype: torch.dtype) -> torch.Tensor:
     """left^T @ right for left [B, m], right [B, n] -> [m, n]: a product over the token axis (a weight gradient).  bf16
     operands are read as they lie (both are stored [K, rows] for this product); fp32 operands are transposed first, for
-    the fp32 kernel contracts over the contiguous axis of both."""
+    the fp32 kernel contracts over the contiguous axis of both.  Either operand may be held in 8 bits."""
+    if isinstance(left, ops.Rows8) or isinstance(right, ops.Rows8):
+        return ops.gemm_over_tokens(*(t if isinstance(t, ops.Rows8) else t.contiguous() for t in (left, right)), out_dtype)
     if (left.dtype == torch.bfloat16 and right.dtype == torch.bfloat16 and left.shape[0] % 64 == 0 and left.shape[1] % 8 == 0
             and right.shape[1] % 8 == 0):
         return ops.gemm(left.contiguous(), right.contiguous(), out_dtype, a_k_major=True, b_k_major=True)
@@ -526,18 +541,17 @@ class _EncoderGemm(torch.autograd.Function):
     kernel."""
 
     @staticmethod
-    def forward(ctx, x, W_E, w_op, amp, defer=False, given=None, grad_view=None):
+    def forward(ctx, x, W_E, w_op, amp, defer=False, given=None, grad_view=None, keep8=False):
         # grad_view: maps the gradient rows [F, K] (K = x's width) to the parameter's shape, for encoder weights that
         # are not a [d, F] view of a [F, d] buffer (a crosscoder's [H, d, F] over [F, H, d])
-        if given is not None:             # (x operand, product) computed by the caller already
-            x_op, pre = given
-        elif amp:
-            x_op = x if x.dtype == torch.bfloat16 else ops.cast_bf16(x.float().contiguous())
-            pre = ops.encoder_gemm(x_op, w_op, torch.bfloat16)
+        # keep8: x is held in 8 bits for the weight gradient
+        if given is not None:             # (x operand, x for the backward pass, product) computed by the caller already
+            _x_op, kept, pre = given
         else:
-            x_op = x.float().contiguous()
-            pre = ops.encoder_gemm(x_op, w_op, torch.float32)
-        ctx.save_for_backward(x_op, w_op)
+            x_op, kept = _input_operand(x, amp, keep8)
+            pre = ops.encoder_gemm(x_op, w_op, torch.bfloat16 if amp else torch.float32)
+        ctx.rows8_d = kept.d if isinstance(kept, ops.Rows8) else None
+        ctx.save_for_backward(kept if ctx.rows8_d is None else kept.data, w_op)
         ctx.x_dtype, ctx.w_dtype = x.dtype, W_E.dtype
         # a bf16 weight gradient can stay bf16 until the optimiser reads it, when the parameter is stored feature-major
         ctx.param = W_E if (defer and amp and W_E.ndim == 2 and W_E.stride() == (1, W_E.shape[0])) else None
@@ -547,6 +561,8 @@ class _EncoderGemm(torch.autograd.Function):
     @staticmethod
     def backward(ctx, g):
         x_op, w_op = ctx.saved_tensors
+        if ctx.rows8_d is not None:
+            x_op = ops.Rows8(x_op, ctx.rows8_d)
         gg = g.to(w_op.dtype)
         # the input's gradient is rarely wanted (activations carry none in training): a library product
         dx = (gg @ w_op).to(ctx.x_dtype) if ctx.needs_input_grad[0] else None
@@ -559,7 +575,7 @@ class _EncoderGemm(torch.autograd.Function):
                 dW = ctx.grad_view(rows).to(ctx.w_dtype)
             else:
                 dW = rows.t().to(ctx.w_dtype)                                      # [d, F] with feature-major strides
-        return dx, dW, None, None, None, None, None
+        return dx, dW, None, None, None, None, None, None
 
 
 def _leave_lowp_grad(param, rows: torch.Tensor) -> None:
@@ -601,9 +617,10 @@ class _DenseDecode(torch.autograd.Function):
     Backward: d acts = g W_D^T contracts over d_model (W_D as it is), dW_D = acts^T g over the tokens."""
 
     @staticmethod
-    def forward(ctx, acts, W_D, w_op, w_t=None, defer=False):
+    def forward(ctx, acts, W_D, w_op, w_t=None, defer=False, keep8=False):
         acts = acts.contiguous()
-        ctx.save_for_backward(acts, w_op)
+        ctx.rows8_d = acts.shape[1] if keep8 else None          # the activations are held in 8 bits for the weight gradient
+        ctx.save_for_backward(ops.quantize_rows(acts).data if keep8 else acts, w_op)
         ctx.param = W_D if (defer and W_D.is_contiguous() and w_op.dtype == torch.bfloat16) else None
         ctx.w_dtype = W_D.dtype
         if w_t is None:
@@ -613,6 +630,8 @@ class _DenseDecode(torch.autograd.Function):
     @staticmethod
     def backward(ctx, g):
         acts, w_op = ctx.saved_tensors
+        if ctx.rows8_d is not None:
+            acts = ops.Rows8(acts, ctx.rows8_d)
         gg = g.to(w_op.dtype).contiguous()
         d_acts = ops.encoder_gemm(gg, w_op, w_op.dtype) if ctx.needs_input_grad[0] else None
         dW = None
@@ -622,7 +641,7 @@ class _DenseDecode(torch.autograd.Function):
                 _leave_lowp_grad(ctx.param, rows)
             else:
                 dW = rows.to(ctx.w_dtype)
-        return d_acts, dW, None, None, None
+        return d_acts, dW, None, None, None, None
 
 
 def dense_decode(model, acts: torch.Tensor, W_D: torch.Tensor, w_op: torch.Tensor, w_t_name: str, defer: bool = False):
@@ -637,11 +656,11 @@ def dense_decode(model, acts: torch.Tensor, W_D: torch.Tensor, w_op: torch.Tenso
     # the forward contracts over F, the backward's d acts = g W_D^T over d: both must be whole slabs of the kernel
     if w_op.dtype == torch.bfloat16:
         if F % 64 == 0 and d % 64 == 0:
-            return _DenseDecode.apply(acts, W_D, w_op, None, defer)
+            return _DenseDecode.apply(acts, W_D, w_op, None, defer, model._keep_rows8())
         return None
     if w_op.dtype == torch.float32 and F % 32 == 0 and d % 32 == 0:
         w_t = model._derive(w_t_name, W_D, lambda old: _transposed(w_op))
-        return _DenseDecode.apply(acts, W_D, w_op, w_t, defer)
+        return _DenseDecode.apply(acts, W_D, w_op, w_t, defer, model._keep_rows8())
     return None
 
 
@@ -779,17 +798,17 @@ class _JumpReLUSparseStep(torch.autograd.Function):
         else:
             d_norm = ops.feature_segment_sums(fi, dn_slot)[0] if dn_slot is not None else None
         coef_dec, coef_enc = val * g, d_pre * g
-        x_op = h["x_op"]
+        x_rows = h["x_rows"]
         grad_dense_D = ops.cast_bf16(grad_recon) if h["amp"] else grad_recon
         db_D = ops.col_sum(grad_recon) * g if ctx.has_b_D else None
         defer = h["defer"]
         if defer and all(getattr(p, "_sparse_grad", None) is None and p.grad is None for p in (sae.W_D, sae.W_E)):
             sae.W_D._sparse_grad = SparseRowGrad(fi, coef_dec, grad_dense_D, F)
-            sae.W_E._sparse_grad = SparseRowGrad(fi, coef_enc, x_op, F, bias_param=sae.b_E)
+            sae.W_E._sparse_grad = SparseRowGrad(fi, coef_enc, x_rows, F, bias_param=sae.b_E)
             dW_D = dW_E = db_E = None
         else:
             dW_D, _ = ops.sparse_grad_rows(fi, coef_dec, grad_dense_D, F)
-            dW_Et, db_E = ops.sparse_grad_rows(fi, coef_enc, x_op, F, want_bias=True)
+            dW_Et, db_E = ops.sparse_grad_rows(fi, coef_enc, x_rows, F, want_bias=True)
             dW_E = dW_Et.t()
         return (d_theta, None if d_norm is None or not ctx.needs_input_grad[1] else d_norm * g,
                 dW_E, db_E, dW_D, db_D, None, None, None)
@@ -951,7 +970,7 @@ class SparseAutoEncoder(SparseDictionary):
                 name = "W_E.bf16" if W is self.W_E else ("W_E_glu.bf16" if W is getattr(self, "W_E_glu", None) else None)
                 wt = self._derive(name, W, lambda old: ops.cast_bf16(wt, old)) if name is not None else ops.cast_bf16(wt)
             lead = x.shape[:-1]
-            pre = _EncoderGemm.apply(x.reshape(-1, d), W, wt, low)
+            pre = _EncoderGemm.apply(x.reshape(-1, d), W, wt, low, False, None, None, self._keep_rows8())
             return pre.view(*lead, pre.shape[-1])
         return x @ W
 
@@ -1118,7 +1137,7 @@ class SparseAutoEncoder(SparseDictionary):
         if (self.jumprelu_sparse_route and not want_lp and B <= 131072
                 and self.cfg.d_model % 8 == 0 and self._jr_dense_steps % max(1, self.jumprelu_sparse_probe_every) == 0):
             with torch.no_grad():
-                x_op = (x if x.dtype == torch.bfloat16 else ops.cast_bf16(x.float().contiguous())) if amp else x.float().contiguous()
+                x_op, x_kept = _input_operand(x, amp, self.rows8_checkpoint)
                 n_raw = self._decoder_norm_nograd() if (scaled or sparsity_loss_type is not None) else None
                 th_raw = theta.detach().float().contiguous()
                 b_raw = self.b_E.detach().float()
@@ -1130,7 +1149,7 @@ class SparseAutoEncoder(SparseDictionary):
                     pre_raw, margin = ops.encoder_gemm_jumprelu_margin(x_op, w_enc_op, b_raw, n_raw if scaled else None, th_raw)
                 else:
                     pre_raw = ops.encoder_gemm(x_op, w_enc_op, torch.bfloat16 if amp else torch.float32)
-                given = (x_op, pre_raw)
+                given = (x_op, x_kept, pre_raw)
                 budget = int(B * self.cfg.d_sae * (1.0 - self.cfg.sparsity_threshold_for_triton_spmm_kernel))
                 picked = ops.jumprelu_select(pre_raw, b_raw, n_raw if scaled else None, th_raw, window,
                                              float(tanh_stretch_coefficient), pen_norm=n_raw,
@@ -1138,11 +1157,11 @@ class SparseAutoEncoder(SparseDictionary):
             if picked is not None:
                 self._jr_dense_steps = 0
                 code, win, tanh_tok, _l0 = picked
-                return self._sparse_code_loss(batch, label, mask, code, win, x_op, pre_raw, amp, defer, theta, window,
+                return self._sparse_code_loss(batch, label, mask, code, win, x_kept, pre_raw, amp, defer, theta, window,
                                               sparsity_loss_type, tanh_tok, float(tanh_stretch_coefficient), float(l1_coefficient),
                                               float(frequency_scale), p, lp_coefficient, auxk_coefficient, return_aux_data)
         self._jr_dense_steps += 1
-        pre = _EncoderGemm.apply(x, self.W_E, w_enc_op, amp, defer, given)
+        pre = _EncoderGemm.apply(x, self.W_E, w_enc_op, amp, defer, given, None, self._keep_rows8())
         n = None
         want_dense_pen = sparsity_loss_type in ("power", "tanh-quad")
         if scaled or want_tanh or want_lp or want_dense_pen:
@@ -1185,7 +1204,7 @@ class SparseAutoEncoder(SparseDictionary):
                 "hidden_pre": lambda: pre.detach().float() + b_E}
         return LazyDict(eager, lazy)
 
-    def _sparse_code_loss(self, batch, label, mask, code, win, x_op, pre_raw, amp, defer, theta, window, sparsity_loss_type,
+    def _sparse_code_loss(self, batch, label, mask, code, win, x_rows, pre_raw, amp, defer, theta, window, sparsity_loss_type,
                           pen_tok, tanh_c, l1_coefficient, frequency_scale, p, lp_coefficient, auxk_coefficient, return_aux_data):
         """Loss of a step whose activations are the sparse code `code` (JumpReLU / ReLU above the sparsity gate, or a TopK
         family selection) with an optional sparsity penalty, through `_JumpReLUSparseStep`."""
@@ -1202,7 +1221,7 @@ class SparseAutoEncoder(SparseDictionary):
         has_theta = self.cfg.act_fn.lower() == "jumprelu"
         if win is None:
             win = torch.zeros_like(code.val)
-        holder = {"model": self, "code": code, "win": win, "pen": sparsity_loss_type, "pen_tok": pen_tok, "x_op": x_op, "amp": amp,
+        holder = {"model": self, "code": code, "win": win, "pen": sparsity_loss_type, "pen_tok": pen_tok, "x_rows": x_rows, "amp": amp,
                   "defer": defer, "scaled": scaled, "tanh_c": tanh_c, "l1": l1_coefficient, "window": window, "p": p,
                   "frequency_scale": frequency_scale, "has_theta": has_theta}
         loss, recon = _JumpReLUSparseStep.apply(theta, n, self.W_E, self.b_E, self.W_D,
@@ -1227,16 +1246,16 @@ class SparseAutoEncoder(SparseDictionary):
 
     @torch.no_grad()
     def _select_code(self, x: torch.Tensor, amp: bool):
-        """GEMM + TopK / BatchTopK select of an fp32 dictionary -> (x operand, pre, code): what the forward of the fused
-        step does, for the routes that continue from the code with other losses."""
+        """GEMM + TopK / BatchTopK select of an fp32 dictionary -> (x for the backward pass, pre, code): what the forward of
+        the fused step does, for the routes that continue from the code with other losses."""
         w_enc_op = self._w_enc_operand(amp)
         B, k = x.shape[0], int(self.current_k)
         batch_wide = self.cfg.act_fn.lower() == "batchtopk"
         b_E = self.b_E.detach().float()
         scale = self._decoder_norm_nograd() if self.cfg.sparsity_include_decoder_norm else None
         gmax = None
+        x_op, x_kept = _input_operand(x, amp, self.rows8_checkpoint)
         if amp:
-            x_op = x if x.dtype == torch.bfloat16 else ops.cast_bf16(x.float().contiguous())
             granule = (getattr(self, "granule_select", True)
                        and (ops.granule_route_supported(x.shape[1], w_enc_op.shape[0], k) if not batch_wide
                             else x.shape[1] % 64 == 0 and w_enc_op.shape[0] % 256 == 0))
@@ -1245,13 +1264,12 @@ class SparseAutoEncoder(SparseDictionary):
             else:
                 pre = ops.encoder_gemm(x_op, w_enc_op, torch.bfloat16)
         else:
-            x_op = x.float().contiguous()
             pre = ops.encoder_gemm(x_op, w_enc_op, torch.float32)
         if batch_wide:
             code = ops.select_topk_batch(pre, b_E, scale, k * B, granule_max=gmax)
         else:
             code = ops.select_topk_row(pre, b_E, scale, k, granule_max=gmax)
-        return x_op, pre, code
+        return x_kept, pre, code
 
     def _flattened_loss(self, batch, x, label, kw):
         """[batch, seq_len, d_model] activations (models/sae.py:288-345 takes both forms): every loss term is a (masked) mean
@@ -1318,11 +1336,11 @@ class SparseAutoEncoder(SparseDictionary):
             # TopK / BatchTopK with a sparsity penalty: select as the plain step does, then decode, loss, penalty and the
             # backward on the code (the penalty's gradient joins the decoder's at every kept entry and reaches W_D
             # through the decoder norm)
-            x_op, pre, code = self._select_code(x, amp)
+            x_rows, pre, code = self._select_code(x, amp)
             defer = bool(self.defer_weight_grads and torch.is_grad_enabled())
             theta, window = self._threshold_and_window() if self.cfg.act_fn.lower() == "jumprelu" else (
                 torch.zeros(1, dtype=torch.float32, device=x.device), 1.0)
-            return self._sparse_code_loss(batch, label, mask, code, None, x_op, pre, amp, defer, theta, window, sparsity_loss_type,
+            return self._sparse_code_loss(batch, label, mask, code, None, x_rows, pre, amp, defer, theta, window, sparsity_loss_type,
                                           None, float(tanh_stretch_coefficient), float(l1_coefficient), float(frequency_scale), p,
                                           lp_coefficient, auxk_coefficient, return_aux_data)
         if mask is None:

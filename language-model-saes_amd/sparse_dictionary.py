@@ -72,6 +72,14 @@ class LazyDict(dict):
 
 
 class SparseDictionary(nn.Module):
+    # True: what the backward pass of a step reads of its inputs, and of dense activations, is held in 8 bits between the
+    # two passes (`ops.Rows8`): half the bytes of bf16 rows, a quarter of fp32 ones.  The forward pass is unchanged; of the
+    # gradients the encoder's weights change (and, where activations are dense, the decoder's), by the rounding of the rows
+    # they are summed over.  Inputs that 8 bits hold exactly (a batch read from an 8-bit buffer without a scale) give the
+    # same gradients.  Taken by the kernel steps of SparseAutoEncoder, Crosscoder and CrossLayerTranscoder, and by the
+    # encoder and decoder products of their `encode` / `decode`.
+    rows8_checkpoint: bool = False
+
     def __init__(self, cfg: SparseDictionaryConfig, device_mesh=None):
         super().__init__()
         if device_mesh is not None:
@@ -83,6 +91,10 @@ class SparseDictionary(nn.Module):
         self.activation_function = self.activation_function_factory(None)
         # derived operands (bf16 shadows, row norms) keyed by name -> (param version, tensor)
         self._derived: dict[str, tuple[int, torch.Tensor]] = {}
+
+    def _keep_rows8(self) -> bool:
+        """Whether a product outside the kernel steps is to hold its saved side in 8 bits."""
+        return self.rows8_checkpoint and torch.is_grad_enabled()
 
     # ---- derived operands, refreshed when the parameter's version counter moves ----
     def _derive(self, name: str, param: torch.Tensor, make) -> torch.Tensor:

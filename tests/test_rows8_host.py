@@ -69,3 +69,167 @@ def test_entry_points_refuse_before_any_launch(pkg):
     assert rows(r=None) == -1 and rows(out=None) == -1 and rows(F=0) == -1 and rows(d=0) == -1 and rows(n=0) == -1
     assert rows(r=P + 8) == -1 and rows(ws=None) == -4 and rows(b=need - 1) == -4 and rows(d=1 << 30) == -2 and rows(n=(1 << 31) - 1) == -2
     assert lib.sae_sparse_grad_rows(P, P, P, P, P, 2, P, None, 4, 40, None) == -1      # records have their own entry point
+
+
+# ---- records made and read without a GPU; the pipeline that carries them -----------------------------------------------
+
+def exact_values(x):
+    """[n, d] fp64: what 8 bits hold of x, block by block, from the definition."""
+    import numpy as np
+
+    x = x.double().numpy()
+    out = np.zeros_like(x)
+    for i in range(x.shape[0]):
+        for b in range(0, x.shape[1], 32):
+            block = x[i, b : b + 32]
+            if not np.isfinite(block).all():
+                out[i, b : b + 32] = np.nan
+                continue
+            top = np.abs(block).max()
+            if top == 0:
+                continue
+            k = max(int(np.floor(np.log2(top))) - 6, -126)
+            k += np.rint(np.ldexp(top, -k)) > 127 and k < 121
+            out[i, b : b + 32] = np.ldexp(np.clip(np.rint(np.ldexp(block, -k)), -127, 127), k)
+    return torch.from_numpy(out)
+
+
+def rows(n, d, seed, dtype=torch.float32):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn(n, d, generator=g) * torch.exp(2 * torch.randn(n, 1, generator=g))).to(dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("n,d", [(1, 1), (5, 32), (7, 33), (4, 100), (3, 768)])
+def test_pack_and_unpack_on_the_cpu(pkg, n, d, dtype):
+    x = rows(n, d, 1, dtype)
+    data = pkg.rows8_pack(x)
+    assert data.dtype == torch.uint8 and tuple(data.shape) == (n, pkg.ops.rows8_pitch(d))
+    assert not data[:, 33 * (-(-d // 32)):].any()
+    back = pkg.rows8_unpack(data, d, torch.float32)
+    assert torch.equal(back.double(), exact_values(x))
+    assert torch.equal(pkg.rows8_unpack(data, d, torch.bfloat16).float(), back)
+    assert torch.equal(pkg.rows8_unpack(data, d, torch.float32, 0.3), back * 0.3)
+    assert torch.equal(pkg.rows8_pack(back), data) or torch.equal(pkg.rows8_unpack(pkg.rows8_pack(back), d, torch.float32), back)
+    stacked = pkg.rows8_pack(x.view(1, n, d))
+    assert tuple(stacked.shape) == (1, n, data.shape[1]) and torch.equal(stacked[0], data)
+    assert torch.equal(pkg.rows8_unpack(stacked, d, torch.float32)[0], back)
+
+
+def test_pack_extremes_on_the_cpu(pkg):
+    top = torch.finfo(torch.float32).max
+    x = torch.zeros(10, 64)
+    x[:, 0] = torch.tensor([float("inf"), float("nan"), top, -top, 2.0**-126, 1e-44, 0.0, -0.0, 127.5 / 64, 2.0**-121])
+    x[:, 40] = 1.0
+    back = pkg.rows8_unpack(pkg.rows8_pack(x), 64, torch.float32)
+    assert back[:2, :32].isnan().all() and torch.isfinite(back[2:]).all() and (back[:, 40] == 1).all()
+    assert torch.equal(back[2:].double(), exact_values(x[2:]))
+
+
+def test_pack_refuses_other_rows(pkg):
+    for bad in (torch.zeros(3, 4, dtype=torch.float64), torch.zeros(3, 4, dtype=torch.int32), torch.zeros(3, 0)):
+        with pytest.raises(ValueError):
+            pkg.rows8_pack(bad)
+    with pytest.raises(ValueError):
+        pkg.rows8_unpack(torch.zeros(3, 48, dtype=torch.uint8), 40, torch.float32)
+
+
+def samples(n, ctx, d, dtype=torch.float32):
+    for i in range(n):
+        t = torch.arange(ctx)[None] + 100 * i
+        yield {"h0": rows(ctx, d, 10 + i, dtype)[None], "h1": rows(ctx, d + 3, 50 + i, dtype)[None], "tokens": t,
+               "mask": (t % 5 != 0).to(torch.int64), "attention_mask": torch.ones_like(t), "meta": {"i": i}}
+
+
+@pytest.mark.parametrize("fmt", ["safetensors", "pt"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_written_and_loaded(pkg, tmp_path, fmt, dtype):
+    hooks = ["h0", "h1"]
+    pkg.ActivationWriter(pkg.ActivationWriterConfig(cache_dir=str(tmp_path / "q"), hook_points=hooks, n_samples_per_chunk=2, format=fmt,
+                                                    row_format="rows8")).process(samples(5, 9, 70, dtype))
+    pkg.ActivationWriter(pkg.ActivationWriterConfig(cache_dir=str(tmp_path / "f"), hook_points=hooks, n_samples_per_chunk=2, format=fmt)
+                         ).process(samples(5, 9, 70, dtype))
+    dirs = lambda k: {hp: tmp_path / k / hp for hp in hooks}  # noqa: E731
+    floats = list(pkg.CachedActivationLoader(dirs("f")).process())
+    loader = pkg.CachedActivationLoader(dirs("q"))
+    got = list(loader.process())
+    kept_loader = pkg.CachedActivationLoader(dirs("q"), keep_rows8=True)
+    kept = list(kept_loader.process())
+    wide = list(pkg.CachedActivationLoader(dirs("q"), dtype=torch.float32).process())
+    assert len(got) == len(floats) == 3 and kept_loader.rows8_widths == {"h0": 70, "h1": 73}
+    for a, b, c, w in zip(got, floats, kept, wide):
+        assert torch.equal(a["tokens"], b["tokens"]) and a["meta"] == b["meta"]
+        for hp, d in (("h0", 70), ("h1", 73)):
+            want = exact_values(b[hp].reshape(-1, d)).view(b[hp].shape)
+            assert a[hp].dtype == dtype and w[hp].dtype == torch.float32 and torch.equal(w[hp].double(), want)
+            assert torch.equal(a[hp], want.to(dtype))
+            assert c[hp].dtype == torch.uint8 and tuple(c[hp].shape) == (*b[hp].shape[:-1], pkg.ops.rows8_pitch(d))
+
+
+def test_stream_of_records_gives_the_rows_they_hold(pkg, tmp_path):
+    """Shuffled batches out of a buffer of records = the same draws out of a buffer of the values."""
+    hooks = ["h0", "h1"]
+    pkg.ActivationWriter(pkg.ActivationWriterConfig(cache_dir=str(tmp_path), hook_points=hooks, n_samples_per_chunk=2, row_format="rows8")
+                         ).process(samples(7, 12, 70))
+    kw = dict(batch_size=10, buffer_size=30, buffer_shuffle_config=pkg.BufferShuffleConfig(perm_seed=3), device="cpu")
+    plain = list(pkg.cached_activation_stream(tmp_path, hooks, **kw))
+    held = list(pkg.cached_activation_stream(tmp_path, hooks, rows8=True, **kw))
+    low = list(pkg.cached_activation_stream(tmp_path, hooks, rows8=True, dtype=torch.float32, **kw))
+    over = list(pkg.cached_activation_stream(tmp_path, hooks, rows8=True, override_dtype=torch.float16, **kw))
+    assert len(plain) == len(held) == len(low) == len(over) > 4
+    for a, b, c, o in zip(plain, held, low, over):
+        assert torch.equal(a["tokens"], b["tokens"])
+        for hp in hooks:
+            assert b[hp].dtype == torch.bfloat16 and c[hp].dtype == torch.float32 and o[hp].dtype == torch.float16
+            assert torch.equal(b[hp].float(), a[hp]) and torch.equal(c[hp], a[hp]) and torch.equal(o[hp], a[hp].half())
+
+
+def test_buffer_that_quantises_what_arrives(pkg):
+    data = [{"x": rows(n, 45, n), "y": torch.arange(n)} for n in (7, 20, 3, 31)]
+    kw = dict(buffer_size=24, buffer_shuffle_config=pkg.BufferShuffleConfig(perm_seed=1))
+    plain = list(pkg.ActivationBatchler(6, **kw).process(data))
+    held = list(pkg.ActivationBatchler(6, rows8={"x": 45}, **kw).process(data))
+    scaled = list(pkg.ActivationBatchler(6, rows8={"x": 45}, scale=0.5, override_dtype=torch.bfloat16, **kw).process(data))
+    assert len(plain) == len(held) == len(scaled)
+    for a, b, c in zip(plain, held, scaled):
+        want = exact_values(a["x"])
+        assert torch.equal(a["y"], b["y"]) and b["x"].dtype == torch.float32 and torch.equal(b["x"].double(), want)
+        assert c["x"].dtype == torch.bfloat16 and torch.equal(c["x"], (want * 0.5).to(torch.bfloat16))
+    mixed = [data[0], {"x": pkg.rows8_pack(data[1]["x"]), "y": data[1]["y"]}]
+    out = torch.cat([b["x"] for b in pkg.ActivationBatchler(9, rows8={"x": 45}).process(mixed)])
+    assert torch.equal(out.double(), exact_values(torch.cat([data[0]["x"], data[1]["x"]])))
+
+
+def test_buffer_refusals(pkg):
+    go = lambda *chunks: list(pkg.ActivationBatchler(4, rows8={"x": 45}).process([{"x": c} for c in chunks]))  # noqa: E731
+    for bad in (rows(5, 44, 0), torch.zeros(5, 45, dtype=torch.int32), rows(5, 45, 0)[:, None], torch.zeros(5, 64, dtype=torch.uint8)):
+        with pytest.raises(ValueError):
+            go(bad)
+        with pytest.raises((ValueError, AssertionError)):
+            go(rows(5, 45, 0), bad)
+    with pytest.raises(ValueError):
+        go(rows(5, 45, 0), torch.zeros(5, 1, dtype=torch.uint8))
+
+
+def test_loader_refuses_files_that_disagree(pkg, tmp_path):
+    from safetensors.torch import load_file, save_file
+
+    w = lambda **kw: pkg.ActivationWriter(pkg.ActivationWriterConfig(cache_dir=str(tmp_path), hook_points=["h0"], **kw))  # noqa: E731
+    w(row_format="rows8").process(samples(2, 4, 40))
+    second = tmp_path / "h0" / "chunk-00000001.safetensors"
+    good = load_file(str(second))
+    load = lambda: list(pkg.CachedActivationLoader({"h0": tmp_path / "h0"}).process())  # noqa: E731
+    assert len(load()) == 2
+    for change in ({"activation_width": torch.tensor([41, 0])}, {"activation_width": torch.tensor([80, 0])},
+                   {"activation_width": torch.tensor([40, 9])}, {"activation": torch.zeros(1, 4, 40)},
+                   {"activation": torch.zeros(1, 4, 48, dtype=torch.uint8), "activation_width": torch.tensor([20, 0])}):
+        save_file(good | change, str(second))
+        with pytest.raises(ValueError, match="cached activation"):
+            load()
+    save_file({k: v for k, v in good.items() if k != "activation_width"}, str(second))
+    with pytest.raises(ValueError, match="float rows after"):
+        load()
+    with pytest.raises(ValueError):
+        w(row_format="rows8").process([{"h0": torch.zeros(1, 4, 8, dtype=torch.float64), "tokens": torch.zeros(1, 4)}])
+    with pytest.raises(ValueError):
+        w(row_format="int4")
