@@ -51,7 +51,7 @@ def rows8_pack(x: torch.Tensor) -> torch.Tensor:
     if x.dtype not in _FLOAT_CODES or d < 1:
         raise ValueError(f"rows held in 8 bits are made of fp32, bf16 or fp16 rows [..., d], got {x.dtype} {tuple(x.shape)}")
     pitch = ops.rows8_pitch(d)
-    rows = x.reshape(-1, d) if x.dtype == torch.bfloat16 else x.reshape(-1, d).float()
+    rows = (x.reshape(-1, d) if x.dtype == torch.bfloat16 else x.reshape(-1, d).float()).contiguous()
     if rows.is_cuda:
         return ops.quantize_rows(rows).data.view(*lead, pitch)
     nb = -(-d // ops.ROWS8_BLOCK)
@@ -414,7 +414,8 @@ class _RowStore:
             if rows.ndim != 2 or rows.shape[1] != (self.width if rows.dtype != torch.uint8 else self.data.shape[1]):
                 raise ValueError(f"{rows.dtype} rows {tuple(rows.shape)} in a buffer of 8-bit rows of {self.width} values")
         if self.width is not None and rows.dtype != torch.uint8:
-            if rows.is_cuda and rows.dtype in (torch.float32, torch.bfloat16) and int(slots_host[-1]) - first == n - 1:
+            if (rows.is_cuda and rows.dtype in (torch.float32, torch.bfloat16) and rows.stride(1) == 1
+                    and int(slots_host[-1]) - first == n - 1):
                 ops.quantize_rows(rows, out=self.data[first:first + n])
                 return
             rows = rows8_pack(rows)

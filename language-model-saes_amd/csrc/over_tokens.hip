@@ -280,7 +280,8 @@ extern "C" int sae_gemm_over_tokens(const void *left, int left_dtype, const void
   const bool wide = left_dtype == SAE_F32 || right_dtype == SAE_F32;
   SAE_REQUIRE(out_dtype == SAE_F32 || (out_dtype == SAE_BF16 && !wide), SAE_ERR_INVALID_ARG, "gemm_over_tokens: bad out_dtype %d", out_dtype);
   const int64_t slab = wide ? 32 : 64, slabs = (tokens + slab - 1) / slab;
-  SAE_REQUIRE(m < (1LL << 29) && n < (1LL << 22) && slabs < (1LL << 30), SAE_ERR_UNSUPPORTED, "gemm_over_tokens: size too large");
+  SAE_REQUIRE(m < (1LL << 29) && n <= 65535LL * OT_TILE && slabs < (1LL << 30), SAE_ERR_UNSUPPORTED, "gemm_over_tokens: size too large");
+  SAE_REQUIRE(n_slices == 1 || (m * n + 1023) / 1024 < (1LL << 31), SAE_ERR_UNSUPPORTED, "gemm_over_tokens: too many outputs for slices");
   SAE_REQUIRE(n_slices <= 65535 && n_slices <= slabs && (n_slices == 1 || partials), SAE_ERR_INVALID_ARG,
               "gemm_over_tokens: %lld slices of %lld slabs (with partial results for more than one)", (long long)n_slices, (long long)slabs);
   SAE_REQUIRE((left_dtype != SAE_ROWS8 || ((uintptr_t)left & 15) == 0) && (right_dtype != SAE_ROWS8 || ((uintptr_t)right & 15) == 0),

@@ -570,8 +570,8 @@ extern "C" int sae_rows8_grad_rows(const int32_t *feat_ptr, const int32_t *feat_
   using namespace sae;
   SAE_REQUIRE(feat_ptr && feat_slot && slot_tok && coef && rows && out, SAE_ERR_INVALID_ARG, "rows8_grad_rows: null pointer");
   SAE_REQUIRE(F > 0 && d > 0 && n_slots > 0, SAE_ERR_INVALID_ARG, "rows8_grad_rows: bad sizes");
-  SAE_REQUIRE(F < (1LL << 31) - 1 && d < (1LL << 30) && n_slots < (1LL << 31) - 128, SAE_ERR_UNSUPPORTED, "rows8_grad_rows: size too large");
-  SAE_REQUIRE((((uintptr_t)rows | (uintptr_t)out | (uintptr_t)workspace) & 15) == 0, SAE_ERR_INVALID_ARG,
+  SAE_REQUIRE(F < (1LL << 31) - 1 && d <= 65535LL * 1024 && n_slots < (1LL << 31) - 128, SAE_ERR_UNSUPPORTED, "rows8_grad_rows: size too large");
+  SAE_REQUIRE((((uintptr_t)rows | (uintptr_t)workspace) & 15) == 0 && ((uintptr_t)out & (d % 4 == 0 ? 15 : 3)) == 0, SAE_ERR_INVALID_ARG,
               "rows8_grad_rows: 16-byte alignment required");
   SAE_REQUIRE(workspace && workspace_bytes >= sae_rows8_grad_rows_workspace_bytes(n_slots, d), SAE_ERR_WORKSPACE,
               "rows8_grad_rows: workspace of %lld bytes needed", (long long)sae_rows8_grad_rows_workspace_bytes(n_slots, d));

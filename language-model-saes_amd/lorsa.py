@@ -29,7 +29,7 @@ from torch import nn
 from . import ops
 from .config import LorsaConfig, register_sae_model
 from .hooks import HookPoint
-from .sae import SparseRowGrad, _autocast_dtype
+from .sae import SparseRowGrad, _autocast_dtype, _input_operand
 from .sparse_dictionary import LazyDict, SparseDictionary
 
 
@@ -89,50 +89,70 @@ class _ProjectAndMix(torch.autograd.Function):
     backward: the attention backward takes the same operands (products over positions read their tiles across the
               rows) and returns dq^T, dk^T, dv^T [., T] in one buffer, which is exactly the operand of the
               weight-gradient product dW = d(.)^T x over the token axis (one GEMM for the three); bias gradients are its
-              row sums."""
+              row sums.
+    With the model's `rows8_checkpoint` nothing but x, in 8 bits, is held for the backward pass, which forms q, k, v, the
+    mixing and its log-sum-exp again from the rows that 8 bits hold: 2 T (2 h dq + 2 F) bytes less, for a second forward."""
+
+    @staticmethod
+    def _mix(x_op, operands, biases, dims, rot):
+        """q, k, v, the mixed values and their log-sum-exp of bf16 rows x_op [T, d_model]."""
+        (wq, wk, wv), (b_Q, b_K, b_V) = operands, biases
+        n_batch, seq, h, scale = dims
+        # the biases join in the products' epilogues (bf16 product + fp32 bias, rounded to bf16 again: what the attention
+        # gets under autocast); added per tile inside the attention kernels they would be re-added for every
+        # (query block, key block) pair and cost those kernels as many vector instructions as their softmax
+        flat = lambda b: b.detach().float().reshape(-1).contiguous()        # noqa: E731
+        if rot is None:
+            q = ops.encoder_gemm_bias(x_op, wq, col_bias=flat(b_Q))         # [T, h dq]
+            k = ops.encoder_gemm_bias(x_op, wk, col_bias=flat(b_K))
+        else:
+            (cos, sin, _cos_t, _sin_t), rdim, adjacent = rot
+            q = ops.rotary_fwd(ops.encoder_gemm(x_op, wq, torch.float32), flat(b_Q), cos, sin, seq, h, rdim, adjacent)
+            k = ops.rotary_fwd(ops.encoder_gemm(x_op, wk, torch.float32), flat(b_K), cos, sin, seq, h, rdim, adjacent)
+        v = ops.encoder_gemm_bias(x_op, wv, col_bias=flat(b_V))             # [T, F]
+        out, lse = ops.attention_fwd(q, k, v, n_batch, seq, h, scale)
+        return q, k, v, out, lse
 
     @staticmethod
     def forward(ctx, x2, W_Q, W_K, W_V, b_Q, b_K, b_V, model, seq):
         cfg = model.cfg
         T = x2.shape[0]
         n_batch, h = T // seq, cfg.n_qk_heads
-        x_op = x2 if x2.dtype == torch.bfloat16 else ops.cast_bf16(x2.float().contiguous())
-        wq, wk, wv = model._w_qk_operand("W_Q"), model._w_qk_operand("W_K"), model._w_val_operand(True)
-        # the biases join in the products' epilogues (bf16 product + fp32 bias, rounded to bf16 again: what the attention
-        # gets under autocast); added per tile inside the attention kernels they would be re-added for every
-        # (query block, key block) pair and cost those kernels as many vector instructions as their softmax
-        flat = lambda b: b.detach().float().reshape(-1).contiguous()        # noqa: E731
-        rot = model._rotary_tables() if cfg.positional_embedding_type == "rotary" else None
-        if rot is None:
-            q = ops.encoder_gemm_bias(x_op, wq, col_bias=flat(b_Q))         # [T, h dq]
-            k = ops.encoder_gemm_bias(x_op, wk, col_bias=flat(b_K))
+        x_op, x_kept = _input_operand(x2, True, model.rows8_checkpoint)
+        operands = (model._w_qk_operand("W_Q"), model._w_qk_operand("W_K"), model._w_val_operand(True))
+        biases = (b_Q.detach(), b_K.detach(), b_V.detach())
+        rot = ((model._rotary_tables(), cfg.rotary_dim, cfg.rotary_adjacent_pairs)
+               if cfg.positional_embedding_type == "rotary" else None)
+        dims = (n_batch, seq, h, 1.0 / model.attn_scale)
+        q, k, v, out, lse = _ProjectAndMix._mix(x_op, operands, biases, dims, rot)
+        ctx.rows8_d = x_kept.d if isinstance(x_kept, ops.Rows8) else None
+        if ctx.rows8_d is None:
+            ctx.save_for_backward(x_op, *operands, *biases, q, k, v, out, lse)
         else:
-            cos, sin = rot[0], rot[1]
-            q = ops.rotary_fwd(ops.encoder_gemm(x_op, wq, torch.float32), flat(b_Q), cos, sin, seq, h, cfg.rotary_dim,
-                               cfg.rotary_adjacent_pairs)
-            k = ops.rotary_fwd(ops.encoder_gemm(x_op, wk, torch.float32), flat(b_K), cos, sin, seq, h, cfg.rotary_dim,
-                               cfg.rotary_adjacent_pairs)
-        v = ops.encoder_gemm_bias(x_op, wv, col_bias=flat(b_V))             # [T, F]
-        scale = 1.0 / model.attn_scale
-        out, lse = ops.attention_fwd(q, k, v, n_batch, seq, h, scale)
-        ctx.save_for_backward(x_op, wq, wk, wv, q, k, v, out, lse, b_Q.detach(), b_K.detach(), b_V.detach())
-        ctx.dims = (n_batch, seq, h, scale)
-        ctx.rotary = None if rot is None else (rot[2], rot[3], cfg.rotary_dim, cfg.rotary_adjacent_pairs)
+            ctx.save_for_backward(x_kept.data, *operands, *biases)
+            ctx.weights = tuple((p, p._version) for p in (W_Q, W_K, W_V))
+        ctx.dims, ctx.rotary = dims, rot
         ctx.shapes = (tuple(W_Q.shape), tuple(W_K.shape))
         ctx.x_dtype = x2.dtype
         return out
 
     @staticmethod
     def backward(ctx, dz):
-        x_op, wq, wk, wv, q, k, v, out, lse, b_Q, b_K, b_V = ctx.saved_tensors
+        x_op, wq, wk, wv, b_Q, b_K, b_V, *mixed = ctx.saved_tensors
         n_batch, seq, h, scale = ctx.dims
+        if ctx.rows8_d is not None:
+            if any(p._version != v for p, v in ctx.weights):
+                raise RuntimeError("a projection's weight was changed between the two passes: the mixing cannot be formed again")
+            x_op = ops.restore_rows(ops.Rows8(x_op, ctx.rows8_d))
+            mixed = _ProjectAndMix._mix(x_op, (wq, wk, wv), (b_Q, b_K, b_V), ctx.dims, ctx.rotary)
+        q, k, v, out, lse = mixed
         dz = dz.contiguous() if dz.dtype == torch.bfloat16 else ops.cast_bf16(dz.float().contiguous())
         dqt, dkt, dvt, stacked = ops.attention_bwd(q, k, v, out, dz, lse, n_batch, seq, h, scale, return_stacked=True)
         d = x_op.shape[1]
         n_qk = q.shape[1]
         dq_w = n_qk // h
         if ctx.rotary is not None:   # the gradients arrive with respect to the rotated q, k
-            cos_t, sin_t, rdim, adjacent = ctx.rotary
+            (_cos, _sin, cos_t, sin_t), rdim, adjacent = ctx.rotary
             ops.rotary_bwd_t(stacked[:n_qk], cos_t, sin_t, seq, h, rdim, adjacent)
             ops.rotary_bwd_t(stacked[n_qk: 2 * n_qk], cos_t, sin_t, seq, h, rdim, adjacent)
         # the three weight gradients d(.)^T x in one product over the token axis: the gradients share one buffer

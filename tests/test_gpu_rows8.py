@@ -274,6 +274,16 @@ def test_the_two_tilings_agree(pkg, dev, monkeypatch):
     assert (np.abs(small - doubles(large)) <= bound(doubles(left), doubles(ops.restore_rows(right, torch.float32)), 256)).all()
 
 
+def test_out_of_an_odd_width_starts_anywhere(pkg, dev):
+    ops = pkg.ops
+    q = ops.quantize_rows(activations(50, 37, 26))
+    code = sparse_code(ops, 50, 9, 3, 27, dev)
+    fi = ops.build_feature_index(code)
+    frame = torch.full((11, 37), 7.0, device=dev)
+    rows, _ = ops.sparse_grad_rows(fi, code.val, q, 9, out=frame[1:10])
+    assert torch.equal(rows, ops.sparse_grad_rows(fi, code.val, q, 9)[0]) and (frame[0] == 7).all() and (frame[10] == 7).all()
+
+
 def test_no_tokens(pkg, dev):
     ops = pkg.ops
     q = ops.quantize_rows(torch.empty(0, 40, device=dev))

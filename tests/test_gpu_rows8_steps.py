@@ -38,6 +38,9 @@ def make_sae(pkg, dev, act_fn="topk", d=128, F=640, k=8, B=192, seed=0, dtype=to
     sae = pkg.SparseAutoEncoder(c)
     host = synthetic.activations(B, d, 16, seed)
     synthetic.load_weights(sae, *[t.to(dev) for t in synthetic.sae_weights(d, F, host, seed)])
+    if act_fn == "jumprelu":             # a new module's thresholds are memory as it came
+        with torch.no_grad():
+            sae.activation_function.log_jumprelu_threshold.fill_(-1.5)
     if cfg.get("use_glu_encoder"):
         with torch.no_grad():
             sae.W_E_glu.copy_(torch.randn(F, d, generator=torch.Generator().manual_seed(seed + 1)).t().to(dev) / d ** 0.5)
@@ -350,6 +353,52 @@ def test_clt_step(pkg, dev, monkeypatch, act_fn, amp):
         clt.compute_loss(batch)["loss"].backward()
     opt.step()
     assert all(torch.isfinite(p).all() for p in clt.parameters())
+
+
+@pytest.mark.parametrize("rotary", [False, True])
+def test_lorsa_step_forms_its_mixing_again(pkg, dev, rotary):
+    """Of inputs that 8 bits hold the mixing formed again in the backward pass is the one of the forward pass: every gradient to
+    the bit, with less held between the passes; of others it is the mixing of the rows that 8 bits hold."""
+    d, F, h, s, b, k = 128, 256, 4, 64, 4, 8
+    kw = dict(positional_embedding_type="rotary" if rotary else "none", rotary_dim=32)
+    lorsa = pkg.LowRankSparseAttention(pkg.LorsaConfig(
+        hook_point_in="in", hook_point_out="out", d_model=d, expansion_factor=F / d, n_qk_heads=h, d_qk_head=32, n_ctx=s, top_k=k,
+        act_fn="topk", norm_activation="inference", device="cuda", dtype=torch.float32, **kw))
+    g = torch.Generator(device=dev).manual_seed(6)
+    with torch.no_grad():
+        for p in lorsa.parameters():
+            p.copy_(torch.randn(p.shape, generator=g, device=dev) * 0.1)
+    raw = torch.randn(b, s, d, generator=g, device=dev)
+    batch = {"in": held(pkg, raw), "out": torch.randn(b, s, d, generator=g, device=dev), "tokens": torch.zeros(b, s, device=dev)}
+    assert lorsa.rows8_checkpoint is False
+    with autocast(True):
+        assert lorsa._mix_kernel_eligible(batch["in"])
+    loss, want = run(lorsa, batch, True, False)
+    loss8, got = run(lorsa, batch, True, True)
+    assert torch.equal(loss, loss8) and set(got) == set(want)
+    for n in want:
+        assert torch.equal(got[n], want[n]), n
+    used = []
+    for keep in (False, True):
+        lorsa.rows8_checkpoint = keep
+        start = torch.cuda.memory_allocated()
+        with autocast(True):
+            z = lorsa.compute_hidden_pre(raw)
+        used.append(torch.cuda.memory_allocated() - start)
+        out = torch.autograd.grad(z, [lorsa.W_Q, lorsa.W_V], torch.ones_like(z))
+        del z
+    with autocast(True):
+        z = lorsa.compute_hidden_pre(held(pkg, raw))
+    for a, c in zip(out, torch.autograd.grad(z, [lorsa.W_Q, lorsa.W_V], torch.ones_like(z))):
+        assert torch.equal(a, c)                            # what the 8-bit run formed from `raw`
+    with autocast(True):
+        z = lorsa.compute_hidden_pre(raw)
+    with torch.no_grad():
+        lorsa.W_K.mul_(1.5)
+    with pytest.raises(RuntimeError, match="changed between the two passes"):
+        z.sum().backward()
+    saved = b * s * (2 * d - pkg.ops.rows8_pitch(d) + 2 * (2 * h * 32 + F))     # x, q, k, v in bf16; the mixing itself is the output
+    assert used[0] - used[1] >= 0.9 * saved, used
 
 
 def test_a_stretch_of_an_index(pkg, dev):

@@ -62,12 +62,12 @@ def test_entry_points_refuse_before_any_launch(pkg):
         l, ldt, r, rdt, T, m, n, out, odt, s, part, None)
     assert ot(l=None) == -1 and ot(r=None) == -1 and ot(out=None) == -1 and ot(T=0) == -1 and ot(m=0) == -1 and ot(n=-1) == -1
     assert ot(ldt=3) == -1 and ot(rdt=-1) == -1 and ot(odt=2) == -1 and ot(ldt=0, odt=1) == -1 and ot(r=P + 8) == -1
-    assert ot(s=0) == -1 and ot(s=2) == -1 and ot(s=3, part=P) == -1 and ot(n=1 << 22) == -2 and ot(m=1 << 29) == -2
+    assert ot(s=0) == -1 and ot(s=2) == -1 and ot(s=3, part=P) == -1 and ot(n=65535 * 64 + 1) == -2 and ot(m=1 << 29) == -2
     need = lib.sae_rows8_grad_rows_workspace_bytes(100, 40)
     assert need >= 100 * 4 and lib.sae_rows8_grad_rows_workspace_bytes(0, 40) == 0
     rows = lambda r=P, out=P, F=4, d=40, n=100, ws=P, b=need: lib.sae_rows8_grad_rows(P, P, P, P, r, out, None, F, d, n, ws, b, None)  # noqa: E731
     assert rows(r=None) == -1 and rows(out=None) == -1 and rows(F=0) == -1 and rows(d=0) == -1 and rows(n=0) == -1
-    assert rows(r=P + 8) == -1 and rows(ws=None) == -4 and rows(b=need - 1) == -4 and rows(d=1 << 30) == -2 and rows(n=(1 << 31) - 1) == -2
+    assert rows(r=P + 8) == -1 and rows(ws=None) == -4 and rows(b=need - 1) == -4 and rows(d=65535 * 1024 + 4, b=1 << 60) == -2 and rows(out=P + 4) == -1 and rows(out=P + 2, d=41) == -1 and rows(n=(1 << 31) - 1) == -2
     assert lib.sae_sparse_grad_rows(P, P, P, P, P, 2, P, None, 4, 40, None) == -1      # records have their own entry point
 
 
