@@ -301,7 +301,7 @@ __global__ __launch_bounds__(256) void transpose_padded_kernel(const void *__res
 // out[f, :] = sum over feature f's slots of coef * (values of the slot's record): a segmented sum over the feature index.
 // Some features are kept by most tokens and most by few, so work is cut by position in feat_slot, not by feature: a wave
 // owns a window of positions and 256 columns.  A segment that lies inside a window goes straight to its row; one that crosses
-// leaves one partial row per window, joined in window order by a third launch.
+// leaves one partial row per window, joined in a fixed order by a third launch.
 // (8192 tokens, 64 of 32768 features, d = 2048: 142 us; a workgroup per feature takes 33 ms there, the most frequent feature's
 // 8000 records one after the other.  292 MB have to move, 42 us at the rate of a large fill; the second launch's vector
 // instructions alone are 90 us: 13 per record and four columns.)
@@ -445,7 +445,9 @@ __global__ __launch_bounds__(256) void rows8_grad_window_kernel(const int32_t *_
   flush();
 }
 
-// The segment that begins in this window and goes on behind it: its partial rows, added in window order.
+// The third launch: the segment that begins in this window and goes on behind it.  A wave adds every fourth partial row of 256
+// columns, in window order, and the four sums are added in wave order: the most frequent feature's rows are a chain of a
+// quarter of their number (8192 tokens, k = 8, d = 700: 29 -> 23 us for all three launches).
 __global__ __launch_bounds__(256) void rows8_grad_join_kernel(const int32_t *__restrict__ feat_ptr, const int32_t *__restrict__ pos_feat,
                                                               const float *__restrict__ part, float *__restrict__ out, int64_t F, int64_t d,
                                                              int length) {
@@ -456,12 +458,24 @@ __global__ __launch_bounds__(256) void rows8_grad_join_kernel(const int32_t *__r
   const int f = pos_feat[w1];
   if (f < 0 || pos_feat[w1 - 1] != f || (w0 > 0 && pos_feat[w0 - 1] == f)) return;
   const int64_t last = (feat_ptr[f + 1] - 1) / length, codes = r8_blocks(d) * R8_BLOCK;
-  const int64_t j = ((int64_t)blockIdx.y * 256 + threadIdx.x) * 4;
-  if (j >= d) return;
-  float4 s = *reinterpret_cast<const float4 *>(part + (window * 2 + 1) * codes + j);
-#pragma unroll 4
-  for (int64_t w = window + 1; w <= last; ++w) {
-    const float4 x = *reinterpret_cast<const float4 *>(part + w * 2 * codes + j);
+  __shared__ float4 sums[4][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t j = ((int64_t)blockIdx.y * 64 + lane) * 4;
+  float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (j < d) {
+    if (wave == 0) s = *reinterpret_cast<const float4 *>(part + (window * 2 + 1) * codes + j);
+#pragma unroll 8
+    for (int64_t w = window + 1 + wave; w <= last; w += 4) {
+      const float4 x = *reinterpret_cast<const float4 *>(part + w * 2 * codes + j);
+      s.x += x.x; s.y += x.y; s.z += x.z; s.w += x.w;
+    }
+  }
+  sums[wave][lane] = s;
+  __syncthreads();   // every thread of the workgroup is here: the returns above are the same for all
+  if (wave != 0 || j >= d) return;
+#pragma unroll
+  for (int w = 1; w < 4; ++w) {
+    const float4 x = sums[w][lane];
     s.x += x.x; s.y += x.y; s.z += x.z; s.w += x.w;
   }
   float *dst = out + (int64_t)f * d + j;
@@ -570,7 +584,7 @@ extern "C" int sae_rows8_grad_rows(const int32_t *feat_ptr, const int32_t *feat_
   using namespace sae;
   SAE_REQUIRE(feat_ptr && feat_slot && slot_tok && coef && rows && out, SAE_ERR_INVALID_ARG, "rows8_grad_rows: null pointer");
   SAE_REQUIRE(F > 0 && d > 0 && n_slots > 0, SAE_ERR_INVALID_ARG, "rows8_grad_rows: bad sizes");
-  SAE_REQUIRE(F < (1LL << 31) - 1 && d <= 65535LL * 1024 && n_slots < (1LL << 31) - 128, SAE_ERR_UNSUPPORTED, "rows8_grad_rows: size too large");
+  SAE_REQUIRE(F < (1LL << 31) - 1 && d <= 65535LL * R8_COLS && n_slots < (1LL << 31) - 128, SAE_ERR_UNSUPPORTED, "rows8_grad_rows: size too large");
   SAE_REQUIRE((((uintptr_t)rows | (uintptr_t)workspace) & 15) == 0 && ((uintptr_t)out & (d % 4 == 0 ? 15 : 3)) == 0, SAE_ERR_INVALID_ARG,
               "rows8_grad_rows: 16-byte alignment required");
   SAE_REQUIRE(workspace && workspace_bytes >= sae_rows8_grad_rows_workspace_bytes(n_slots, d), SAE_ERR_WORKSPACE,
@@ -593,7 +607,7 @@ extern "C" int sae_rows8_grad_rows(const int32_t *feat_ptr, const int32_t *feat_
   else if (length == 64) SAE_R8_GRAD(64);
   else SAE_R8_GRAD(128);
 #undef SAE_R8_GRAD
-  hipLaunchKernelGGL(rows8_grad_join_kernel, dim3((unsigned)windows, (unsigned)((d + 1023) / 1024)), dim3(256), 0, st, feat_ptr, pos_feat, part,
+  hipLaunchKernelGGL(rows8_grad_join_kernel, dim3((unsigned)windows, (unsigned)((d + R8_COLS - 1) / R8_COLS)), dim3(256), 0, st, feat_ptr, pos_feat, part,
                      out, F, d, length);
   return check_launch("rows8_grad_rows");
 }

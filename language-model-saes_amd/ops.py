@@ -1417,15 +1417,17 @@ def quantize_rows(x: torch.Tensor, out: Optional[torch.Tensor] = None, bf16_copy
     dt = _dt(x)
     if d > 1 and x.stride(1) != 1:
         raise ValueError("the values of a row of x must lie side by side")
-    pitch = rows8_pitch(d)
     if out is None:
-        out = torch.empty(n, pitch, dtype=torch.uint8, device=x.device)
-    elif out.device != x.device:
-        raise ValueError("out must be on x's device")
-    rows = Rows8(out, d)
-    _req_rows8(rows, "out")
-    if len(rows) != n:
-        raise ValueError(f"out has {len(rows)} records for {n} rows")
+        out = x.new_empty((n, rows8_pitch(d)), dtype=torch.uint8)
+        rows = object.__new__(Rows8)         # of the right form by construction: its checks are a tenth of a small call
+        rows.data, rows.d = out, d
+    else:
+        if out.device != x.device:
+            raise ValueError("out must be on x's device")
+        rows = Rows8(out, d)
+        _req_rows8(rows, "out")
+        if len(rows) != n:
+            raise ValueError(f"out has {len(rows)} records for {n} rows")
     copy = None
     if bf16_copy:
         copy = x.contiguous() if x.dtype == torch.bfloat16 else torch.empty(n, d, dtype=torch.bfloat16, device=x.device)
@@ -1439,22 +1441,24 @@ def _read_rows8(src: Rows8, row_idx: Optional[torch.Tensor], out_dtype: Optional
                 out: Optional[torch.Tensor]) -> torch.Tensor:
     _req_rows8(src, "src")
     out_dtype = out_dtype or torch.bfloat16
-    n, d = len(src) if row_idx is None else row_idx.numel(), src.d
-    if row_idx is not None and row_idx.device != src.device:
+    data, d = src.data, src.d
+    held = data.shape[0]
+    n = held if row_idx is None else row_idx.numel()
+    if row_idx is not None and row_idx.device != data.device:
         raise ValueError("row_idx must be on the buffer's device")
     if out is None:
-        out = torch.empty(n, d, dtype=out_dtype, device=src.device)
+        out = data.new_empty((n, d), dtype=out_dtype)
     else:
         _req(out, "out", out_dtype, 2)
-        if tuple(out.shape) != (n, d) or out.device != src.device:
+        if tuple(out.shape) != (n, d) or out.device != data.device:
             raise ValueError(f"out must be {(n, d)} on the buffer's device")
     dt = _dt(out)
     if n == 0:
         return out
-    if len(src) == 0:
+    if held == 0:
         raise ValueError("rows asked of an empty buffer")
-    _launch("rows8_gather", src.data, _lib.load().sae_rows8_gather, src.data.data_ptr(), _ptr(row_idx), len(src), n, d,
-            out.data_ptr(), dt, float(scale))
+    _launch("rows8_gather", data, _lib.load().sae_rows8_gather, data.data_ptr(), _ptr(row_idx), held, n, d, out.data_ptr(), dt,
+            float(scale))
     return out
 
 
