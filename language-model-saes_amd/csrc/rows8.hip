@@ -445,39 +445,35 @@ __global__ __launch_bounds__(256) void rows8_grad_window_kernel(const int32_t *_
   flush();
 }
 
-// The third launch: the segment that begins in this window and goes on behind it.  A wave adds every fourth partial row of 256
-// columns, in window order, and the four sums are added in wave order: the most frequent feature's rows are a chain of a
-// quarter of their number (8192 tokens, k = 8, d = 700: 29 -> 23 us for all three launches).
-__global__ __launch_bounds__(256) void rows8_grad_join_kernel(const int32_t *__restrict__ feat_ptr, const int32_t *__restrict__ pos_feat,
+// The third launch: the segment that begins in this window and goes on behind it, 1024 columns per workgroup.  The first half of
+// the threads adds the first, third, ... partial row, the second half the others, and the two sums are added: the most
+// frequent feature's rows are a chain of half their number (8192 tokens, k = 8, d = 700: 29 -> 23 us for all three launches;
+// four chains of 256 columns take 23 too, and 7 us more at 8192, 64, 2048, in workgroups that find nothing to do).
+__global__ __launch_bounds__(512) void rows8_grad_join_kernel(const int32_t *__restrict__ feat_ptr, const int32_t *__restrict__ pos_feat,
                                                               const float *__restrict__ part, float *__restrict__ out, int64_t F, int64_t d,
                                                              int length) {
   const int64_t window = blockIdx.x;
   const int total = feat_ptr[F];
   const int64_t w0 = window * length, w1 = w0 + length;
-  if (w1 >= total) return;
-  const int f = pos_feat[w1];
-  if (f < 0 || pos_feat[w1 - 1] != f || (w0 > 0 && pos_feat[w0 - 1] == f)) return;
+  const int f = pos_feat[w1 < (int64_t)gridDim.x * length ? w1 : w0], inside = pos_feat[w1 - 1], before = pos_feat[w0 > 0 ? w0 - 1 : 0];
+  if (w1 >= total || f < 0 || inside != f || (w0 > 0 && before == f)) return;
   const int64_t last = (feat_ptr[f + 1] - 1) / length, codes = r8_blocks(d) * R8_BLOCK;
-  __shared__ float4 sums[4][64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t j = ((int64_t)blockIdx.y * 64 + lane) * 4;
+  __shared__ float4 sums[256];
+  const int half = threadIdx.x >> 8, at = threadIdx.x & 255;
+  const int64_t j = ((int64_t)blockIdx.y * 256 + at) * 4;
   float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
   if (j < d) {
-    if (wave == 0) s = *reinterpret_cast<const float4 *>(part + (window * 2 + 1) * codes + j);
+    if (half == 0) s = *reinterpret_cast<const float4 *>(part + (window * 2 + 1) * codes + j);
 #pragma unroll 8
-    for (int64_t w = window + 1 + wave; w <= last; w += 4) {
+    for (int64_t w = window + 1 + half; w <= last; w += 2) {
       const float4 x = *reinterpret_cast<const float4 *>(part + w * 2 * codes + j);
       s.x += x.x; s.y += x.y; s.z += x.z; s.w += x.w;
     }
   }
-  sums[wave][lane] = s;
+  if (half) sums[at] = s;
   __syncthreads();   // every thread of the workgroup is here: the returns above are the same for all
-  if (wave != 0 || j >= d) return;
-#pragma unroll
-  for (int w = 1; w < 4; ++w) {
-    const float4 x = sums[w][lane];
-    s.x += x.x; s.y += x.y; s.z += x.z; s.w += x.w;
-  }
+  if (half || j >= d) return;
+  s.x += sums[at].x; s.y += sums[at].y; s.z += sums[at].z; s.w += sums[at].w;
   float *dst = out + (int64_t)f * d + j;
   if ((d & 3) == 0) {
     store_stream(dst, 0, s);
@@ -584,7 +580,7 @@ extern "C" int sae_rows8_grad_rows(const int32_t *feat_ptr, const int32_t *feat_
   using namespace sae;
   SAE_REQUIRE(feat_ptr && feat_slot && slot_tok && coef && rows && out, SAE_ERR_INVALID_ARG, "rows8_grad_rows: null pointer");
   SAE_REQUIRE(F > 0 && d > 0 && n_slots > 0, SAE_ERR_INVALID_ARG, "rows8_grad_rows: bad sizes");
-  SAE_REQUIRE(F < (1LL << 31) - 1 && d <= 65535LL * R8_COLS && n_slots < (1LL << 31) - 128, SAE_ERR_UNSUPPORTED, "rows8_grad_rows: size too large");
+  SAE_REQUIRE(F < (1LL << 31) - 1 && d <= 65535LL * 1024 && n_slots < (1LL << 31) - 128, SAE_ERR_UNSUPPORTED, "rows8_grad_rows: size too large");
   SAE_REQUIRE((((uintptr_t)rows | (uintptr_t)workspace) & 15) == 0 && ((uintptr_t)out & (d % 4 == 0 ? 15 : 3)) == 0, SAE_ERR_INVALID_ARG,
               "rows8_grad_rows: 16-byte alignment required");
   SAE_REQUIRE(workspace && workspace_bytes >= sae_rows8_grad_rows_workspace_bytes(n_slots, d), SAE_ERR_WORKSPACE,
@@ -607,7 +603,7 @@ extern "C" int sae_rows8_grad_rows(const int32_t *feat_ptr, const int32_t *feat_
   else if (length == 64) SAE_R8_GRAD(64);
   else SAE_R8_GRAD(128);
 #undef SAE_R8_GRAD
-  hipLaunchKernelGGL(rows8_grad_join_kernel, dim3((unsigned)windows, (unsigned)((d + R8_COLS - 1) / R8_COLS)), dim3(256), 0, st, feat_ptr, pos_feat, part,
+  hipLaunchKernelGGL(rows8_grad_join_kernel, dim3((unsigned)windows, (unsigned)((d + 1023) / 1024)), dim3(512), 0, st, feat_ptr, pos_feat, part,
                      out, F, d, length);
   return check_launch("rows8_grad_rows");
 }

@@ -67,7 +67,7 @@ def test_entry_points_refuse_before_any_launch(pkg):
     assert need >= 100 * 4 and lib.sae_rows8_grad_rows_workspace_bytes(0, 40) == 0
     rows = lambda r=P, out=P, F=4, d=40, n=100, ws=P, b=need: lib.sae_rows8_grad_rows(P, P, P, P, r, out, None, F, d, n, ws, b, None)  # noqa: E731
     assert rows(r=None) == -1 and rows(out=None) == -1 and rows(F=0) == -1 and rows(d=0) == -1 and rows(n=0) == -1
-    assert rows(r=P + 8) == -1 and rows(ws=None) == -4 and rows(b=need - 1) == -4 and rows(d=65535 * 256 + 4, b=1 << 60) == -2 and rows(out=P + 4) == -1 and rows(out=P + 2, d=41) == -1 and rows(n=(1 << 31) - 1) == -2
+    assert rows(r=P + 8) == -1 and rows(ws=None) == -4 and rows(b=need - 1) == -4 and rows(d=65535 * 1024 + 4, b=1 << 60) == -2 and rows(out=P + 4) == -1 and rows(out=P + 2, d=41) == -1 and rows(n=(1 << 31) - 1) == -2
     assert lib.sae_sparse_grad_rows(P, P, P, P, P, 2, P, None, 4, 40, None) == -1      # records have their own entry point
 
 
