@@ -414,7 +414,7 @@ class _RowStore:
             if rows.ndim != 2 or rows.shape[1] != (self.width if rows.dtype != torch.uint8 else self.data.shape[1]):
                 raise ValueError(f"{rows.dtype} rows {tuple(rows.shape)} in a buffer of 8-bit rows of {self.width} values")
         if self.width is not None and rows.dtype != torch.uint8:
-            if (rows.is_cuda and rows.dtype in (torch.float32, torch.bfloat16) and rows.stride(1) == 1
+            if (rows.is_cuda and rows.device == self.data.device and rows.dtype in (torch.float32, torch.bfloat16) and rows.stride(1) == 1
                     and int(slots_host[-1]) - first == n - 1):
                 ops.quantize_rows(rows, out=self.data[first:first + n])
                 return

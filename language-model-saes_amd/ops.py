@@ -1477,6 +1477,8 @@ def _rows8_grad_rows(fi: FeatureIndex, coef: torch.Tensor, rows: Rows8, F: int, 
         if bias is not None:
             bias.zero_()
         return
+    if len(rows) == 0:
+        raise ValueError(f"{n_slots} slots of tokens that have no rows")
     lib = _lib.load()
     nbytes = lib.sae_rows8_grad_rows_workspace_bytes(n_slots, d)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=rows.device)

@@ -76,9 +76,10 @@ class SparseDictionary(nn.Module):
     # two passes (`ops.Rows8`): half the bytes of bf16 rows, a quarter of fp32 ones.  The forward pass is unchanged; of the
     # gradients the encoder's weights change (and, where activations are dense, the decoder's), by the rounding of the rows
     # they are summed over.  Inputs that 8 bits hold exactly (a batch read from an 8-bit buffer without a scale) give the
-    # same gradients.  Taken by the kernel steps of SparseAutoEncoder, Crosscoder and CrossLayerTranscoder and by the encoder
-    # and decoder products of their `encode` / `decode`; LowRankSparseAttention's mixing holds nothing but its inputs then, and
-    # is formed again from them in the backward pass.
+    # same gradients, up to the order of the sums where dense gradients are written.  Taken by the kernel steps of
+    # SparseAutoEncoder, Crosscoder and CrossLayerTranscoder and by the encoder and decoder products of their `encode` /
+    # `decode`; LowRankSparseAttention's mixing holds nothing but its inputs then, and is formed again from them in the
+    # backward pass.
     rows8_checkpoint: bool = False
 
     def __init__(self, cfg: SparseDictionaryConfig, device_mesh=None):

@@ -433,6 +433,41 @@ def test_captured_and_replayed_with_new_inputs(pkg, dev):
             assert torch.equal(a, b)
 
 
+def test_two_graphs_replayed_in_turn(pkg, dev):
+    """Two captures, each with its own temporary buffers, replayed in any order between eager work of the same operators."""
+    ops = pkg.ops
+    sizes = [(192, 160, 64, 4), (700, 96, 40, 9)]
+    inputs = []
+    for i, (T, d, F, k) in enumerate(sizes):
+        inputs.append((activations(T, d, 40 + i), activations(T, F, 50 + i, torch.bfloat16), sparse_code(ops, T, F, k, 60 + i, dev, True)))
+
+    def step(i):
+        x, g, code = inputs[i]
+        kept = ops.quantize_rows(x)
+        fi = ops.build_feature_index(code)
+        return (ops.restore_rows(kept, torch.float32), ops.gemm_over_tokens(g, kept),
+                *ops.sparse_grad_rows(fi, code.val, kept, sizes[i][2], want_bias=True))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(0), step(1)
+    torch.cuda.current_stream().wait_stream(side)
+    graphs, outs = [], []
+    for i in range(2):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[i]):
+            outs.append(step(i))
+    for turn, i in enumerate((0, 1, 1, 0, 1, 0)):
+        x, g, code = inputs[i]
+        x.copy_(activations(*x.shape, 70 + turn))
+        code.val.copy_(torch.randn_like(code.val))
+        graphs[i].replay()
+        torch.cuda.synchronize()
+        for a, b in zip(outs[i], step(i)):
+            assert torch.equal(a, b)
+
+
 # ---- refusals -------------------------------------------------------------------------------------------------
 
 def test_refusals_on_the_device(pkg, dev):
@@ -479,6 +514,8 @@ def test_refusals_on_the_device(pkg, dev):
         ops.sparse_grad_rows(fi, code.val[:-1].contiguous(), q, 6)
     with pytest.raises(ValueError):
         ops.sparse_grad_rows(fi, code.val, q, 6, out=torch.empty(6, 65, device=dev))
+    with pytest.raises(ValueError):
+        ops.sparse_grad_rows(fi, code.val, ops.quantize_rows(x[:0]), 6)      # slots of tokens, and no rows
     p = torch.zeros(6, 66, device=dev)
     odd = ops.quantize_rows(activations(8, 66, 25))
     with pytest.raises(RuntimeError):                                        # the Adam pass moves four values at a time

@@ -156,6 +156,125 @@ def test_what_the_optimiser_is_handed(pkg, dev, act_fn, amp):
     assert torch.isfinite(sae.W_E).all() and not torch.equal(before, sae.W_E)
 
 
+@pytest.mark.parametrize("amp", [False, True])
+@pytest.mark.parametrize("act_fn", ["topk", "jumprelu"])
+def test_masked_tokens_give_the_gradients_nothing(pkg, dev, monkeypatch, act_fn, amp):
+    """A padded batch: the step with masked tokens is the one without rows8_checkpoint, and other rows in their places change
+    neither its loss nor its gradients (but for the order of the sums)."""
+    sae, batch = make_sae(pkg, dev, act_fn)
+    sae.jumprelu_sparse_route = False
+    B, d = batch["in"].shape
+    mask = torch.ones(B, device=dev)
+    mask[B - 50:] = 0
+    mask[7] = 0
+    junk = batch["in"].clone()
+    junk[mask == 0] = held(pkg, 30.0 * torch.randn(51, d, generator=torch.Generator(device=dev).manual_seed(2), device=dev))
+    first = None
+    for x in (batch["in"], junk):
+        padded = dict(batch, mask=mask, **{"in": x})
+        loss, want = run(sae, padded, amp, False)
+        with monkeypatch.context() as patch:
+            sizes = Sizes(pkg, patch)
+            loss8, got = run(sae, padded, amp, True)
+        assert torch.equal(loss, loss8)
+        assert close(got["W_E"], want["W_E"], sizes.encoder[0].t(), B, amp)
+        if first is None:
+            first = loss8, got["W_E"]
+        assert torch.equal(loss8, first[0])
+        assert close(got["W_E"], first[1], sizes.encoder[0].t(), B, amp)
+
+
+def test_gradients_against_differences_of_the_loss(pkg, dev):
+    """The loss is a quadratic of W_E, and of W_D, as long as the selection stays: its central difference along any direction
+    is the gradient's product with that direction, whatever the step.  The loss in 64 bits, from its formula, with the step's
+    selection; the limit follows the rounding through the step: every sum of n terms is off by (n + 2) u of their magnitudes,
+    u = 2^-23 for additions that round or, inside a matrix instruction, truncate."""
+    u = 2.0**-23
+    sae, batch = make_sae(pkg, dev)
+    x, label = (batch[k].double() for k in ("in", "out"))
+    B, d = x.shape
+    sae.rows8_checkpoint = True
+    sae.zero_grad(set_to_none=True)
+    ctx = sae.compute_loss(batch)
+    ctx["loss"].backward()
+    on = (ctx["feature_acts"].detach() != 0).double()
+    assert on.sum() > 0.5 * B * 8
+    W_E, b_E, W_D, b_D = (p.detach().double() for p in (sae.W_E, sae.b_E, sae.W_D, sae.b_D))
+
+    def loss(we, wd):
+        recon = ((x @ we + b_E) * on) @ wd + b_D
+        return ((recon - label) ** 2).sum(1).mean()
+
+    # |error| of each quantity of the step
+    acts, e_acts = (x @ W_E + b_E).abs() * on, (d + 3) * u * (x.abs() @ W_E.abs() + b_E.abs()) * on
+    recon = ((x @ W_E + b_E) * on) @ W_D + b_D
+    e_recon = e_acts @ W_D.abs() + (8 + 3) * u * (acts @ W_D.abs() + b_D.abs())
+    g = 2.0 * (recon - label) / B
+    e_g = 2.0 * (e_recon + u * (recon.abs() + label.abs())) / B + 4 * u * g.abs()
+    dval = (g.abs() @ W_D.abs().t()) * on
+    e_dval = (e_g @ W_D.abs().t()) * on + (d + 2) * u * dval
+    e_WE = x.abs().t() @ e_dval + (B + 2) * u * (x.abs().t() @ dval)
+    e_WD = e_acts.t() @ g.abs() + acts.t() @ e_g + (B + 2) * u * (acts.t() @ g.abs())
+    rng = torch.Generator(device=dev).manual_seed(9)
+    for name, grad, error in (("W_E", sae.W_E.grad.double(), e_WE), ("W_D", sae.W_D.grad.double(), e_WD)):
+        directions = [grad / grad.norm()] + [torch.randn(grad.shape, generator=rng, device=dev, dtype=torch.float64) for _ in range(3)]
+        one = torch.zeros(grad.shape, dtype=torch.float64, device=dev)
+        one.view(-1)[grad.abs().reshape(-1).argmax()] = 1.0
+        for v in directions + [one]:
+            diff = ((loss(W_E + v, W_D) - loss(W_E - v, W_D)) if name == "W_E" else (loss(W_E, W_D + v) - loss(W_E, W_D - v))) / 2
+            slack = 1e-12 * (loss(W_E + v, W_D) if name == "W_E" else loss(W_E, W_D + v))       # the difference's own, in 64 bits
+            assert (diff - (grad * v).sum()).abs() <= (error * v.abs()).sum() + slack, name
+
+
+def test_gradient_of_a_dense_decoder_against_differences(pkg, dev):
+    """The same for the dense product over the token axis: acts @ W_D with activations that 8 bits hold, under a quadratic loss."""
+    u = 2.0**-23
+    sae, batch = make_sae(pkg, dev, "relu", d=128, F=640, B=77)
+    sae.rows8_checkpoint = True
+    acts = held(pkg, torch.rand(77, 640, generator=torch.Generator(device=dev).manual_seed(1), device=dev))
+    label = batch["out"]
+    timer = pkg.ops.KernelTimer()
+    pkg.ops.set_kernel_timer(timer)
+    try:
+        (0.5 * (sae.decode(acts) - label).pow(2).sum()).backward()
+    finally:
+        pkg.ops.set_kernel_timer(None)
+    assert "gemm_over_tokens" in timer.records and "rows8_quantize" in timer.records
+    grad = sae.W_D.grad.double()
+    W_D, b_D, A, y = sae.W_D.detach().double(), sae.b_D.detach().double(), acts.double(), label.double()
+    loss = lambda w: 0.5 * (A @ w + b_D - y).pow(2).sum()                                       # noqa: E731
+    out = A @ W_D + b_D
+    e_out = (640 + 3) * u * (A @ W_D.abs() + b_D.abs()) + 2 * u * (out.abs() + y.abs())
+    error = A.t() @ e_out + (77 + 2) * u * (A.t() @ (out - y).abs())
+    rng = torch.Generator(device=dev).manual_seed(9)
+    for v in [grad / grad.norm()] + [torch.randn(grad.shape, generator=rng, device=dev, dtype=torch.float64) for _ in range(3)]:
+        diff = (loss(W_D + v) - loss(W_D - v)) / 2
+        assert (diff - (grad * v).sum()).abs() <= (error * v.abs()).sum() + 1e-12 * loss(W_D + v)
+
+
+@pytest.mark.parametrize("amp", [torch.float32, torch.bfloat16])
+def test_a_trainer_over_held_inputs(pkg, dev, amp):
+    """Trainer.fit with clipping: the same parameters to the bit with the inputs held as floats and in 8 bits."""
+    from lm_saes_amd import synthetic
+
+    d, F, B = 128, 512, 96
+    finals = []
+    for keep in (False, True):
+        sae, _ = make_sae(pkg, dev, d=d, F=F, B=B)
+        sae.rows8_checkpoint = keep
+        stream = []
+        for s in range(6):
+            x = held(pkg, synthetic.activations(B, d, 16, s).to(dev))
+            stream.append({"in": x, "out": x, "tokens": torch.zeros(B, device=dev)})
+        trainer = pkg.Trainer(pkg.TrainerConfig(lr=1e-3, lr_warm_up_steps=2, lr_cool_down_steps=1, total_training_tokens=B * 6, amp_dtype=amp,
+                                                l1_coefficient=None, log_frequency=3, k_warmup_steps=0, clip_grad_norm=0.05))
+        trainer.fit(sae, stream)
+        assert trainer.cur_step == 6
+        finals.append([p.detach().clone() for p in sae.parameters()])
+    for a, b in zip(*finals):
+        assert torch.isfinite(a).all() and torch.equal(a, b)
+
+
 @pytest.mark.parametrize("lowp", [False, True])
 def test_training_from_a_held_buffer_is_training_on_the_floats(pkg, dev, lowp):
     """A stream whose buffer holds records, steps that keep records, Adam that reads records: parameters and moments to the bit
@@ -454,3 +573,13 @@ def test_cached_stream_of_records_on_the_gpu_equals_the_cpu_stream(pkg, dev, tmp
                 for hp in hooks:
                     assert b[hp].is_cuda and a[hp].dtype == b[hp].dtype and torch.equal(a[hp], b[hp].cpu())
                 assert torch.equal(a["tokens"], b["tokens"].cpu())
+
+
+def test_rows_that_arrive_on_another_device_than_the_buffer(pkg, dev):
+    """A buffer lies where its first rows did; later ones may come from the other side."""
+    x = torch.randn(90, 70, generator=torch.Generator().manual_seed(4))
+    want = pkg.rows8_unpack(pkg.rows8_pack(x), 70, torch.float32)
+    for first, second in ((torch.device("cpu"), dev), (dev, torch.device("cpu"))):
+        chunks = [{"in": x[:40].to(first)}, {"in": x[40:].to(second)}]
+        got = torch.cat([b["in"] for b in pkg.ActivationBatchler(30, buffer_size=100, rows8={"in": 70}).process(chunks)])
+        assert got.device.type == first.type and got.dtype == torch.float32 and torch.equal(got.cpu(), want)
