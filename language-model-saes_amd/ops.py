@@ -1506,19 +1506,25 @@ def _operand_dt(t) -> int:
     return SAE_ROWS8 if isinstance(t, Rows8) else _dt(t)
 
 
-OVER_TOKENS_FLOP = 3.4e10
+OVER_TOKENS_FLOP = 4.3e10      # of a product on 64 x 64 tiles at most, a tile counted 1000 tokens longer than it is
 
 
 def _over_tokens_slices(tokens: int, m: int, n: int, wide: bool) -> int:
     """Into how many slices of the tokens the product of 64 x 64 tiles is cut: the least estimated time.  A slab (64 tokens, 32
-    in fp32) takes a workgroup about 1 us, longer once more than two of them share every CU; joining costs a launch of 4 us,
-    0.3 us per slice and 8 bytes per output and slice at 4 TB/s.  Measured at 4096 x 1024 x 768 (192 tiles): 46 us uncut, 28 in
-    4 slices, 39 in 16; 8192 x 64 x 64 (one tile): 73 us uncut, 15 in 16 slices, 17 in 32; 1000 x 1003 x 521: 24 uncut, 17 in
-    4; 2048 x 2048 x 768: 29 uncut, 30 in two; fp32 4096 x 1024 x 768: 153 uncut, 77 in 4, 85 in 16."""
+    in fp32) takes a workgroup 0.47 us alone on its CU and 0.2 us more with each further one there (fp32: 0.9 and 0.35); joining
+    costs a launch of 4 us, 0.3 us per slice and 8 bytes per output and slice at 4 TB/s.  Measured in 1 / 2 / 4 / 8 slices:
+    4096 x 1024 x 768 (192 tiles) 33 / 27 / 24 / 28 us; 8192 x 2048 x 512 (256) 64 / 45 / 44 / 48; 8192 x 64 x 64 (one) 60 / 29 /
+    18 / 13; 1000 x 1003 x 521 (144) 12 / 15 / 18 / 23; 2048 x 2048 x 768 (384) 24 / 27 / 30 / 38; fp32 4096 x 1024 x 768 112 / 82 /
+    62 / 63."""
     slabs, tiles = -(-tokens // (32 if wide else 64)), -(-m // 64) * -(-n // 64)
-    best, best_us = 1, slabs * max(1.0, tiles / 512)
+    alone, more = (0.55, 0.35) if wide else (0.27, 0.2)
+
+    def slab_us(s):
+        return alone + more * -(-tiles * s // 256)
+
+    best, best_us = 1, slabs * slab_us(1)
     for s in (2, 4, 8, 16, 32):
-        us = -(-slabs // s) * max(1.0, tiles * s / 512) + 4.0 + s * (m * n * 2e-6 + 0.3)
+        us = -(-slabs // s) * slab_us(s) + 4.0 + s * (m * n * 2e-6 + 0.3)
         if s <= slabs and us < best_us:
             best, best_us = s, us
     return best
@@ -1530,12 +1536,14 @@ def gemm_over_tokens(left, right, out_dtype: torch.dtype = torch.float32) -> tor
     bits are exact in bf16; with an fp32 operand the product is an fp32 product (and so is `out_dtype`), otherwise a bf16
     product with fp32 accumulation.
 
-    Products of up to 34 GFLOP, and all fp32 ones, run on a kernel of 64 x 64 tiles that reads every operand as it lies; larger
+    Small and middle products, and all fp32 ones, run on a kernel of 64 x 64 tiles that reads every operand as it lies; larger
     ones on the GEMM kernel's 256 x 256 tiles, for which rows held in 8 bits (and operands that its slabs do not divide) are
     first copied into a transposed bf16 operand: their steps change along the contraction, so codes cannot enter the matrix
     cores as they are, and widening them inside that product's tiles would be done again for every tile of the other side.
-    Measured: 4096 x 2048 x 2048 (34 GFLOP) 89 us against 91, 4096 x 4096 x 768 68 against 86, 8192 x 2048 x 2048 169 against
-    112; fp32 4096 x 4096 x 768 0.26 ms against 1.04."""
+    Measured, us on 64 x 64 tiles against us with copies: 1000 x 1003 x 521 12 / 46, 4096 x 4096 x 768 59 / 80,
+    4096 x 2048 x 2048 75 / 86, 8192 x 4096 x 768 117 / 90, 8192 x 2048 x 2048 138 / 105; with many outputs for their tokens
+    1024 x 4096 x 2048 43 / 46, 512 x 8192 x 2048 49 / 42, 64 x 8192 x 2048 22 / 30; fp32 4096 x 2048 x 2048 282 us (122
+    TFLOP/s)."""
     for name, t in (("left", left), ("right", right)):
         if isinstance(t, Rows8):
             _req_rows8(t, name)
@@ -1555,7 +1563,7 @@ def gemm_over_tokens(left, right, out_dtype: torch.dtype = torch.float32) -> tor
     dev = left.device
     if T == 0:
         return torch.zeros(m, n, dtype=out_dtype, device=dev)
-    if wide or 2.0 * T * m * n <= OVER_TOKENS_FLOP:
+    if wide or 2.0 * (T + 1000) * m * n <= OVER_TOKENS_FLOP:
         slices = _over_tokens_slices(T, m, n, wide)
         out = torch.empty(m, n, dtype=out_dtype, device=dev)
         part = torch.empty(slices * m * n, dtype=torch.float32, device=dev) if slices > 1 else None

@@ -226,7 +226,7 @@ def test_gemm_over_tokens(pkg, dev, T, m, n, left_kind):
 def test_large_products(pkg, dev, T, m, n, left_kind):
     """Past the size that the 64 x 64 tiles take: tokens and widths that the GEMM kernel's slabs divide, or do not."""
     ops = pkg.ops
-    assert 2.0 * T * m * n > ops.OVER_TOKENS_FLOP
+    assert 2.0 * (T + 1000) * m * n > ops.OVER_TOKENS_FLOP
     left, right = activations(T, m, 9, torch.bfloat16), ops.quantize_rows(activations(T, n, 10))
     left = ops.quantize_rows(left) if left_kind == "rows8" else left
     lv = (ops.restore_rows(left, torch.float32) if left_kind == "rows8" else left).double()
@@ -282,6 +282,39 @@ def test_out_of_an_odd_width_starts_anywhere(pkg, dev):
     frame = torch.full((11, 37), 7.0, device=dev)
     rows, _ = ops.sparse_grad_rows(fi, code.val, q, 9, out=frame[1:10])
     assert torch.equal(rows, ops.sparse_grad_rows(fi, code.val, q, 9)[0]) and (frame[0] == 7).all() and (frame[10] == 7).all()
+
+
+@pytest.mark.parametrize("left_kind", ["bf16", "f32", "rows8"])
+@pytest.mark.parametrize("T,m,n", [(700, 1, 1), (700, 3, 2), (257, 5, 31), (129, 7, 70), (640, 2, 130), (66, 1, 9)])
+def test_products_of_few_columns(pkg, dev, T, m, n, left_kind):
+    """Rows shorter than one load: what it reads behind a row enters no sum."""
+    ops = pkg.ops
+    left = activations(T, m, 81, torch.float32 if left_kind == "f32" else torch.bfloat16)
+    left_q = ops.quantize_rows(left) if left_kind == "rows8" else left
+    right = ops.quantize_rows(activations(T, n, 82))
+    values = doubles(ops.restore_rows(left_q, torch.float32)) if left_kind == "rows8" else doubles(left)
+    r = doubles(ops.restore_rows(right, torch.float32))
+    got = doubles(ops.gemm_over_tokens(left_q, right))
+    # bf16 and 8-bit operands: exact products; fp32: products rounded once; sums of T terms
+    assert (np.abs(got - values.T @ r) <= 2 * (T + 1) * 2.0**-24 * (np.abs(values).T @ np.abs(r)) + 1e-30).all()
+
+
+@pytest.mark.parametrize("kind", [torch.bfloat16, torch.float32])
+def test_what_is_not_finite_stays_in_its_row_and_column(pkg, dev, kind):
+    """A NaN in the first column of a row lies right behind the row before it, and one in the last token in the last slab."""
+    ops = pkg.ops
+    T, m, n = 203, 131, 69
+    left, right = activations(T, m, 83, kind), activations(T, n, 84)
+    want = ops.gemm_over_tokens(left, ops.quantize_rows(right))
+    left[90, 0] = float("nan")
+    left[T - 1, m - 1] = float("inf")
+    got = ops.gemm_over_tokens(left, ops.quantize_rows(right))
+    assert not torch.isfinite(got[0]).any() and not torch.isfinite(got[m - 1]).any()
+    assert torch.equal(got[1:-1], want[1:-1])
+    held_nan = right.clone()
+    held_nan[5, 3] = float("nan")                        # its block of 32 values
+    got = ops.gemm_over_tokens(activations(T, m, 83, kind), ops.quantize_rows(held_nan))
+    assert torch.isnan(got[:, :32]).all() and torch.equal(got[:, 32:], want[:, 32:])
 
 
 def test_no_tokens(pkg, dev):
