@@ -89,47 +89,53 @@ __device__ __forceinline__ uint32_t r8_block_max(uint32_t x) {
 }
 
 // A thread takes pieces of 16 source bytes (8 bf16 or 4 fp32 values), 4 or 8 neighbouring lanes a block of 32.  All loads are
-// requested before the first is used: none stands behind a branch (WHOLE: d is a multiple of the piece, so no piece crosses
-// the row's end; a piece past the task list or the row's end reads one that is inside and drops it).
+// requested before the first is used, and none stands behind a branch: a piece past the task list or the row's end reads one
+// that is inside and drops it; one that crosses the row's end (not where WHOLE: d is a multiple of the piece) reads on into what
+// lies behind the row and drops that; only where that would pass the source's last value, `extent` from its first, are
+// values read one by one (5003 rows of 2049 bf16, 37 apart: 12.8 us with every row's last piece read so, 11.9 now).
 template <int DT, bool WHOLE>
 __global__ __launch_bounds__(256) void rows8_quantize_kernel(const void *__restrict__ src, int64_t stride, int64_t d, uint8_t *__restrict__ dst,
-                                                             uint16_t *__restrict__ copy, R8Split split, uint32_t n_tasks) {
+                                                             uint16_t *__restrict__ copy, R8Split split, uint32_t n_tasks,
+                                                             int64_t extent) {
   constexpr int W = DT == SAE_BF16 ? 8 : 4, LANES = R8_BLOCK / W, U = 2, ES = DT == SAE_BF16 ? 2 : 4;
   const int64_t nb = r8_blocks(d), codes = nb * R8_BLOCK, pitch = r8_pitch(d);
   const uint32_t first = blockIdx.x * (256 * U) + threadIdx.x;
-  float x[U][W];
+  const char *base = reinterpret_cast<const char *>(extent >= W ? src : dst);   // fewer values than a piece: any 16 bytes, dropped
+  typename R8Bytes16<ES>::type q[U];
+  int64_t start[U];
   uint32_t row[U], col[U];
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     const uint32_t t = first + u * 256 < n_tasks ? first + u * 256 : n_tasks - 1;
     row[u] = split.row(t);
     col[u] = (t - row[u] * split.per_row) * W;
-    const char *at = reinterpret_cast<const char *>(src) + ((int64_t)row[u] * stride + (col[u] < d ? col[u] : 0)) * ES;
-    if (WHOLE || col[u] >= d || col[u] + W <= d) {
-      if (WHOLE || col[u] < d) {
-        const auto q = __builtin_nontemporal_load(reinterpret_cast<const typename R8Bytes16<ES>::type *>(at));
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          if constexpr (DT == SAE_BF16) {
-            x[u][2 * e] = __uint_as_float(q[e] << 16);
-            x[u][2 * e + 1] = __uint_as_float(q[e] & 0xffff0000u);
-          } else {
-            x[u][e] = __uint_as_float(q[e]);
-          }
-        }
-      }
-    } else {
-#pragma unroll
-      for (int e = 0; e < W; ++e) x[u][e] = col[u] + e < d ? r8_load<DT>(at, e) : 0.f;
-    }
+    start[u] = (int64_t)row[u] * stride + (col[u] < d ? col[u] : 0);
+    const int64_t from = WHOLE || start[u] + W <= extent ? start[u] : 0;
+    q[u] = __builtin_nontemporal_load(reinterpret_cast<const typename R8Bytes16<ES>::type *>(base + from * ES));
   }
 #pragma unroll
+  for (int u = 0; u < U; ++u) asm volatile("" : "+v"(q[u]));   // the loads stay up here, before the branches
+#pragma unroll
   for (int u = 0; u < U; ++u) {
+    float x[W];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if constexpr (DT == SAE_BF16) {
+        x[2 * e] = __uint_as_float(q[u][e] << 16);
+        x[2 * e + 1] = __uint_as_float(q[u][e] & 0xffff0000u);
+      } else {
+        x[e] = __uint_as_float(q[u][e]);
+      }
+    }
+    if (!WHOLE && start[u] + W > extent) {
+#pragma unroll
+      for (int e = 0; e < W; ++e) x[e] = col[u] + e < d ? r8_load<DT>(src, start[u] + e) : 0.f;
+    }
     uint32_t top = 0u;
 #pragma unroll
     for (int e = 0; e < W; ++e) {
-      x[u][e] = col[u] < d ? x[u][e] : 0.f;
-      const uint32_t m = __float_as_uint(x[u][e]) & 0x7fffffffu;
+      x[e] = (WHOLE ? col[u] : col[u] + e) < d ? x[e] : 0.f;
+      const uint32_t m = __float_as_uint(x[e]) & 0x7fffffffu;
       top = m > top ? m : top;
     }
     const uint32_t field = r8_field(r8_block_max<LANES>(top));
@@ -137,7 +143,7 @@ __global__ __launch_bounds__(256) void rows8_quantize_kernel(const void *__restr
     uint8_t *rec = dst + (int64_t)row[u] * pitch;
     uint32_t packed[W / 4];
 #pragma unroll
-    for (int e = 0; e < W; e += 4) packed[e / 4] = r8_codes(&x[u][e], field);
+    for (int e = 0; e < W; e += 4) packed[e / 4] = r8_codes(&x[e], field);
     if constexpr (W == 8) *reinterpret_cast<uint2 *>(rec + col[u]) = make_uint2(packed[0], packed[W / 4 - 1]);
     else *reinterpret_cast<uint32_t *>(rec + col[u]) = packed[0];
     const int in_block = (int)(col[u] & 31) / W;
@@ -149,13 +155,13 @@ __global__ __launch_bounds__(256) void rows8_quantize_kernel(const void *__restr
         uint16_t *c = copy + (int64_t)row[u] * d + col[u];
         if (WHOLE ? col[u] < d : col[u] + 4 <= d) {
           R8Bytes8<2> o;
-          o.w[0] = pack_bf16x2(x[u][0], x[u][1]);
-          o.w[1] = pack_bf16x2(x[u][2], x[u][3]);
+          o.w[0] = pack_bf16x2(x[0], x[1]);
+          o.w[1] = pack_bf16x2(x[2], x[3]);
           *reinterpret_cast<R8Bytes8<2> *>(c) = o;
         } else if constexpr (!WHOLE) {
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            if (col[u] + e < d) c[e] = f32_to_bf16_bits(x[u][e]);
+            if (col[u] + e < d) c[e] = f32_to_bf16_bits(x[e]);
         }
       }
     }
@@ -505,11 +511,12 @@ extern "C" int sae_rows8_quantize(const void *src, int src_dtype, int64_t n, int
     const int64_t m = n - r0 < rows_per_launch ? n - r0 : rows_per_launch, tasks = m * split.per_row;
     const dim3 grid((unsigned)((tasks + 511) / 512));
     const void *in = reinterpret_cast<const char *>(src) + r0 * src_stride * size;
+    const int64_t extent = (m - 1) * src_stride + d;   // values from the first to the last that may be read
     uint8_t *out = reinterpret_cast<uint8_t *>(rows) + r0 * r8_pitch(d);
     uint16_t *copy = bf16_copy ? reinterpret_cast<uint16_t *>(bf16_copy) + r0 * d : nullptr;
 #define SAE_R8_QUANTIZE(DT, WHOLE)                                                                                              \
   hipLaunchKernelGGL((rows8_quantize_kernel<DT, WHOLE>), grid, dim3(256), 0, (hipStream_t)stream, in, src_stride, d, out, copy, split, \
-                     (uint32_t)tasks)
+                     (uint32_t)tasks, extent)
     if (src_dtype == SAE_BF16) { if (d % width == 0) SAE_R8_QUANTIZE(SAE_BF16, true); else SAE_R8_QUANTIZE(SAE_BF16, false); }
     else { if (d % width == 0) SAE_R8_QUANTIZE(SAE_F32, true); else SAE_R8_QUANTIZE(SAE_F32, false); }
 #undef SAE_R8_QUANTIZE
