@@ -62,7 +62,8 @@ struct R8Split {
 
 // 16 bytes at any element's address: rows may start anywhere, and the memory instructions take any alignment.  Float rows
 // pass once, records stay: float rows are read and written past the caches (16384 x 4096 bf16 read 39 -> 30 us, 32768 x 2048
-// gathered to fp32 71 -> 53 us).
+// gathered to fp32 71 -> 52 us).  Writing and reading are bound by HBM from a few thousand rows on: 16384 x 4096 bf16 written in
+// 34 us (6.0 TB/s), read in 30 (6.7).
 template <int ALIGN>
 struct R8Bytes16;
 template <>
@@ -308,9 +309,9 @@ __global__ __launch_bounds__(256) void transpose_padded_kernel(const void *__res
 // Some features are kept by most tokens and most by few, so work is cut by position in feat_slot, not by feature: a wave
 // owns a window of positions and 256 columns.  A segment that lies inside a window goes straight to its row; one that crosses
 // leaves one partial row per window, joined in a fixed order by a third launch.
-// (8192 tokens, 64 of 32768 features, d = 2048: 142 us; a workgroup per feature takes 33 ms there, the most frequent feature's
+// (8192 tokens, 64 of 32768 features, d = 2048: 147 us; a workgroup per feature takes 33 ms there, the most frequent feature's
 // 8000 records one after the other.  292 MB have to move, 42 us at the rate of a large fill; the second launch's vector
-// instructions alone are 90 us: 13 per record and four columns.)
+// instructions alone are 94 us of its 122: 13 per record and four columns.)
 constexpr int R8_COLS = 256;   // columns of a chunk: four per lane (eight per lane: 196 us instead of 184, before the streaming
                                // stores)
 
