@@ -17,6 +17,7 @@ from ._lib import SAE_BF16, SAE_F32, SAE_ROWS8, check
 
 # handle of a device's current stream; a build of torch without a GPU side has none to hand out
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
 def _stream(t: torch.Tensor) -> int:
@@ -146,7 +147,7 @@ def rows8_pitch(d: int) -> int:
     return -(-(nb * (ROWS8_BLOCK + 1)) // 16) * 16
 
 
-@dataclass
+@dataclass(frozen=True, eq=False)
 class Rows8:
     """[n, d] rows held in 8 bits: int8 codes with one power-of-two step per 32 values (see include/sae_hip.h, "Rows held in
     8 bits").  `data` is uint8 [n, rows8_pitch(d)], one record per row: copying, slicing, indexing and saving those rows
@@ -182,10 +183,10 @@ class _on_device:
     """Makes a tensor's device the current one for a launch on it (a no-op where it is already)."""
 
     def __init__(self, t: torch.Tensor):
-        self.index = t.device.index
+        self.index = t.get_device()
 
     def __enter__(self):
-        self.prev = torch.cuda.current_device()
+        self.prev = _current_device()
         if self.prev != self.index:
             torch.cuda.set_device(self.index)
         return self
@@ -200,8 +201,8 @@ def _launch(name: str, t: torch.Tensor, fn, *args) -> None:
     """One library call on `t`'s device and that device's current stream (appended as the last argument).  Small calls are
     as long as their host side: with no timer installed and the device current already, nothing stands around the call, and
     the stream's handle is taken without a Stream object around it (1 us of 8)."""
-    index = t.device.index
-    if _timer is None and torch.cuda.current_device() == index:
+    index = t.get_device()
+    if _timer is None and _current_device() == index:
         rc = fn(*args, _raw_stream(index))
     else:
         with _on_device(t), _timed(name):
@@ -211,8 +212,10 @@ def _launch(name: str, t: torch.Tensor, fn, *args) -> None:
 
 
 def _req_rows8(q: Rows8, name: str):
-    _req(q.data, name, torch.uint8, 2)
-    if q.data.data_ptr() % 16:
+    data = q.data                        # uint8 [n, record] since it was made
+    if not (data.is_cuda and data.is_contiguous()):
+        _req(data, name)
+    if data.data_ptr() & 15:
         raise ValueError(f"{name} must start on a 16-byte boundary")
 
 
@@ -1420,7 +1423,7 @@ def quantize_rows(x: torch.Tensor, out: Optional[torch.Tensor] = None, bf16_copy
     if out is None:
         out = x.new_empty((n, rows8_pitch(d)), dtype=torch.uint8)
         rows = object.__new__(Rows8)         # of the right form by construction: its checks are a tenth of a small call
-        rows.data, rows.d = out, d
+        rows.__dict__.update(data=out, d=d)
     else:
         if out.device != x.device:
             raise ValueError("out must be on x's device")
@@ -1444,7 +1447,7 @@ def _read_rows8(src: Rows8, row_idx: Optional[torch.Tensor], out_dtype: Optional
     data, d = src.data, src.d
     held = data.shape[0]
     n = held if row_idx is None else row_idx.numel()
-    if row_idx is not None and row_idx.device != data.device:
+    if row_idx is not None and row_idx.get_device() != data.get_device():
         raise ValueError("row_idx must be on the buffer's device")
     if out is None:
         out = data.new_empty((n, d), dtype=out_dtype)

@@ -32,6 +32,14 @@ def test_rows8_holds_whole_records(pkg):
             R(data, d)
 
 
+def test_rows8_stay_what_they_were_made(pkg):
+    """The kernels read records by the width they were made with."""
+    q = pkg.Rows8(torch.zeros(3, pkg.ops.rows8_pitch(40), dtype=torch.uint8), 40)
+    for name, value in (("data", q.data[:, :32]), ("d", 41)):
+        with pytest.raises(AttributeError):
+            setattr(q, name, value)
+
+
 def test_the_kernels_have_no_cpu_fallback(pkg):
     ops = pkg.ops
     q = ops.Rows8(torch.zeros(3, 80, dtype=torch.uint8), 40)
