@@ -529,6 +529,10 @@ int sae_transpose_padded(const void *src, int src_dtype, int64_t rows, int64_t c
 int sae_gemm_over_tokens(const void *left, int left_dtype, const void *right, int right_dtype, int64_t tokens, int64_t m, int64_t n,
                          void *out, int out_dtype, int64_t n_slices, float *partials, void *stream);
 
+/* out[i] = the sum over z of partials[z, i], in ascending z; partials fp32 [n_slices, count], out in SAE_F32 or SAE_BF16: joins what
+ * sae_gemm_bf16 leaves with n_splits > 1. */
+int sae_join_slices(const float *partials, int64_t n_slices, int64_t count, void *out, int out_dtype, void *stream);
+
 /* sae_sparse_grad_rows for a dense operand held as records (any d): out[f, :] = sum over the slots s of feature f of
  * coef[s] * values of record slot_tok[s]; rows without slots are written as zeros; bias_out (nullable) [F].  n_slots: the
  * length of feat_slot (positions feat_ptr[0] .. feat_ptr[F] of it are in use: the index may be a stretch of a longer one's

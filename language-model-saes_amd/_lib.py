@@ -63,6 +63,7 @@ SIGNATURES = {
     "sae_rows8_grad_rows_workspace_bytes": (_L, [_L, _L]),
     "sae_rows8_grad_rows": (_I, [_P, _P, _P, _P, _P, _P, _P, _L, _L, _L, _P, _L, _P]),
     "sae_gemm_over_tokens": (_I, [_P, _I, _P, _I, _L, _L, _L, _P, _I, _L, _P, _P]),
+    "sae_join_slices": (_I, [_P, _L, _L, _P, _I, _P]),
     "sae_transpose_padded": (_I, [_P, _I, _L, _L, _P, _L, _P]),
     "sae_transpose_to_bf16": (_I, [_P, _I, _P, _L, _L, _P, _P, _P]),
     "sae_code_to_dense": (_I, [_P, _P, _P, _P, _L, _L, _P, _P, _P]),

@@ -313,7 +313,23 @@ __global__ __launch_bounds__(256) void over_tokens_join_kernel(const float *__re
   }
 }
 
+static void launch_join(const float *partials, int64_t count, int64_t slices, void *out, int out_dtype, hipStream_t st) {
+  const dim3 grid((unsigned)((count + 1023) / 1024));
+  if (out_dtype == SAE_BF16) hipLaunchKernelGGL(over_tokens_join_kernel<SAE_BF16>, grid, dim3(256), 0, st, partials, count, (int)slices, out);
+  else hipLaunchKernelGGL(over_tokens_join_kernel<SAE_F32>, grid, dim3(256), 0, st, partials, count, (int)slices, out);
+}
+
 }  // namespace sae
+
+extern "C" int sae_join_slices(const float *partials, int64_t n_slices, int64_t count, void *out, int out_dtype, void *stream) {
+  using namespace sae;
+  SAE_REQUIRE(partials && out, SAE_ERR_INVALID_ARG, "join_slices: null pointer");
+  SAE_REQUIRE(n_slices > 0 && count > 0, SAE_ERR_INVALID_ARG, "join_slices: sizes must be positive");
+  SAE_REQUIRE(out_dtype == SAE_F32 || out_dtype == SAE_BF16, SAE_ERR_INVALID_ARG, "join_slices: bad dtype %d", out_dtype);
+  SAE_REQUIRE(n_slices < (1LL << 31) && (count + 1023) / 1024 < (1LL << 31), SAE_ERR_UNSUPPORTED, "join_slices: size too large");
+  launch_join(partials, count, n_slices, out, out_dtype, (hipStream_t)stream);
+  return check_launch("join_slices");
+}
 
 extern "C" int sae_gemm_over_tokens(const void *left, int left_dtype, const void *right, int right_dtype, int64_t tokens, int64_t m, int64_t n,
                                     void *out, int out_dtype, int64_t n_slices, float *partials, void *stream) {
@@ -353,10 +369,6 @@ extern "C" int sae_gemm_over_tokens(const void *left, int left_dtype, const void
 #undef SAE_OT_WIDE
 #undef SAE_OT_LOW
 #undef SAE_OT
-  if (slices > 1) {
-    const dim3 join((unsigned)((m * n + 1023) / 1024));
-    if (out_dtype == SAE_BF16) hipLaunchKernelGGL(over_tokens_join_kernel<SAE_BF16>, join, dim3(256), 0, st, partials, m * n, (int)slices, out);
-    else hipLaunchKernelGGL(over_tokens_join_kernel<SAE_F32>, join, dim3(256), 0, st, partials, m * n, (int)slices, out);
-  }
+  if (slices > 1) launch_join(partials, m * n, slices, out, out_dtype, st);
   return check_launch("gemm_over_tokens");
 }

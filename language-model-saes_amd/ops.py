@@ -1576,12 +1576,22 @@ def gemm_over_tokens(left, right, out_dtype: torch.dtype = torch.float32) -> tor
         return out
     pitch = -(-T // 64) * 64
 
-    def operand(t):
+    def operand(t, rows, other_rows, a_side):
         """(operand, whether it is stored [tokens, columns])"""
-        if not isinstance(t, Rows8) and T == pitch and t.shape[1] % 8 == 0 and t.data_ptr() % 16 == 0:
+        if (not isinstance(t, Rows8) and T == pitch and rows % 8 == 0 and t.data_ptr() % 16 == 0
+                and _k_major_read_pays(rows, other_rows, pitch, a_side)):
             return t, True
         return _transpose_padded(t, pitch), False
 
     with _on_device(left.data):
-        (a, a_k), (b, b_k) = operand(left), operand(right)
-        return gemm(a, b, out_dtype, a_k_major=a_k, b_k_major=b_k)
+        (a, a_k), (b, b_k) = operand(left, m, n, True), operand(right, n, m, False)
+        slices = gemm_split_k(m, pitch, n) if m * n % 4 == 0 else 1
+        if slices == 1:
+            return gemm(a, b, out_dtype, a_k, b_k, copy_when_faster=False)
+        part = torch.empty(slices, m, n, dtype=torch.float32, device=dev)
+        out = torch.empty(m, n, dtype=out_dtype, device=dev)
+        lib = _lib.load()
+        _launch("encoder_gemm", part, lib.sae_gemm_bf16, a.data_ptr(), int(a_k), b.data_ptr(), int(b_k), part.data_ptr(), SAE_F32, m, n,
+                pitch, slices)
+        _launch("join_slices", part, lib.sae_join_slices, part.data_ptr(), slices, m * n, out.data_ptr(), _dt(out))
+        return out

@@ -236,6 +236,28 @@ def test_large_products(pkg, dev, T, m, n, left_kind):
     assert ((ops.gemm_over_tokens(right, left).double() - r.t() @ lv).abs() <= limit.t()).all()
 
 
+@pytest.mark.parametrize("out_dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("T,m,n", [(8192, 2048, 1536), (8192, 1111, 2500), (8130, 2056, 1532)])
+def test_large_products_of_few_tiles(pkg, dev, T, m, n, out_dtype):
+    """Few 256 x 256 tiles over many tokens: slices of the tokens, joined in order."""
+    ops = pkg.ops
+    assert 2.0 * (T + 1000) * m * n > ops.OVER_TOKENS_FLOP and ops.gemm_split_k(m, -(-T // 64) * 64, n) > 1
+    left, right = activations(T, m, 11, torch.bfloat16), ops.quantize_rows(activations(T, n, 12))
+    r = ops.restore_rows(right, torch.float32).double()
+    want, size = left.double().t() @ r, left.double().abs().t() @ r.abs()
+    got = ops.gemm_over_tokens(left, right, out_dtype)
+    assert got.dtype == out_dtype and torch.equal(got, ops.gemm_over_tokens(left, right, out_dtype))
+    low = 2.0**-8 * want.abs() if out_dtype == torch.bfloat16 else 0.0
+    assert ((got.double() - want).abs() <= 2.0 * T * 2.0**-24 * size + low + 1e-38).all()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = ops.gemm_over_tokens(left, right, out_dtype)
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(held, got) and torch.equal(ops.gemm_over_tokens(left, right, out_dtype), got)
+
+
 @pytest.mark.parametrize("wide", [False, True])
 @pytest.mark.parametrize("slices", [1, 2, 3, 7])
 def test_slices_of_the_tokens(pkg, dev, slices, wide):

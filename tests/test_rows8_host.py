@@ -71,6 +71,8 @@ def test_entry_points_refuse_before_any_launch(pkg):
     assert ot(l=None) == -1 and ot(r=None) == -1 and ot(out=None) == -1 and ot(T=0) == -1 and ot(m=0) == -1 and ot(n=-1) == -1
     assert ot(ldt=3) == -1 and ot(rdt=-1) == -1 and ot(odt=2) == -1 and ot(ldt=0, odt=1) == -1 and ot(r=P + 8) == -1
     assert ot(s=0) == -1 and ot(s=2) == -1 and ot(s=3, part=P) == -1 and ot(n=65535 * 64 + 1) == -2 and ot(m=1 << 29) == -2
+    join = lambda p=P, s=2, c=100, out=P, odt=0: lib.sae_join_slices(p, s, c, out, odt, None)   # noqa: E731
+    assert join(p=None) == -1 and join(out=None) == -1 and join(s=0) == -1 and join(c=0) == -1 and join(odt=2) == -1 and join(c=1 << 42) == -2
     need = lib.sae_rows8_grad_rows_workspace_bytes(100, 40)
     assert need >= 100 * 4 and lib.sae_rows8_grad_rows_workspace_bytes(0, 40) == 0
     rows = lambda r=P, out=P, F=4, d=40, n=100, ws=P, b=need: lib.sae_rows8_grad_rows(P, P, P, P, r, out, None, F, d, n, ws, b, None)  # noqa: E731
