@@ -890,15 +890,14 @@ def sparse_grad_rows(fi: FeatureIndex, coef: torch.Tensor, dense: torch.Tensor, 
     """out[f, :] = sum over feature f's slots of coef[slot] * dense[token(slot), :]; optional bias_out[f] = sum coef.
     `dense`: [n, d] fp32 / bf16 (d a multiple of 4), or `Rows8` (any d)."""
     _req(coef, "coef", torch.float32, 1)
-    dense_ptr, dense_dt, label = _req_dense(dense)
+    if isinstance(dense, Rows8):
+        return _rows8_grad_rows(fi, coef, dense, F, want_bias, out)
+    _req(dense, "dense", ndim=2)
     d = dense.shape[1]
     dev = dense.device
     if out is None:
         out = torch.empty(F, d, dtype=torch.float32, device=dev)
     bias = torch.empty(F, dtype=torch.float32, device=dev) if want_bias else None
-    if label == "rows8":
-        _rows8_grad_rows(fi, coef, dense, F, out, bias)
-        return out, bias
     with _timed("sparse_grad_rows[bf16 dense]" if dense.dtype == torch.bfloat16 else "sparse_grad_rows[f32 dense]"):
         check(
             _lib.load().sae_sparse_grad_rows(fi.feat_ptr.data_ptr(), fi.feat_slot.data_ptr(), fi.slot_tok.data_ptr(),
@@ -1465,29 +1464,38 @@ def _read_rows8(src: Rows8, row_idx: Optional[torch.Tensor], out_dtype: Optional
     return out
 
 
-def _rows8_grad_rows(fi: FeatureIndex, coef: torch.Tensor, rows: Rows8, F: int, out: torch.Tensor, bias: Optional[torch.Tensor]):
-    _req(out, "out", torch.float32, 2)
-    n_slots, d = coef.numel(), rows.d
-    if tuple(out.shape) != (F, d):
-        raise ValueError(f"out must be {(F, d)}, got {tuple(out.shape)}")
-    if fi.feat_ptr.numel() != F + 1 or fi.feat_slot.numel() != n_slots or fi.slot_tok.numel() != n_slots:
-        raise ValueError(f"a feature index of {fi.feat_ptr.numel() - 1} features and {fi.feat_slot.numel()} slots does not fit "
+def _rows8_grad_rows(fi: FeatureIndex, coef: torch.Tensor, rows: Rows8, F: int, want_bias: bool, out: Optional[torch.Tensor]):
+    _req_rows8(rows, "dense")
+    data, d, n_slots = rows.data, rows.d, coef.numel()
+    feat_ptr, feat_slot, slot_tok = fi.feat_ptr, fi.feat_slot, fi.slot_tok
+    if feat_ptr.numel() != F + 1 or feat_slot.numel() != n_slots or slot_tok.numel() != n_slots:
+        raise ValueError(f"a feature index of {feat_ptr.numel() - 1} features and {feat_slot.numel()} slots does not fit "
                          f"{F} features and {n_slots} coefficients")
-    if any(t.device != rows.device for t in (coef, out, fi.feat_ptr, fi.feat_slot, fi.slot_tok)):
+    dev = data.get_device()
+    if (coef.get_device() != dev or feat_ptr.get_device() != dev or feat_slot.get_device() != dev or slot_tok.get_device() != dev
+            or (out is not None and out.get_device() != dev)):
         raise ValueError("the index, the coefficients, the rows and out must be on one device")
+    if out is None:
+        out = coef.new_empty((F, d))
+    else:
+        _req(out, "out", torch.float32, 2)
+        if tuple(out.shape) != (F, d):
+            raise ValueError(f"out must be {(F, d)}, got {tuple(out.shape)}")
+    bias = coef.new_empty(F) if want_bias else None
     if F == 0 or n_slots == 0:
         out.zero_()
-        if bias is not None:
+        if want_bias:
             bias.zero_()
-        return
-    if len(rows) == 0:
+        return out, bias
+    n_rows = data.shape[0]
+    if n_rows == 0:
         raise ValueError(f"{n_slots} slots of tokens that have no rows")
     lib = _lib.load()
-    nbytes = lib.sae_rows8_grad_rows_workspace_bytes(n_slots, d)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=rows.device)
-    _launch("sparse_grad_rows[rows8 dense]", coef, lib.sae_rows8_grad_rows, fi.feat_ptr.data_ptr(), fi.feat_slot.data_ptr(),
-            fi.slot_tok.data_ptr(), coef.data_ptr(), rows.data.data_ptr(), out.data_ptr(), _ptr(bias), F, d, n_slots,
-            ws.data_ptr(), nbytes)
+    nbytes = lib.sae_rows8_grad_rows_workspace_bytes(n_rows, n_slots, d)
+    ws = data.new_empty(nbytes) if nbytes else None
+    _launch("sparse_grad_rows[rows8 dense]", data, lib.sae_rows8_grad_rows, feat_ptr.data_ptr(), feat_slot.data_ptr(), slot_tok.data_ptr(),
+            coef.data_ptr(), data.data_ptr(), n_rows, out.data_ptr(), _ptr(bias), F, d, n_slots, _ptr(ws), nbytes)
+    return out, bias
 
 
 def restore_rows(src: Rows8, out_dtype: torch.dtype = torch.bfloat16, scale: float = 1.0,

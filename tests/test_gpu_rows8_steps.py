@@ -520,10 +520,11 @@ def test_lorsa_step_forms_its_mixing_again(pkg, dev, rotary):
     assert used[0] - used[1] >= 0.9 * saved, used
 
 
-def test_a_stretch_of_an_index(pkg, dev):
+@pytest.mark.parametrize("T", [60, 96, 97, 700])
+def test_a_stretch_of_an_index(pkg, dev, T):
     """Gradient rows of features in the middle of an index: neither what lies before nor behind them is touched or read."""
     ops = pkg.ops
-    T, F, k, d = 700, 90, 9, 132
+    F, k, d = 90, 9, 132
     g = torch.Generator(device=dev).manual_seed(3)
     idx = torch.rand(T, F, generator=g, device=dev).topk(k, 1).indices.sort(1).values.to(torch.int32).reshape(-1).contiguous()
     val = torch.randn(T * k, generator=g, device=dev)
