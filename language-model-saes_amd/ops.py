@@ -6,6 +6,7 @@ synchronising.  torch is used for device memory and streams only.
 
 from __future__ import annotations
 
+import functools
 from dataclasses import dataclass
 from typing import Optional, Tuple
 
@@ -1520,6 +1521,7 @@ def _operand_dt(t) -> int:
 OVER_TOKENS_FLOP = 4.3e10      # of a product on 64 x 64 tiles at most, a tile counted 1000 tokens longer than it is
 
 
+@functools.lru_cache(maxsize=1024)
 def _over_tokens_slices(tokens: int, m: int, n: int, wide: bool) -> int:
     """Into how many slices of the tokens the product of 64 x 64 tiles is cut: the least estimated time.  A slab (64 tokens, 32
     in fp32) takes a workgroup 0.47 us alone on its CU and 0.2 us more with each further one there (fp32: 0.9 and 0.35); joining
@@ -1562,7 +1564,8 @@ def gemm_over_tokens(left, right, out_dtype: torch.dtype = torch.float32) -> tor
             _req(t, name, ndim=2)
             _dt(t)
     (T, m), (T2, n) = left.shape, right.shape
-    if T != T2 or left.device != right.device:
+    dev = left.device
+    if T != T2 or dev != right.device:
         raise ValueError(f"operands must share their tokens and device: left {tuple(left.shape)} on {left.device}, "
                          f"right {tuple(right.shape)} on {right.device}")
     if m < 1 or n < 1:
@@ -1571,7 +1574,6 @@ def gemm_over_tokens(left, right, out_dtype: torch.dtype = torch.float32) -> tor
     wide = SAE_F32 in (left_dt, right_dt)
     if out_dtype not in ((torch.float32,) if wide else (torch.float32, torch.bfloat16)):
         raise TypeError(f"out_dtype {out_dtype} of a product of {'fp32' if wide else 'bf16'} operands")
-    dev = left.device
     if T == 0:
         return torch.zeros(m, n, dtype=out_dtype, device=dev)
     if wide or 2.0 * (T + 1000) * m * n <= OVER_TOKENS_FLOP:
