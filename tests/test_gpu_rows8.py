@@ -188,6 +188,27 @@ def test_offsets_past_32_bits(pkg, dev):
     assert torch.equal(got, want[[7, 7, 0, 0]])
 
 
+def test_more_pieces_than_one_launch_counts(pkg, dev):
+    """2^27 rows of 32 fp32 values are 2^30 pieces, the most of one launch: rows behind them go through a second one."""
+    ops = pkg.ops
+    n, d = (1 << 27) + 5, 32
+    base = torch.randn(n + d - 1, generator=torch.Generator(device=dev).manual_seed(6), device=dev)
+    x = base.as_strided((n, d), (1, 1))                  # row i: the 32 values from the i-th on
+    q = ops.quantize_rows(x)
+    out = ops.restore_rows(q, torch.float32)
+    for at in (0, 12345, (1 << 27) - 3, n - 6):
+        some = slice(at, at + 6)
+        want = ops.quantize_rows(x[some].contiguous())
+        assert torch.equal(q.data[some], want.data)
+        assert torch.equal(out[some], ops.restore_rows(want, torch.float32))
+    del out, x, base
+    idx = torch.arange(n - 1, -1, -1, device=dev)
+    got = ops.gather_rows(q, idx, torch.float32)
+    for at in (0, 777, (1 << 27) - 3, n - 6):
+        some = slice(at, at + 6)
+        assert torch.equal(got[some], ops.gather_rows(q, idx[some].contiguous(), torch.float32))
+
+
 # ---- dense weight gradients ------------------------------------------------------------------------------------
 
 def bound(left, right, terms):
@@ -398,6 +419,24 @@ def test_gradient_rows(pkg, dev, T, F, k, d, heavy):
         assert torch.equal(out[whole], wide[whole])
     again, _ = ops.sparse_grad_rows(fi, code.val, q, F)
     assert torch.equal(out, again)                          # the order of every sum is fixed
+
+
+def test_gradient_rows_of_the_longest_index(pkg, dev):
+    """131072 tokens, the most a feature index takes, one feature kept by all of them."""
+    ops = pkg.ops
+    T, F, k, d = 131072, 200, 3, 70
+    q = ops.quantize_rows(activations(T, d, 15))
+    code = sparse_code(ops, T, F, k, 16, dev, True)
+    fi = ops.build_feature_index(code)
+    out, bias = ops.sparse_grad_rows(fi, code.val, q, F, want_bias=True)
+    dense, values = code.to_dense().double(), ops.restore_rows(q, torch.float32).double()
+    kept = (dense != 0).sum(0)
+    assert kept.max() == T
+    size = dense.abs().t() @ values.abs()
+    assert ((out.double() - dense.t() @ values).abs() <= 2.0**-23 * (kept[:, None] + 1) * size + 1e-40).all()
+    assert ((bias.double() - dense.sum(0)).abs() <= 2.0**-23 * (kept + 1) * dense.abs().sum(0) + 1e-40).all()
+    again, _ = ops.sparse_grad_rows(fi, code.val, q, F)
+    assert torch.equal(out, again)
 
 
 @pytest.mark.parametrize("lowp", [False, True])
