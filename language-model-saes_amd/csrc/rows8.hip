@@ -79,6 +79,12 @@ struct __attribute__((packed, aligned(ALIGN))) R8Bytes8 {
   uint32_t w[2];
 };
 
+// Pieces per thread, the same for writing and reading: a record is then read back on the XCD whose L2 it was written from.
+// 5003 x 2049 bf16 written and read at once: 2 and 2 pieces 14.8 us, 4 and 4 15.7, 2 and 4 18.5, 4 and 2 19.1, 8 and 4 20.9.
+// Alone: 20000 x 1037 bf16 read 10.8 / 13.4 / 15.4 us at 2 / 4 / 8 pieces, written 14.1 / 14.9 / 17.6; whole pieces, 32768 x 2048 gathered
+// to fp32 62 / 50 / 51, 20000 x 2048 fp32 written 34.2 / 33.6 / 35.1.
+__host__ __device__ constexpr int r8_pieces(bool whole) { return whole ? 4 : 2; }
+
 // largest of the 4 (8) neighbouring lanes that hold a block: lane permutations inside the vector unit, no LDS
 template <int LANES>
 __device__ __forceinline__ uint32_t r8_block_max(uint32_t x) {
@@ -93,12 +99,12 @@ __device__ __forceinline__ uint32_t r8_block_max(uint32_t x) {
 // requested before the first is used, and none stands behind a branch: a piece past the task list or the row's end reads one
 // that is inside and drops it; one that crosses the row's end (not where WHOLE: d is a multiple of the piece) reads on into what
 // lies behind the row and drops that; only where that would pass the source's last value, `extent` from its first, are
-// values read one by one (5003 rows of 2049 bf16, 37 apart: 12.8 us with every row's last piece read so, 11.9 now).
+// values read one by one (5003 rows of 2049 bf16, 37 apart: 12.8 us with every row's last piece read so, 11.9 without).
 template <int DT, bool WHOLE>
 __global__ __launch_bounds__(256) void rows8_quantize_kernel(const void *__restrict__ src, int64_t stride, int64_t d, uint8_t *__restrict__ dst,
                                                              uint16_t *__restrict__ copy, R8Split split, uint32_t n_tasks,
                                                              int64_t extent) {
-  constexpr int W = DT == SAE_BF16 ? 8 : 4, LANES = R8_BLOCK / W, U = 2, ES = DT == SAE_BF16 ? 2 : 4;
+  constexpr int W = DT == SAE_BF16 ? 8 : 4, LANES = R8_BLOCK / W, U = r8_pieces(WHOLE), ES = DT == SAE_BF16 ? 2 : 4;
   const int64_t nb = r8_blocks(d), codes = nb * R8_BLOCK, pitch = r8_pitch(d);
   const uint32_t first = blockIdx.x * (256 * U) + threadIdx.x;
   const char *base = reinterpret_cast<const char *>(extent >= W ? src : dst);   // fewer values than a piece: any 16 bytes, dropped
@@ -176,7 +182,7 @@ template <int DT, bool IDX, bool WHOLE>
 __global__ __launch_bounds__(256) void rows8_gather_kernel(const uint8_t *__restrict__ rows, const int64_t *__restrict__ row_idx,
                                                            int64_t n_src, int64_t d, float scale, void *__restrict__ dst, R8Split split,
                                                            uint32_t n_tasks) {
-  constexpr int W = DT == SAE_BF16 ? 8 : 4, U = 4, ES = DT == SAE_BF16 ? 2 : 4;
+  constexpr int W = DT == SAE_BF16 ? 8 : 4, U = r8_pieces(WHOLE), ES = DT == SAE_BF16 ? 2 : 4;
   const int64_t codes = r8_blocks(d) * R8_BLOCK, pitch = r8_pitch(d);
   const uint32_t first = blockIdx.x * (256 * U) + threadIdx.x;
   uint32_t row[U], col[U], packed[U][W / 4], field[U];
@@ -571,7 +577,8 @@ extern "C" int sae_rows8_quantize(const void *src, int src_dtype, int64_t n, int
   const int64_t rows_per_launch = (1LL << 30) / split.per_row;   // task numbers stay below 2^31
   for (int64_t r0 = 0; r0 < n; r0 += rows_per_launch) {
     const int64_t m = n - r0 < rows_per_launch ? n - r0 : rows_per_launch, tasks = m * split.per_row;
-    const dim3 grid((unsigned)((tasks + 511) / 512));
+    const int64_t per_block = 256 * r8_pieces(d % width == 0);
+    const dim3 grid((unsigned)((tasks + per_block - 1) / per_block));
     const void *in = reinterpret_cast<const char *>(src) + r0 * src_stride * size;
     const int64_t extent = (m - 1) * src_stride + d;   // values from the first to the last that may be read
     uint8_t *out = reinterpret_cast<uint8_t *>(rows) + r0 * r8_pitch(d);
@@ -600,7 +607,8 @@ extern "C" int sae_rows8_gather(const void *rows, const int64_t *row_idx, int64_
   const int64_t rows_per_launch = (1LL << 30) / split.per_row;   // task numbers stay below 2^31
   for (int64_t r0 = 0; r0 < n_rows; r0 += rows_per_launch) {
     const int64_t m = n_rows - r0 < rows_per_launch ? n_rows - r0 : rows_per_launch, tasks = m * split.per_row;
-    const dim3 grid((unsigned)((tasks + 1023) / 1024));
+    const int64_t per_block = 256 * r8_pieces(d % width == 0);
+    const dim3 grid((unsigned)((tasks + per_block - 1) / per_block));
     const uint8_t *in = reinterpret_cast<const uint8_t *>(rows) + (row_idx ? 0 : r0 * r8_pitch(d));
     const int64_t *idx = row_idx ? row_idx + r0 : nullptr;
     void *out = reinterpret_cast<char *>(dst) + r0 * d * size;
