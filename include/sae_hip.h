@@ -538,11 +538,11 @@ int sae_join_slices(const float *partials, int64_t n_slices, int64_t count, void
  * length of feat_slot (positions feat_ptr[0] .. feat_ptr[F] of it are in use: the index may be a stretch of a longer one's
  * features).  A feature's slots are added in ascending order, as
  * sae_sparse_grad_rows adds them; where they cross a multiple of 32, 64 or 128 (by n_slots and d) in feat_slot the pieces are summed apart and
- * then joined in a fixed order, so a feature that many tokens keep costs no more time than as many slots of rare ones (of up to
- * 96 records all are added one after the other, in one launch).  slot_tok's values are below n_rows.  workspace:
- * sae_rows8_grad_rows_workspace_bytes(n_rows, n_slots, d) bytes (0: may be NULL), 16-byte aligned, as is out where d is a multiple of
+ * then joined in a fixed order, so a feature that many tokens keep costs no more time than as many slots of rare ones (of
+ * few slots, in one launch: a feature's up to 32 one after the other, more in eighths).  slot_tok's values are below n_rows.
+ * workspace: sae_rows8_grad_rows_workspace_bytes(n_rows, n_slots, F, d) bytes (0: may be NULL), 16-byte aligned, as is out where d is a multiple of
  * 4. */
-int64_t sae_rows8_grad_rows_workspace_bytes(int64_t n_rows, int64_t n_slots, int64_t d);
+int64_t sae_rows8_grad_rows_workspace_bytes(int64_t n_rows, int64_t n_slots, int64_t F, int64_t d);
 int sae_rows8_grad_rows(const int32_t *feat_ptr, const int32_t *feat_slot, const int32_t *slot_tok, const float *coef,
                         const void *rows, int64_t n_rows, float *out, float *bias_out, int64_t F, int64_t d, int64_t n_slots,
                         void *workspace, int64_t workspace_bytes, void *stream);

@@ -60,7 +60,7 @@ SIGNATURES = {
     "sae_rows8_pitch": (_L, [_L]),
     "sae_rows8_quantize": (_I, [_P, _I, _L, _L, _L, _P, _P, _P]),
     "sae_rows8_gather": (_I, [_P, _P, _L, _L, _L, _P, _I, _F, _P]),
-    "sae_rows8_grad_rows_workspace_bytes": (_L, [_L, _L, _L]),
+    "sae_rows8_grad_rows_workspace_bytes": (_L, [_L, _L, _L, _L]),
     "sae_rows8_grad_rows": (_I, [_P, _P, _P, _P, _P, _L, _P, _P, _L, _L, _L, _P, _L, _P]),
     "sae_gemm_over_tokens": (_I, [_P, _I, _P, _I, _L, _L, _L, _P, _I, _L, _P, _P]),
     "sae_join_slices": (_I, [_P, _L, _L, _P, _I, _P]),

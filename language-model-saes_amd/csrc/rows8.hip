@@ -498,64 +498,102 @@ __global__ __launch_bounds__(512) void rows8_grad_join_kernel(const int32_t *__r
   }
 }
 
-// At most R8_SHORT records: no segment is long (a token keeps a feature once), and three launches take longer than their work.
-// A wave per feature and chunk of columns looks its slots up itself, one per lane, and adds their records in ascending order.
-// us as a call among others, this and the three launches: 64 tokens, k = 32, F = 6144, d = 768 10 and 17 (host time of three
-// launches), 96, 16, 4096, 768 12 and 17, 128 14 and 17, 192 19 and 17, 256, 32, 6144, 768 27 and 17; 64, 64, 32768, 2048 57 and 60.
-constexpr int R8_SHORT = 96;
+// Few slots: three launches take longer (17 us of host time) than their work.  Here a workgroup owns eight features and 256 columns;
+// a wave looks a feature's slots up itself, one per lane, and adds their records in ascending order, 32 requested together.  A
+// segment of more than 32 slots is cut into eighths, one per wave, whose sums are added in order.
+// us as a call among others, this and the three launches: 64 tokens, k = 32, F = 6144, d = 768 10 and 17, 384 tokens of it 15 and 17, 512
+// 17 and 17, 1024 25 and 19; 1024, 4, 512, 512 11 and 17; 64, 64, 32768, 2048 54 and 58, 256 tokens of it 73 and 62; features that
+// nearly all tokens keep: 512, 16, 256, 768 14 and 17, 96, 64, 64, 512 18 and 17.
+static bool r8_short(int64_t n_rows, int64_t n_slots, int64_t F, int64_t d) {
+  return n_rows <= 1024 && n_slots * ((d + R8_COLS - 1) / R8_COLS) <= 40000 && n_slots <= 32 * F;
+}
 
-__global__ __launch_bounds__(256) void rows8_grad_short_kernel(const int32_t *__restrict__ feat_ptr, const int32_t *__restrict__ feat_slot,
+__global__ __launch_bounds__(512) void rows8_grad_short_kernel(const int32_t *__restrict__ feat_ptr, const int32_t *__restrict__ feat_slot,
                                                                const int32_t *__restrict__ slot_tok, const float *__restrict__ coef,
                                                                const uint8_t *__restrict__ rows, float *__restrict__ out,
                                                                float *__restrict__ bias_out, int64_t F, int64_t d) {
   constexpr int G = 32, PART = 8;   // records requested together, and in how many steps: a feature of few slots reads few
-  const int64_t f = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int lane = threadIdx.x & 63;
-  if (f >= F) return;
-  const int lo = feat_ptr[f], hi = feat_ptr[f + 1];
+  constexpr int SHARED = 32;        // slots from which a segment is shared by the workgroup's waves
+  __shared__ float4 part[8][64];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int64_t f0 = (int64_t)blockIdx.x * 8, f = f0 + wave;
+  const int bound = feat_ptr[f0 + lane < F ? f0 + lane : F];   // lanes 0 .. 8: where the workgroup's segments begin and end
+  const int lo = __builtin_amdgcn_readlane(bound, wave), hi = __builtin_amdgcn_readlane(bound, wave + 1);
   const int64_t codes = r8_blocks(d) * R8_BLOCK, col = (int64_t)blockIdx.y * R8_COLS + lane * 4;
   const uint32_t pitch = (uint32_t)r8_pitch(d);
   const bool on = col < codes;
   const uint32_t code_at = on ? (uint32_t)col : 0u, field_at = (uint32_t)(codes + (on ? col >> 5 : 0));
-  float acc[4] = {0.f, 0.f, 0.f, 0.f};
-  for (int p0 = lo; p0 < hi; p0 += 64) {
-    const int n = hi - p0 < 64 ? hi - p0 : 64, slot = feat_slot[p0 + (lane < n ? lane : n - 1)];   // 64 slots, one per lane
-    const int tok = slot_tok[slot];
-    const float cf = coef[slot];
-    for (int p = 0; p < n; p += G) {
-      uint32_t codes4[G], field[G];
+  float acc[4];
+  auto sum = [&](int first, int last) {   // of the records at positions first .. last - 1
 #pragma unroll
-      for (int i = 0; i < G; i += PART) {
-        if (p + i >= n) break;
+    for (int e = 0; e < 4; ++e) acc[e] = 0.f;
+    for (int p0 = first; p0 < last; p0 += 64) {
+      const int n = last - p0 < 64 ? last - p0 : 64, slot = feat_slot[p0 + (lane < n ? lane : n - 1)];   // 64 slots, one per lane
+      const int tok = slot_tok[slot];
+      const float cf = coef[slot];
+      for (int p = 0; p < n; p += G) {
+        uint32_t codes4[G], field[G];
 #pragma unroll
-        for (int j = i; j < i + PART; ++j) {
-          const uint8_t *rec = rows + (uint64_t)(uint32_t)__builtin_amdgcn_readlane(tok, p + j) * pitch;   // past n: the last one again
-          codes4[j] = *reinterpret_cast<const uint32_t *>(rec + code_at);
-          field[j] = rec[field_at];
+        for (int i = 0; i < G; i += PART) {
+          if (p + i >= n) break;
+#pragma unroll
+          for (int j = i; j < i + PART; ++j) {
+            const uint8_t *rec = rows + (uint64_t)(uint32_t)__builtin_amdgcn_readlane(tok, p + j) * pitch;   // past n: the last one again
+            codes4[j] = *reinterpret_cast<const uint32_t *>(rec + code_at);
+            field[j] = rec[field_at];
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < G; ++j) {
+          if (p + j >= n) break;
+          const float c = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(cf), p + j)), step = __uint_as_float(field[j] << 23);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[e] = fmaf(c, (float)(int8_t)(codes4[j] >> (8 * e)) * step, acc[e]);
         }
       }
+    }
+  };
+  auto store = [&]() {
+    float *dst = out + f * d + col;
+    if ((d & 3) == 0) {
+      if (col < d) store_stream(dst, 0, make_float4(acc[0], acc[1], acc[2], acc[3]));
+    } else {
 #pragma unroll
-      for (int j = 0; j < G; ++j) {
-        if (p + j >= n) break;
-        const float c = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(cf), p + j)), step = __uint_as_float(field[j] << 23);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) acc[e] = fmaf(c, (float)(int8_t)(codes4[j] >> (8 * e)) * step, acc[e]);
-      }
+      for (int e = 0; e < 4; ++e)
+        if (col + e < d) dst[e] = acc[e];
+    }
+  };
+  if (f < F) {
+    if (hi - lo <= SHARED) {
+      sum(lo, hi);
+      store();
+    }
+    if (bias_out && blockIdx.y == 0) {
+      float s = 0.f;
+      for (int i = lo + lane; i < hi; i += 64) s += coef[feat_slot[i]];
+      s = wave_sum(s);
+      if (lane == 0) bias_out[f] = s;
     }
   }
-  float *dst = out + f * d + col;
-  if ((d & 3) == 0) {
-    if (col < d) store_stream(dst, 0, make_float4(acc[0], acc[1], acc[2], acc[3]));
-  } else {
+  const int next = __shfl_down(bound, 1, 64);   // every lane takes part: lane 7 reads lane 8
+  // the same for every thread of the workgroup; past F all bounds are equal
+  for (uint64_t shared = __ballot(lane < 8 && next - bound > SHARED); shared; shared &= shared - 1) {
+    const int g = __builtin_ctzll(shared), first = __builtin_amdgcn_readlane(bound, g), n = __builtin_amdgcn_readlane(bound, g + 1) - first;
+    const int each = (n + 63) / 64 * 8, a = first + (wave * each < n ? wave * each : n);   // an eighth for each wave, in whole PARTs
+    sum(a, a + each < first + n ? a + each : first + n);
+    part[wave][lane] = make_float4(acc[0], acc[1], acc[2], acc[3]);
+    __syncthreads();
+    if (wave == g) {
+      float4 s = part[0][lane];
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (col + e < d) dst[e] = acc[e];
-  }
-  if (bias_out && blockIdx.y == 0) {
-    float s = 0.f;
-    for (int i = lo + lane; i < hi; i += 64) s += coef[feat_slot[i]];
-    s = wave_sum(s);
-    if (lane == 0) bias_out[f] = s;
+      for (int w = 1; w < 8; ++w) {
+        const float4 x = part[w][lane];
+        s.x += x.x; s.y += x.y; s.z += x.z; s.w += x.w;
+      }
+      acc[0] = s.x; acc[1] = s.y; acc[2] = s.z; acc[3] = s.w;
+      store();
+    }
+    __syncthreads();   // part is written again
   }
 }
 
@@ -643,9 +681,9 @@ extern "C" int sae_transpose_padded(const void *src, int src_dtype, int64_t rows
   return check_launch("transpose_padded");
 }
 
-extern "C" int64_t sae_rows8_grad_rows_workspace_bytes(int64_t n_rows, int64_t n_slots, int64_t d) {
+extern "C" int64_t sae_rows8_grad_rows_workspace_bytes(int64_t n_rows, int64_t n_slots, int64_t F, int64_t d) {
   using namespace sae;
-  if (n_rows <= R8_SHORT || n_slots <= 0 || d <= 0) return 0;
+  if (n_rows <= 0 || n_slots <= 0 || F <= 0 || d <= 0 || r8_short(n_rows, n_slots, F, d)) return 0;
   const int64_t length = r8_window(n_slots, d), windows = (n_slots + length - 1) / length;
   // feature, token and coefficient of every position, and two partial rows per window
   return windows * length * 12 + windows * 2 * r8_blocks(d) * R8_BLOCK * 4;
@@ -660,7 +698,7 @@ extern "C" int sae_rows8_grad_rows(const int32_t *feat_ptr, const int32_t *feat_
   SAE_REQUIRE(F < (1LL << 31) - 1 && d <= 65535LL * R8_COLS && n_slots < (1LL << 31) - 128, SAE_ERR_UNSUPPORTED, "rows8_grad_rows: size too large");
   SAE_REQUIRE((((uintptr_t)rows | (uintptr_t)workspace) & 15) == 0 && ((uintptr_t)out & (d % 4 == 0 ? 15 : 3)) == 0, SAE_ERR_INVALID_ARG,
               "rows8_grad_rows: 16-byte alignment required");
-  const int64_t need = sae_rows8_grad_rows_workspace_bytes(n_rows, n_slots, d);
+  const int64_t need = sae_rows8_grad_rows_workspace_bytes(n_rows, n_slots, F, d);
   SAE_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), SAE_ERR_WORKSPACE, "rows8_grad_rows: workspace of %lld bytes needed",
               (long long)need);
   hipStream_t st = (hipStream_t)stream;
@@ -673,7 +711,7 @@ extern "C" int sae_rows8_grad_rows(const int32_t *feat_ptr, const int32_t *feat_
   const int64_t per_xcd = (tasks + 7) / 8, blocks = (per_xcd + 3) / 4 * 8;
   SAE_REQUIRE(blocks < (1LL << 31), SAE_ERR_UNSUPPORTED, "rows8_grad_rows: size too large");
   if (need == 0) {
-    hipLaunchKernelGGL(rows8_grad_short_kernel, dim3((unsigned)feat_blocks, (unsigned)chunks), dim3(256), 0, st, feat_ptr, feat_slot, slot_tok,
+    hipLaunchKernelGGL(rows8_grad_short_kernel, dim3((unsigned)((F + 7) / 8), (unsigned)chunks), dim3(512), 0, st, feat_ptr, feat_slot, slot_tok,
                        coef, rec, out, bias_out, F, d);
     return check_launch("rows8_grad_rows");
   }

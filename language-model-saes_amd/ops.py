@@ -1492,7 +1492,7 @@ def _rows8_grad_rows(fi: FeatureIndex, coef: torch.Tensor, rows: Rows8, F: int, 
     if n_rows == 0:
         raise ValueError(f"{n_slots} slots of tokens that have no rows")
     lib = _lib.load()
-    nbytes = lib.sae_rows8_grad_rows_workspace_bytes(n_rows, n_slots, d)
+    nbytes = lib.sae_rows8_grad_rows_workspace_bytes(n_rows, n_slots, F, d)
     ws = data.new_empty(nbytes) if nbytes else None
     _launch("sparse_grad_rows[rows8 dense]", data, lib.sae_rows8_grad_rows, feat_ptr.data_ptr(), feat_slot.data_ptr(), slot_tok.data_ptr(),
             coef.data_ptr(), data.data_ptr(), n_rows, out.data_ptr(), _ptr(bias), F, d, n_slots, _ptr(ws), nbytes)

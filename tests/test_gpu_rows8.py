@@ -390,7 +390,7 @@ def sparse_code(ops, T, F, k, seed, dev, heavy=False):
     return ops.SparseCode(idx.reshape(-1).contiguous(), val.reshape(-1).contiguous(), torch.arange(T, device=dev) * k, nnz, T, F)
 
 
-CODES = [(96, 30, 9, 40), (97, 30, 9, 40), (90, 3000, 5, 700), (1, 5, 1, 40), (7, 30, 4, 33), (64, 100, 8, 768), (300, 17, 5, 1037), (513, 64, 12, 520), (1500, 12, 3, 2052), (40, 9, 2, 4100),
+CODES = [(96, 30, 9, 40), (120, 30, 9, 40), (90, 3000, 5, 700), (1024, 130, 4, 40), (1025, 130, 4, 40), (900, 512, 8, 517), (333, 41, 3, 1030), (1, 5, 1, 40), (7, 30, 4, 33), (64, 100, 8, 768), (300, 17, 5, 1037), (513, 64, 12, 520), (1500, 12, 3, 2052), (40, 9, 2, 4100),
          (33, 50, 6, 1), (128, 5, 1, 64), (2000, 400, 16, 260), (640, 8, 5, 36), (4096, 3, 1, 300),
          (4100, 60, 32, 1500), (9000, 300, 48, 516)]
 

@@ -520,7 +520,7 @@ def test_lorsa_step_forms_its_mixing_again(pkg, dev, rotary):
     assert used[0] - used[1] >= 0.9 * saved, used
 
 
-@pytest.mark.parametrize("T", [60, 96, 97, 700])
+@pytest.mark.parametrize("T", [60, 300, 330, 700])
 def test_a_stretch_of_an_index(pkg, dev, T):
     """Gradient rows of features in the middle of an index: neither what lies before nor behind them is touched or read."""
     ops = pkg.ops
@@ -532,11 +532,13 @@ def test_a_stretch_of_an_index(pkg, dev, T):
     fi = ops.build_feature_index(code)
     q = ops.quantize_rows(torch.randn(T, d, generator=g, device=dev))
     whole, bias = ops.sparse_grad_rows(fi, val, q, F, want_bias=True)
+    size, _ = ops.sparse_grad_rows(fi, val.abs(), ops.quantize_rows(ops.restore_rows(q, torch.float32).abs()), F)
     for lo, hi in ((0, 30), (30, 60), (60, 90), (41, 42), (89, 90)):
         part = ops.FeatureIndex(fi.feat_ptr[lo : hi + 1], fi.feat_slot, fi.slot_tok)
         frame = torch.full((hi - lo + 2, d), 7.0, device=dev)
         rows, b = ops.sparse_grad_rows(part, val, q, hi - lo, want_bias=True, out=frame[1:-1])
-        assert torch.equal(rows, whole[lo:hi]) and torch.equal(b, bias[lo:hi]) and (frame[0] == 7).all() and (frame[-1] == 7).all()
+        # the same terms, which the number of features may let in another order
+        assert close(rows, whole[lo:hi], size[lo:hi], T, False) and torch.equal(b, bias[lo:hi]) and (frame[0] == 7).all() and (frame[-1] == 7).all()
 
 
 # ---- the stream --------------------------------------------------------------------------------------------------

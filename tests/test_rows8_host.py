@@ -73,9 +73,10 @@ def test_entry_points_refuse_before_any_launch(pkg):
     assert ot(s=0) == -1 and ot(s=2) == -1 and ot(s=3, part=P) == -1 and ot(n=65535 * 64 + 1) == -2 and ot(m=1 << 29) == -2
     join = lambda p=P, s=2, c=100, out=P, odt=0: lib.sae_join_slices(p, s, c, out, odt, None)   # noqa: E731
     assert join(p=None) == -1 and join(out=None) == -1 and join(s=0) == -1 and join(c=0) == -1 and join(odt=2) == -1 and join(c=1 << 42) == -2
-    need = lib.sae_rows8_grad_rows_workspace_bytes(1000, 100, 40)
-    assert need >= 100 * 4 and lib.sae_rows8_grad_rows_workspace_bytes(1000, 0, 40) == 0
-    rows = lambda r=P, nr=1000, out=P, F=4, d=40, n=100, ws=P, b=need: lib.sae_rows8_grad_rows(  # noqa: E731
+    need = lib.sae_rows8_grad_rows_workspace_bytes(2000, 100, 4, 40)
+    assert need >= 100 * 4 and lib.sae_rows8_grad_rows_workspace_bytes(2000, 0, 4, 40) == 0
+    assert lib.sae_rows8_grad_rows_workspace_bytes(1024, 100, 4, 40) == 0 < lib.sae_rows8_grad_rows_workspace_bytes(1024, 129, 4, 40)   # one launch
+    rows = lambda r=P, nr=2000, out=P, F=4, d=40, n=100, ws=P, b=need: lib.sae_rows8_grad_rows(  # noqa: E731
         P, P, P, P, r, nr, out, None, F, d, n, ws, b, None)
     assert rows(nr=0) == -1 and rows(r=None) == -1 and rows(out=None) == -1 and rows(F=0) == -1 and rows(d=0) == -1 and rows(n=0) == -1
     assert rows(r=P + 8) == -1 and rows(ws=None) == -4 and rows(b=need - 1) == -4 and rows(d=65535 * 256 + 4, b=1 << 60) == -2 and rows(out=P + 4) == -1 and rows(out=P + 2, d=41) == -1 and rows(n=(1 << 31) - 1) == -2
