@@ -461,8 +461,10 @@ __global__ __launch_bounds__(256) void rows8_grad_window_kernel(const int32_t *_
 // The third launch: the segment that begins in this window and goes on behind it, 1024 columns per workgroup.  The first half of
 // the threads adds the first, third, ... partial row, the second half the others, and the two sums are added: the most
 // frequent feature's rows are a chain of half their number (8192 tokens, k = 8, d = 700: 29 -> 23 us for all three launches;
-// four chains of 256 columns take 23 too, and 7 us more at 8192, 64, 2048, in workgroups that find nothing to do).
-__global__ __launch_bounds__(512) void rows8_grad_join_kernel(const int32_t *__restrict__ feat_ptr, const int32_t *__restrict__ pos_feat,
+// four chains of 256 columns take 23 too, and 7 us more at 8192, 64, 2048, in workgroups that find nothing to do).  Workgroups of
+// two waves for up to 256 columns: 38 instead of 44 us at 8192, 64, 64.
+template <int LANES>
+__global__ __launch_bounds__(2 * LANES) void rows8_grad_join_kernel(const int32_t *__restrict__ feat_ptr, const int32_t *__restrict__ pos_feat,
                                                               const float *__restrict__ part, float *__restrict__ out, int64_t F, int64_t d,
                                                              int length) {
   const int64_t window = blockIdx.x;
@@ -471,9 +473,9 @@ __global__ __launch_bounds__(512) void rows8_grad_join_kernel(const int32_t *__r
   const int f = pos_feat[w1 < (int64_t)gridDim.x * length ? w1 : w0], inside = pos_feat[w1 - 1], before = pos_feat[w0 > 0 ? w0 - 1 : 0];
   if (w1 >= total || f < 0 || inside != f || (w0 > 0 && before == f)) return;
   const int64_t last = (feat_ptr[f + 1] - 1) / length, codes = r8_blocks(d) * R8_BLOCK;
-  __shared__ float4 sums[256];
-  const int half = threadIdx.x >> 8, at = threadIdx.x & 255;
-  const int64_t j = ((int64_t)blockIdx.y * 256 + at) * 4;
+  __shared__ float4 sums[LANES];
+  const int half = threadIdx.x / LANES, at = threadIdx.x % LANES;
+  const int64_t j = ((int64_t)blockIdx.y * LANES + at) * 4;
   float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
   if (j < d) {
     if (half == 0) s = *reinterpret_cast<const float4 *>(part + (window * 2 + 1) * codes + j);
@@ -724,7 +726,10 @@ extern "C" int sae_rows8_grad_rows(const int32_t *feat_ptr, const int32_t *feat_
   else if (length == 64) SAE_R8_GRAD(64);
   else SAE_R8_GRAD(128);
 #undef SAE_R8_GRAD
-  hipLaunchKernelGGL(rows8_grad_join_kernel, dim3((unsigned)windows, (unsigned)((d + 1023) / 1024)), dim3(512), 0, st, feat_ptr, pos_feat, part,
-                     out, F, d, length);
+  if (d <= 256)
+    hipLaunchKernelGGL(rows8_grad_join_kernel<64>, dim3((unsigned)windows), dim3(128), 0, st, feat_ptr, pos_feat, part, out, F, d, length);
+  else
+    hipLaunchKernelGGL(rows8_grad_join_kernel<256>, dim3((unsigned)windows, (unsigned)((d + 1023) / 1024)), dim3(512), 0, st, feat_ptr, pos_feat,
+                       part, out, F, d, length);
   return check_launch("rows8_grad_rows");
 }
