@@ -192,21 +192,23 @@ class ChunkInfo:
 
 
 _REQUIRED = ("activation", "tokens", "mask", "attention_mask")
+_ROWS8 = "rows8 (width, type)"       # of a chunk read ahead: how its 8-bit rows are read back, by hook point
 
 
 class CachedActivationLoader:
     """Streams cached chunks in (shard, chunk) order; one output dict per chunk index with every hook point's
     activation under its name plus tokens / mask / attention_mask / meta, leading sample dims flattened
     until `tokens` is at most 2-D (cached_activation.py:318-420).  Rows held in 8 bits come out as the float rows they stand for
-    (`dtype`, or the type they were written from), read back on `device`; with `keep_rows8` as they are, uint8 records, whose
-    widths `rows8_widths` then names by hook point.  With a GPU `device`, chunk i + 1 is read
-    from disk by a worker thread into pinned memory and copied on a side stream while chunk i is in use."""
+    (`dtype`, or the type each chunk was written from), read back on `device`; with `keep_rows8` as they are, uint8 records, whose
+    widths `rows8_widths` then names by hook point.  The 8-bit rows of a hook point have one width and any float types.  Files of
+    float rows may stand in front of them (a cache whose writer was switched over) where floats come out, not behind them; with
+    `keep_rows8` a pass meets one form only.  A file that breaks this is refused when its turn comes.  With a GPU `device`,
+    chunk i + 1 is read from disk by a worker thread into pinned memory and copied on a side stream while chunk i is in use."""
 
     def __init__(self, cache_dirs: Mapping[str, str | Path], device: str = "cpu", dtype: Optional[torch.dtype] = None,
                  prefetch: int = 2, keep_rows8: bool = False):
         self.keep_rows8 = bool(keep_rows8)
         self.rows8_widths: dict[str, int] = {}                     # hook points whose files hold 8-bit rows -> width
-        self._rows8_types: dict[str, torch.dtype] = {}
         self.cache_dirs = {k: Path(v) for k, v in cache_dirs.items()}
         self.device = torch.device(device)
         self.dtype = dtype
@@ -236,7 +238,13 @@ class CachedActivationLoader:
             return torch.load(chunk_path, map_location="cpu", weights_only=True)
         raise ValueError(f"Invalid chunk file format: {chunk_path}. Expected .safetensors or .pt")
 
-    def _read_chunk_index(self, i: int, hook_chunks: dict[str, list[ChunkInfo]]) -> dict[str, Any]:
+    def _read_chunk_index(self, i: int, hook_chunks: dict[str, list[ChunkInfo]],
+                          widths: Optional[dict[str, Optional[int]]] = None) -> dict[str, Any]:
+        """Chunk i of every hook point.  Chunks are read ahead of the ones in use, so what 8-bit rows are read back with, their
+        width and float type, stays with the chunk (under `_ROWS8`, taken off by `_floats`).  `widths`: the pass's width of 8-bit
+        rows by hook point (None: float rows), filled and checked here."""
+        widths = {} if widths is None else widths
+        held: dict[str, tuple[int, torch.dtype]] = {}
         out: dict[str, Any] = {}
         for hp, chunks in hook_chunks.items():
             path = chunks[i].path
@@ -255,17 +263,23 @@ class CachedActivationLoader:
                 if act.dtype != torch.uint8 or d < 1 or act.shape[-1] != ops.rows8_pitch(d) or code not in _FLOAT_CODES.values():
                     raise ValueError(f"Loading cached activation {path} error: {act.dtype} {tuple(act.shape)} does not hold "
                                      f"8-bit rows of width {d}, type {code}")
-                if self.rows8_widths.setdefault(hp, d) != d:
-                    raise ValueError(f"Loading cached activation {path} error: rows of width {d} after {self.rows8_widths[hp]}")
-                self._rows8_types[hp] = next(t for t, c in _FLOAT_CODES.items() if c == code)
+                before = widths.get(hp, d)
+                if before != d and (self.keep_rows8 or before is not None):
+                    raise ValueError(f"Loading cached activation {path} error: 8-bit rows of width {d} after "
+                                     f"{'float rows' if before is None else f'rows of width {before}'}")
+                widths[hp] = self.rows8_widths[hp] = d
+                held[hp] = d, next(t for t, c in _FLOAT_CODES.items() if c == code)
                 out[hp] = act
                 continue
-            if hp in self.rows8_widths:
+            if widths.setdefault(hp, None) is not None:
                 raise ValueError(f"Loading cached activation {path} error: float rows after 8-bit ones")
+            self.rows8_widths.pop(hp, None)
             out[hp] = act.to(self.dtype) if self.dtype is not None else act
         while out["tokens"].ndim >= 3:
             out = {k: (v.flatten(0, 1) if isinstance(v, torch.Tensor) else ([a for b in v for a in b] if v is not None else None))
                    for k, v in out.items()}
+        if held:
+            out[_ROWS8] = held
         return out
 
     @staticmethod
@@ -307,10 +321,11 @@ class CachedActivationLoader:
 
     def _floats(self, chunk: dict[str, Any]) -> dict[str, Any]:
         """The chunk with its 8-bit rows read back, unless they are to be kept."""
-        if self.keep_rows8 or not self.rows8_widths:
-            return chunk
-        return {k: rows8_unpack(v, self.rows8_widths[k], self.dtype or self._rows8_types[k]) if k in self.rows8_widths else v
-                for k, v in chunk.items()}
+        held = chunk.pop(_ROWS8, {})
+        if not self.keep_rows8:
+            for hp, (d, written) in held.items():
+                chunk[hp] = rows8_unpack(chunk[hp], d, self.dtype or written)
+        return chunk
 
     def process(self, data: None = None, **kwargs) -> Iterator[dict[str, Any]]:
         hook_chunks = {hp: self._get_sorted_chunks(hp) for hp in self.cache_dirs}
@@ -319,9 +334,10 @@ class CachedActivationLoader:
             raise ValueError(f"Hook points have different numbers of chunks: {counts}. "
                              "All hook points must have the same number of chunks.")
         n = next(iter(counts.values()))
+        widths: dict[str, Optional[int]] = {}
         if self.device.type != "cuda":
             for i in range(n):
-                yield self._floats(self._read_chunk_index(i, hook_chunks))
+                yield self._floats(self._read_chunk_index(i, hook_chunks, widths))
             return
 
         q: Queue = Queue(maxsize=self.prefetch)
@@ -332,7 +348,7 @@ class CachedActivationLoader:
                 for i in range(n):
                     if stop.is_set():
                         return
-                    q.put(("chunk", self._pin(self._read_chunk_index(i, hook_chunks))))
+                    q.put(("chunk", self._pin(self._read_chunk_index(i, hook_chunks, widths))))
                 q.put(("end", None))
             except BaseException as e:  # noqa: BLE001  (handed to the consumer, which re-raises)
                 q.put(("error", e))
@@ -344,13 +360,13 @@ class CachedActivationLoader:
             pending = None
             while True:
                 kind, payload = q.get()
-                if kind == "error":
-                    raise payload
                 nxt = self._to_device(payload, copy_stream) if kind == "chunk" else None
                 if pending is not None:
                     staged, (done, _host) = pending
                     yield self._floats(self._hand_over(staged, done, torch.cuda.current_stream(self.device)))
                 pending = nxt
+                if kind == "error":      # the chunks in front of the one that failed have been handed over
+                    raise payload
                 if kind == "end":
                     break
         finally:

@@ -586,3 +586,32 @@ def test_rows_that_arrive_on_another_device_than_the_buffer(pkg, dev):
         chunks = [{"in": x[:40].to(first)}, {"in": x[40:].to(second)}]
         got = torch.cat([b["in"] for b in pkg.ActivationBatchler(30, buffer_size=100, rows8={"in": 70}).process(chunks)])
         assert got.device.type == first.type and got.dtype == torch.float32 and torch.equal(got.cpu(), want)
+
+
+def test_chunks_of_several_types_and_forms_on_the_gpu(pkg, dev, tmp_path):
+    """What a chunk comes out as is its own, though the reader is ahead of it; a file that is refused ends the pass behind the
+    chunks in front of it, as on the CPU."""
+    def write(path, parts):
+        for i, (dtype, form) in enumerate(parts):
+            t = torch.arange(16)[None]
+            x = torch.randn(1, 16, 40, generator=torch.Generator().manual_seed(i)).to(dtype)
+            x[0, 3, 3] = 6e4 if dtype == torch.float16 else 1e5
+            pkg.ActivationWriter(pkg.ActivationWriterConfig(cache_dir=str(path), hook_points=["h"], row_format=form)).process(
+                [{"h": x, "tokens": t, "mask": torch.ones_like(t), "attention_mask": torch.ones_like(t)}], start_shard=i)
+
+    f32, bf16, f16 = torch.float32, torch.bfloat16, torch.float16
+    for n, parts in enumerate(([(bf16, "rows8"), (f16, "rows8"), (f32, "rows8")], [(f32, "float"), (bf16, "rows8"), (f16, "rows8")])):
+        write(tmp_path / str(n), parts)
+        for dtype in (None, f32):
+            cpu, gpu = (pkg.CachedActivationLoader({"h": tmp_path / str(n) / "h"}, device=d, dtype=dtype) for d in ("cpu", "cuda"))
+            for _ in range(2):
+                a, b = list(cpu.process()), list(gpu.process())
+                assert len(a) == len(b) == 3
+                for u, v, (written, _form) in zip(a, b, parts):
+                    assert u["h"].dtype == v["h"].dtype == (dtype or written) and torch.equal(u["h"], v["h"].cpu())
+    write(tmp_path / "refused", [(f32, "rows8"), (f32, "rows8"), (f32, "float")])
+    for d in ("cpu", "cuda"):
+        it = pkg.CachedActivationLoader({"h": tmp_path / "refused" / "h"}, device=d).process()
+        assert next(it)["h"].dtype == next(it)["h"].dtype == f32
+        with pytest.raises(ValueError, match="float rows after"):
+            next(it)

@@ -245,3 +245,64 @@ def test_loader_refuses_files_that_disagree(pkg, tmp_path):
         w(row_format="rows8").process([{"h0": torch.zeros(1, 4, 8, dtype=torch.float64), "tokens": torch.zeros(1, 4)}])
     with pytest.raises(ValueError):
         w(row_format="int4")
+
+
+def write_chunks(pkg, path, parts):
+    """One chunk of two samples per part (d, dtype, row format): -> the float rows that each is to come out as."""
+    want = []
+    for i, (d, dtype, form) in enumerate(parts):
+        part = list(samples(2, 4, d, dtype))
+        part[0]["h0"][0, 0, 0] = 1e5 if dtype != torch.float16 else 6e4        # past fp16's largest where the type holds it
+        pkg.ActivationWriter(pkg.ActivationWriterConfig(cache_dir=str(path), hook_points=["h0"], n_samples_per_chunk=2, row_format=form)
+                             ).process(part, start_shard=i)
+        x = torch.cat([s["h0"] for s in part])
+        want.append(exact_values(x.reshape(-1, d)).view(x.shape).to(dtype) if form == "rows8" else x)
+    return want
+
+
+def read_ahead(loader):
+    """All chunks as a reader thread far ahead of its consumer leaves them: every one read before the first is handed over."""
+    chunks = {hp: loader._get_sorted_chunks(hp) for hp in loader.cache_dirs}
+    widths = {}
+    held = [loader._read_chunk_index(i, chunks, widths) for i in range(len(chunks["h0"]))]
+    return [loader._floats(c) for c in held]
+
+
+MIXED = [[(40, torch.bfloat16, "rows8"), (40, torch.float16, "rows8"), (40, torch.float32, "rows8")],
+         [(40, torch.float32, "float"), (40, torch.bfloat16, "rows8")],
+         [(24, torch.bfloat16, "float"), (40, torch.float32, "rows8"), (40, torch.bfloat16, "rows8")]]
+
+
+@pytest.mark.parametrize("parts", MIXED)
+def test_chunks_are_read_back_as_they_were_written(pkg, tmp_path, parts):
+    """The type and form of a chunk do not depend on how far ahead of it the reader is, nor on an earlier pass."""
+    want = write_chunks(pkg, tmp_path, parts)
+    loader = pkg.CachedActivationLoader({"h0": tmp_path / "h0"})
+    for got in (list(loader.process()), read_ahead(loader), list(loader.process())):
+        assert len(got) == len(parts)
+        for a, b in zip(got, want):
+            assert set(a) == {"tokens", "mask", "attention_mask", "meta", "h0"}
+            assert a["h0"].dtype == b.dtype and torch.equal(a["h0"], b)
+    for a, b in zip(pkg.CachedActivationLoader({"h0": tmp_path / "h0"}, dtype=torch.float32).process(), want):
+        assert a["h0"].dtype == torch.float32 and torch.equal(a["h0"], b.float())
+
+
+@pytest.mark.parametrize("first,second", [("float", "rows8"), ("rows8", "float")])
+def test_records_that_are_kept_do_not_mix_with_floats(pkg, tmp_path, first, second):
+    write_chunks(pkg, tmp_path, [(40, torch.float32, first), (40, torch.float32, second)])
+    loader = pkg.CachedActivationLoader({"h0": tmp_path / "h0"}, keep_rows8=True)
+    for _ in range(2):      # every pass starts anew
+        it = loader.process()
+        assert next(it)["h0"].dtype == (torch.uint8 if first == "rows8" else torch.float32)
+        with pytest.raises(ValueError, match="float rows"):
+            next(it)
+
+
+def test_widths_follow_the_files(pkg, tmp_path):
+    """A directory that is written anew in another form or width is read as it is."""
+    loader = pkg.CachedActivationLoader({"h0": tmp_path / "h0"}, keep_rows8=True)
+    for d, form in ((40, "rows8"), (70, "rows8"), (70, "float"), (40, "rows8")):
+        write_chunks(pkg, tmp_path, [(d, torch.float32, form)])
+        (got,) = loader.process()
+        assert loader.rows8_widths == ({"h0": d} if form == "rows8" else {})
+        assert got["h0"].shape[-1] == (pkg.ops.rows8_pitch(d) if form == "rows8" else d)
