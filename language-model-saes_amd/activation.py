@@ -65,7 +65,7 @@ def rows8_pack(x: torch.Tensor) -> torch.Tensor:
     inv = torch.clamp(254 - field, 1, 254).bitwise_left_shift(23).view(torch.float32)
     codes = torch.where(bad[..., None], torch.zeros_like(blocks), blocks * inv[..., None]).round().clamp(-127, 127).to(torch.int8)
     out = torch.zeros(rows.shape[0], pitch, dtype=torch.uint8)
-    out[:, : nb * ops.ROWS8_BLOCK] = codes.view(rows.shape[0], -1).view(torch.uint8)
+    out[:, : nb * ops.ROWS8_BLOCK] = codes.view(-1, nb * ops.ROWS8_BLOCK).view(torch.uint8)
     out[:, nb * ops.ROWS8_BLOCK : nb * ops.ROWS8_BLOCK + nb] = torch.where(bad, torch.full_like(field, 255), field).to(torch.uint8)
     return out.view(*lead, pitch)
 

@@ -554,6 +554,13 @@ def test_records_made_on_either_side_are_the_same(pkg, dev):
             assert v.dtype == to and torch.equal(u.isnan(), v.cpu().isnan()) and torch.equal(u.nan_to_num(), v.cpu().nan_to_num())
 
 
+def test_no_rows_on_the_gpu(pkg, dev):
+    for shape in ((0, 40), (2, 0, 33), (0, 1)):
+        data = pkg.rows8_pack(torch.zeros(shape, device=dev))
+        assert data.is_cuda and tuple(data.shape) == (*shape[:-1], pkg.ops.rows8_pitch(shape[-1]))
+        assert tuple(pkg.rows8_unpack(data, shape[-1], torch.bfloat16).shape) == shape
+
+
 def test_cached_stream_of_records_on_the_gpu_equals_the_cpu_stream(pkg, dev, tmp_path):
     hooks = ["in", "out"]
     g = torch.Generator().manual_seed(4)

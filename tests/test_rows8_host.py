@@ -138,6 +138,15 @@ def test_pack_extremes_on_the_cpu(pkg):
     assert torch.equal(back[2:].double(), exact_values(x[2:]))
 
 
+@pytest.mark.parametrize("shape", [(0, 40), (2, 0, 33), (0, 5, 32), (0, 1)])
+def test_no_rows_on_the_cpu(pkg, shape):
+    data = pkg.rows8_pack(torch.zeros(shape))
+    assert data.dtype == torch.uint8 and tuple(data.shape) == (*shape[:-1], pkg.ops.rows8_pitch(shape[-1]))
+    for dtype in (torch.float32, torch.bfloat16, torch.float16):
+        back = pkg.rows8_unpack(data, shape[-1], dtype, 0.5)
+        assert back.dtype == dtype and tuple(back.shape) == shape
+
+
 def test_pack_refuses_other_rows(pkg):
     for bad in (torch.zeros(3, 4, dtype=torch.float64), torch.zeros(3, 4, dtype=torch.int32), torch.zeros(3, 0)):
         with pytest.raises(ValueError):
