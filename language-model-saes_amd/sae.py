@@ -238,7 +238,8 @@ def _input_operand(x: torch.Tensor, low: bool, keep8: bool):
     fp32 otherwise; with `keep8` the second is held in 8 bits, written by the pass that rounds fp32 rows to bf16."""
     if low and x.dtype != torch.bfloat16:
         if keep8:
-            kept, x_op = ops.quantize_rows(x.float(), bf16_copy=True)
+            rows = x.float()                       # any distance apart, but their values side by side
+            kept, x_op = ops.quantize_rows(rows if rows.stride(1) == 1 else rows.contiguous(), bf16_copy=True)
             return x_op, kept
         x_op = ops.cast_bf16(x.float().contiguous())
     else:

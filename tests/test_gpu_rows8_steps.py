@@ -120,6 +120,29 @@ def test_rows_that_8_bits_hold_give_the_same_step(pkg, dev, monkeypatch, act_fn,
             assert torch.equal(got[n], want[n]), n
 
 
+LAYOUTS = [lambda x: x.t().contiguous().t(), lambda x: torch.cat([x, x], 1)[:, : x.shape[1]],
+           lambda x: torch.stack([x, x], 2)[:, :, 0]]
+
+
+@pytest.mark.parametrize("layout", LAYOUTS)
+@pytest.mark.parametrize("amp", [False, True])
+@pytest.mark.parametrize("act_fn,cfg,kw", [STEPS[0], STEPS[3], STEPS[4], STEPS[5], STEPS[6]])
+def test_inputs_of_any_strides(pkg, dev, act_fn, cfg, kw, amp, layout):
+    """An fp32 batch that is a transposed or sliced view gives the step of its contiguous copy, with the option as without."""
+    sae, batch = make_sae(pkg, dev, act_fn, **cfg)
+    view = layout(batch["in"])
+    assert not view.is_contiguous() and torch.equal(view, batch["in"])
+    for keep in (False, True):
+        loss, want = run(sae, batch, amp, keep, **kw)
+        loss_v, got = run(sae, dict(batch, **{"in": view}), amp, keep, **kw)
+        assert torch.equal(loss, loss_v) and set(got) == set(want)
+        for n in want:
+            assert torch.equal(got[n], want[n]), n
+        sae.rows8_checkpoint = keep
+        with autocast(amp):
+            assert torch.equal(sae.encode(view), sae.encode(batch["in"]))
+
+
 @pytest.mark.parametrize("amp", [False, True])
 @pytest.mark.parametrize("act_fn", ["topk", "batchtopk"])
 def test_what_the_optimiser_is_handed(pkg, dev, act_fn, amp):
