@@ -160,7 +160,7 @@ class _FusedCLTStep(torch.autograd.Function):
         holder.update(code=cat, pres=pres, norms=norms, layer_cnt=layer_cnt)
         ctx.cat, ctx.grads, ctx.dval, ctx.w_enc_op = cat, grads, dval, w_enc_op
         ctx.x_rows = ([ops.Rows8(rows, d) for rows in ops.quantize_rows(x_op.reshape(L * B, d)).data.view(L, B, -1)]
-                      if m.rows8_checkpoint else x_op)                     # per layer: what the encoders' gradient rows gather
+                      if holder["keep8"] else x_op)                        # per layer: what the encoders' gradient rows gather
         ctx.shape = (B, L, d, F)
         ctx.amp = bool(amp)
         ctx.defer_to = m if holder.get("defer") else None
@@ -599,7 +599,8 @@ class CrossLayerTranscoder(SparseDictionary):
         n_tokens = (lambda: batch["tokens"].numel()) if mask is None else (lambda: int(mask.sum().item()))
         if self._fused_eligible(x, sparsity_loss_type):
             amp = _autocast_dtype("cuda") == torch.bfloat16
-            holder: dict[str, Any] = {"model": self, "defer": self.defer_weight_grads and torch.is_grad_enabled()}
+            holder: dict[str, Any] = {"model": self, "defer": self.defer_weight_grads and torch.is_grad_enabled(),
+                                      "keep8": self._keep_rows8()}
             xin = x.to(torch.float32) if x.dtype not in (torch.float32, torch.bfloat16) else x
             loss, recon = _FusedCLTStep.apply(xin, label.to(torch.float32), amp, holder, self.W_E, self.b_E,
                                               *self.W_D, *self.b_D)

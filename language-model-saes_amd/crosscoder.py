@@ -46,7 +46,7 @@ class _FusedCrosscoderStep(torch.autograd.Function):
         F = m.cfg.d_sae
         w_enc_op = m._w_enc_operand(amp)                              # [F, H*d]
         x_cat = x.reshape(B, H * d)
-        x_op, x_kept = _input_operand(x_cat, amp, m.rows8_checkpoint)
+        x_op, x_kept = _input_operand(x_cat, amp, holder["keep8"])
         pre = ops.encoder_gemm(x_op, w_enc_op, torch.bfloat16 if amp else torch.float32)
         norms = m._decoder_norm_nograd()                              # [H, F]
         w_dec_op = m._w_dec_operand(amp)                              # [H, F, d]
@@ -344,7 +344,8 @@ class Crosscoder(SparseDictionary):
             mf = mask.to(torch.float32)
             tok_w = mf / mf.sum()
         amp = _autocast_dtype("cuda") == torch.bfloat16
-        holder: dict[str, Any] = {"model": self, "defer": self.defer_weight_grads and torch.is_grad_enabled()}
+        holder: dict[str, Any] = {"model": self, "defer": self.defer_weight_grads and torch.is_grad_enabled(),
+                                  "keep8": self._keep_rows8()}
         xin = x.to(torch.float32) if x.dtype not in (torch.float32, torch.bfloat16) else x
         loss, recon = _FusedCrosscoderStep.apply(xin.contiguous(), label.to(torch.float32).contiguous(), tok_w, self.W_E,
                                                  self.b_E, self.W_D, self.b_D, int(self.current_k), amp, holder)

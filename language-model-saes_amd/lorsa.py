@@ -114,11 +114,11 @@ class _ProjectAndMix(torch.autograd.Function):
         return q, k, v, out, lse
 
     @staticmethod
-    def forward(ctx, x2, W_Q, W_K, W_V, b_Q, b_K, b_V, model, seq):
+    def forward(ctx, x2, W_Q, W_K, W_V, b_Q, b_K, b_V, model, seq, keep8):
         cfg = model.cfg
         T = x2.shape[0]
         n_batch, h = T // seq, cfg.n_qk_heads
-        x_op, x_kept = _input_operand(x2, True, model.rows8_checkpoint)
+        x_op, x_kept = _input_operand(x2, True, keep8)
         operands = (model._w_qk_operand("W_Q"), model._w_qk_operand("W_K"), model._w_val_operand(True))
         biases = (b_Q.detach(), b_K.detach(), b_V.detach())
         rot = ((model._rotary_tables(), cfg.rotary_dim, cfg.rotary_adjacent_pairs)
@@ -173,7 +173,7 @@ class _ProjectAndMix(torch.autograd.Function):
         if ctx.needs_input_grad[0]:
             # rare (activations do not carry gradients in training): library products on the transposed gradients
             dx = (dqt.t().float() @ wq.float() + dkt.t().float() @ wk.float() + dvt.t().float() @ wv.float()).to(ctx.x_dtype)
-        return dx, dW_Q, dW_K, dW_V, db_Q, db_K, db_V, None, None
+        return dx, dW_Q, dW_K, dW_V, db_Q, db_K, db_V, None, None, None
 
 
 class _AttentionMix(torch.autograd.Function):
@@ -563,7 +563,8 @@ class LowRankSparseAttention(SparseDictionary):
         """lorsa.py:642-662: causal attention of every feature's value over key positions."""
         if self._mix_kernel_eligible(x):
             b, s, d = x.shape
-            z = _ProjectAndMix.apply(x.reshape(b * s, d), self.W_Q, self.W_K, self.W_V, self.b_Q, self.b_K, self.b_V, self, s)
+            z = _ProjectAndMix.apply(x.reshape(b * s, d), self.W_Q, self.W_K, self.W_V, self.b_Q, self.b_K, self.b_V, self, s,
+                                     self._keep_rows8())
             return z.view(b, s, self.cfg.d_sae)
         q, k, v = self._compute_qkv(x)
         if self._attention_kernel_eligible(x):

@@ -42,6 +42,7 @@ class _Holder:
     scale: Optional[torch.Tensor] = None
     defer_to: Optional["SparseAutoEncoder"] = None  # module whose optimiser consumes factored weight gradients
     model: Optional["SparseAutoEncoder"] = None
+    keep8: bool = False             # hold the step's inputs in 8 bits for the backward pass
     aux: Optional[dict] = None      # aux-k request: {"is_dead": callable(code) -> bool [F], "k_aux": int, "coefficient": float}
     aux_code: ops.SparseCode = None
     l_aux: Optional[torch.Tensor] = None
@@ -284,7 +285,7 @@ class _FusedSparseStep(torch.autograd.Function):
                    and (ops.granule_route_supported(x.shape[1], w_enc_op.shape[0], int(k)) if not batch_wide
                         else x.shape[1] % 64 == 0 and w_enc_op.shape[0] % 256 == 0))
         gmax = None
-        x_op, x_kept = _input_operand(x, amp, sae.rows8_checkpoint)
+        x_op, x_kept = _input_operand(x, amp, holder.keep8)
         if granule:
             scale = sae._decoder_norm_nograd() if sae.cfg.sparsity_include_decoder_norm else None
             if lowp and scale is not None:
@@ -461,7 +462,7 @@ class _GluSparseStep(torch.autograd.Function):
     def forward(ctx, x, label, tok_w, W_E, b_E, W_G, b_G, W_D, b_D, k, amp, holder):
         sae = holder.model
         w_enc_op, w_glu_op = sae._w_enc_operand(amp), sae._w_glu_operand(amp)
-        x_op, x_kept = _input_operand(x, amp, sae.rows8_checkpoint)
+        x_op, x_kept = _input_operand(x, amp, holder.keep8)
         out_dtype = torch.bfloat16 if amp else torch.float32
         pre, pre_g = ops.encoder_gemm(x_op, w_enc_op, out_dtype), ops.encoder_gemm(x_op, w_glu_op, out_dtype)
         lin = pre.float() + b_E
@@ -1082,7 +1083,7 @@ class SparseAutoEncoder(SparseDictionary):
             m = mask.to(torch.float32)
             tok_w = m / m.sum()
         holder = _Holder()
-        holder.model = self
+        holder.model, holder.keep8 = self, self._keep_rows8()
         loss, recon = _GluSparseStep.apply(
             x.to(torch.float32) if x.dtype not in (torch.float32, torch.bfloat16) else x, label.to(torch.float32).contiguous(),
             tok_w, self.W_E, self.b_E, self.W_E_glu, self.b_E_glu, self.W_D, self.b_D if self.cfg.use_decoder_bias else None,
@@ -1133,12 +1134,12 @@ class SparseAutoEncoder(SparseDictionary):
         want_tanh, want_lp = sparsity_loss_type == "tanh", lp_coefficient > 0.0 and is_jr
         scaled = bool(self.cfg.sparsity_include_decoder_norm)
         w_enc_op = self._w_enc_operand(amp)
-        given = None
+        given, keep8 = None, self._keep_rows8()
         B = x.shape[0]
         if (self.jumprelu_sparse_route and not want_lp and B <= 131072
                 and self.cfg.d_model % 8 == 0 and self._jr_dense_steps % max(1, self.jumprelu_sparse_probe_every) == 0):
             with torch.no_grad():
-                x_op, x_kept = _input_operand(x, amp, self.rows8_checkpoint)
+                x_op, x_kept = _input_operand(x, amp, keep8)
                 n_raw = self._decoder_norm_nograd() if (scaled or sparsity_loss_type is not None) else None
                 th_raw = theta.detach().float().contiguous()
                 b_raw = self.b_E.detach().float()
@@ -1162,7 +1163,7 @@ class SparseAutoEncoder(SparseDictionary):
                                               sparsity_loss_type, tanh_tok, float(tanh_stretch_coefficient), float(l1_coefficient),
                                               float(frequency_scale), p, lp_coefficient, auxk_coefficient, return_aux_data)
         self._jr_dense_steps += 1
-        pre = _EncoderGemm.apply(x, self.W_E, w_enc_op, amp, defer, given, None, self._keep_rows8())
+        pre = _EncoderGemm.apply(x, self.W_E, w_enc_op, amp, defer, given, None, keep8)
         n = None
         want_dense_pen = sparsity_loss_type in ("power", "tanh-quad")
         if scaled or want_tanh or want_lp or want_dense_pen:
@@ -1246,7 +1247,7 @@ class SparseAutoEncoder(SparseDictionary):
         return LazyDict(eager, lazy)
 
     @torch.no_grad()
-    def _select_code(self, x: torch.Tensor, amp: bool):
+    def _select_code(self, x: torch.Tensor, amp: bool, keep8: bool):
         """GEMM + TopK / BatchTopK select of an fp32 dictionary -> (x for the backward pass, pre, code): what the forward of
         the fused step does, for the routes that continue from the code with other losses."""
         w_enc_op = self._w_enc_operand(amp)
@@ -1255,7 +1256,7 @@ class SparseAutoEncoder(SparseDictionary):
         b_E = self.b_E.detach().float()
         scale = self._decoder_norm_nograd() if self.cfg.sparsity_include_decoder_norm else None
         gmax = None
-        x_op, x_kept = _input_operand(x, amp, self.rows8_checkpoint)
+        x_op, x_kept = _input_operand(x, amp, keep8)
         if amp:
             granule = (getattr(self, "granule_select", True)
                        and (ops.granule_route_supported(x.shape[1], w_enc_op.shape[0], k) if not batch_wide
@@ -1337,7 +1338,7 @@ class SparseAutoEncoder(SparseDictionary):
             # TopK / BatchTopK with a sparsity penalty: select as the plain step does, then decode, loss, penalty and the
             # backward on the code (the penalty's gradient joins the decoder's at every kept entry and reaches W_D
             # through the decoder norm)
-            x_rows, pre, code = self._select_code(x, amp)
+            x_rows, pre, code = self._select_code(x, amp, self._keep_rows8())
             defer = bool(self.defer_weight_grads and torch.is_grad_enabled())
             theta, window = self._threshold_and_window() if self.cfg.act_fn.lower() == "jumprelu" else (
                 torch.zeros(1, dtype=torch.float32, device=x.device), 1.0)
@@ -1350,7 +1351,7 @@ class SparseAutoEncoder(SparseDictionary):
             m = mask.to(torch.float32)
             tok_w = m / m.sum()
         holder = _Holder()
-        holder.model = self
+        holder.model, holder.keep8 = self, self._keep_rows8()
         if auxk_coefficient > 0.0:
             assert update_dead_statistics is not None, "update_dead_statistics must be set when auxk_coefficient > 0.0"
 

@@ -95,7 +95,8 @@ class SparseDictionary(nn.Module):
         self._derived: dict[str, tuple[int, torch.Tensor]] = {}
 
     def _keep_rows8(self) -> bool:
-        """Whether a product outside the kernel steps is to hold its saved side in 8 bits."""
+        """Whether a step or product is to hold what its backward pass reads in 8 bits; asked in the caller's grad mode (inside an
+        autograd function it is off): without a backward pass no records are written."""
         return self.rows8_checkpoint and torch.is_grad_enabled()
 
     # ---- derived operands, refreshed when the parameter's version counter moves ----

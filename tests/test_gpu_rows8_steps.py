@@ -564,6 +564,64 @@ def test_a_stretch_of_an_index(pkg, dev, T):
         assert close(rows, whole[lo:hi], size[lo:hi], T, False) and torch.equal(b, bias[lo:hi]) and (frame[0] == 7).all() and (frame[-1] == 7).all()
 
 
+def make_variant(pkg, dev, kind):
+    """A small crosscoder, cross-layer transcoder or Lorsa, and a batch of it."""
+    n, d, F, B = 2, 64, 256, 128
+    common = dict(d_model=d, expansion_factor=F / d, act_fn="topk", top_k=5, norm_activation="inference", device="cuda", dtype=torch.float32)
+    g = torch.Generator(device=dev).manual_seed(2)
+    x = torch.randn(n, B, d, generator=g, device=dev)
+    hin, hout = [f"i{i}" for i in range(n)], [f"o{i}" for i in range(n)]
+    if kind == "crosscoder":
+        model = pkg.Crosscoder(pkg.CrosscoderConfig(hook_points=hin, **common))
+    elif kind == "clt":
+        model = pkg.CrossLayerTranscoder(pkg.CLTConfig(hook_points_in=hin, hook_points_out=hout, **common))
+    else:
+        model = pkg.LowRankSparseAttention(pkg.LorsaConfig(hook_point_in="i0", hook_point_out="o0", n_qk_heads=4, d_qk_head=32, n_ctx=64,
+                                                           positional_embedding_type="none", rotary_dim=32, **common))
+        x = x.view(2, 2, 64, d)
+    with torch.no_grad():
+        for p in model.parameters():
+            p.copy_(torch.randn(p.shape, generator=g, device=dev) * 0.1)
+    return model, dict(zip(hin, x)) | dict(zip(hout, x.flip(0))) | {"tokens": torch.zeros(x.shape[1:-1], device=dev)}
+
+
+KINDS = list(range(len(STEPS))) + ["aux", "dense", "crosscoder", "clt"]
+
+
+@pytest.mark.parametrize("kind,amp", [(k, amp) for k in KINDS for amp in (False, True)] + [("lorsa", True)])
+def test_records_are_written_for_a_backward_pass_only(pkg, dev, kind, amp):
+    """A loss without gradients (an evaluation, a search over scales) is that of the model without the option, and writes nothing."""
+    kw = {}
+    if kind in ("crosscoder", "clt", "lorsa"):
+        model, batch = make_variant(pkg, dev, kind)
+    elif kind == "aux":
+        model, batch = make_sae(pkg, dev)
+        dead = torch.arange(640, device=dev) % 3 == 0
+        kw = dict(auxk_coefficient=0.1, k_aux=16, update_dead_statistics=lambda *a, **k: dead)
+    elif kind == "dense":
+        model, batch = make_sae(pkg, dev, "relu")
+        model.jumprelu_sparse_route = False
+    else:
+        act_fn, cfg, kw = STEPS[kind]
+        model, batch = make_sae(pkg, dev, act_fn, **cfg)
+    timer = pkg.ops.KernelTimer()
+    pkg.ops.set_kernel_timer(timer)
+    try:
+        losses = []
+        for keep, mode in ((False, torch.no_grad), (True, torch.no_grad), (True, torch.inference_mode)):
+            model.rows8_checkpoint = keep
+            with mode(), autocast(amp):
+                losses.append(model.compute_loss(batch, **kw)["loss"].clone())
+        assert torch.equal(losses[0], losses[1]) and torch.equal(losses[0], losses[2])
+        assert "rows8_quantize" not in timer.records
+        with autocast(amp):
+            loss = model.compute_loss(batch, **kw)["loss"]
+        assert torch.equal(loss.detach(), losses[0]) and "rows8_quantize" in timer.records
+        loss.backward()
+    finally:
+        pkg.ops.set_kernel_timer(None)
+
+
 # ---- the stream --------------------------------------------------------------------------------------------------
 
 def test_records_made_on_either_side_are_the_same(pkg, dev):
