@@ -132,11 +132,22 @@ def stack_codes(a: SparseCode, b: SparseCode) -> SparseCode:
                       a.n_tokens + b.n_tokens, a.d_sae)
 
 
-@dataclass
+@dataclass(frozen=True, eq=False)
 class FeatureIndex:
+    """Slots of a sparse code by feature (`build_feature_index`).  The kernels read the three arrays by their addresses, so an index
+    is made of 32-bit entries that lie side by side, and stays what it was made."""
+
     feat_ptr: torch.Tensor   # int32 [F + 1]
     feat_slot: torch.Tensor  # int32 [n_slots]
     slot_tok: torch.Tensor   # int32 [n_slots]
+
+    def __post_init__(self):
+        for name in ("feat_ptr", "feat_slot", "slot_tok"):
+            t = getattr(self, name)
+            if t.dtype != torch.int32:
+                raise TypeError(f"{name} must be {torch.int32}, got {t.dtype}")
+            if t.ndim != 1 or not t.is_contiguous():
+                raise ValueError(f"{name} must be one contiguous axis, got {tuple(t.shape)} with strides {t.stride()}")
 
 
 ROWS8_BLOCK = 32             # values that share a step in rows held in 8 bits
@@ -227,6 +238,15 @@ def _req_dense(dense, name: str = "dense"):
         return dense.data.data_ptr(), SAE_ROWS8, "rows8"
     _req(dense, name, ndim=2)
     return dense.data_ptr(), _dt(dense), "bf16" if dense.dtype == torch.bfloat16 else "f32"
+
+
+def _req_slots(fi: FeatureIndex, coef: torch.Tensor):
+    """Every slot of the index has a coefficient, on the same device."""
+    n, dev = coef.numel(), coef.get_device()
+    if fi.slot_tok.numel() > n or fi.feat_slot.numel() > n:
+        raise ValueError(f"{n} coefficients for a feature index of {fi.feat_slot.numel()} slots")
+    if fi.feat_ptr.get_device() != dev or fi.feat_slot.get_device() != dev or fi.slot_tok.get_device() != dev:
+        raise ValueError("the index and the coefficients must be on one device")
 
 
 # ---- element-wise ---------------------------------------------------------------------------
@@ -979,6 +999,7 @@ def adam_step_sparse_rows(fi: FeatureIndex, coef: torch.Tensor, dense: torch.Ten
         raise ValueError("shape mismatch between p, m, v and the dense operand")
     if fi.feat_ptr.numel() != F + 1:
         raise ValueError("feature index was built for a different number of features")
+    _req_slots(fi, coef)
     if shadow_bf16 is not None:
         _req(shadow_bf16, "shadow_bf16", torch.bfloat16)
     if grad_scale is not None:
@@ -1039,6 +1060,7 @@ def sparse_rows_grad_sq_nnz(fi: FeatureIndex, coef: torch.Tensor, dense: torch.T
     (fi, coef, dense) stand for; optionally writes the per-feature bias gradient as well."""
     _req(coef, "coef", torch.float32, 1)
     dense_ptr, dense_dt, _ = _req_dense(dense)
+    _req_slots(fi, coef)
     _req(acc, "acc", torch.float64, 1)
     F, d = fi.feat_ptr.numel() - 1, dense.shape[1]
     lib = _lib.load()

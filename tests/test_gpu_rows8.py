@@ -614,3 +614,20 @@ def test_refusals_on_the_device(pkg, dev):
     odd = ops.quantize_rows(activations(8, 66, 25))
     with pytest.raises(RuntimeError):                                        # the Adam pass moves four values at a time
         ops.adam_step_sparse_rows(fi, code.val, odd, p, p.clone(), p.clone(), lr=1e-3, beta1=0.9, beta2=0.99, eps=1e-8, step=1)
+
+
+def test_an_index_that_does_not_fit_is_refused(pkg, dev):
+    ops = pkg.ops
+    q = ops.quantize_rows(activations(8, 64, 23))
+    code = sparse_code(ops, 8, 6, 2, 24, dev)
+    fi = ops.build_feature_index(code)
+    short, wide = code.val[:-1].contiguous(), torch.zeros(6, 64, device=dev)
+    with pytest.raises(ValueError):
+        ops.adam_step_sparse_rows(fi, short, q, wide, wide.clone(), wide.clone(), lr=1e-3, beta1=0.9, beta2=0.99, eps=1e-8, step=1)
+    with pytest.raises(ValueError):
+        ops.sparse_rows_grad_sq_nnz(fi, short, q, torch.zeros(2, dtype=torch.float64, device=dev))
+    host = ops.FeatureIndex(fi.feat_ptr.cpu(), fi.feat_slot, fi.slot_tok)
+    for call in (lambda: ops.sparse_grad_rows(host, code.val, q, 6),
+                 lambda: ops.sparse_rows_grad_sq_nnz(host, code.val, q, torch.zeros(2, dtype=torch.float64, device=dev))):
+        with pytest.raises(ValueError):
+            call()

@@ -40,6 +40,31 @@ def test_rows8_stay_what_they_were_made(pkg):
             setattr(q, name, value)
 
 
+def test_an_index_is_of_32_bit_entries_side_by_side(pkg):
+    """The kernels read it by its addresses: wider entries, or entries that lie apart, would be read as slots and tokens that do not
+    exist."""
+    ptr, slot, tok = (torch.zeros(n, dtype=torch.int32) for n in (5, 8, 8))
+    fi = pkg.FeatureIndex(ptr, slot, tok)
+    for i in range(3):
+        for wrong in (torch.int64, torch.int16, torch.float32):
+            with pytest.raises(TypeError):
+                pkg.FeatureIndex(*[t.to(wrong) if j == i else t for j, t in enumerate((ptr, slot, tok))])
+        for wrong in (lambda t: torch.stack([t, t], 1)[:, 0], lambda t: t[None], lambda t: t[:1].expand(len(t))):
+            with pytest.raises(ValueError):
+                pkg.FeatureIndex(*[wrong(t) if j == i else t for j, t in enumerate((ptr, slot, tok))])
+    assert pkg.FeatureIndex(ptr[1:4], slot, tok).feat_ptr.numel() == 3
+    for name in ("feat_ptr", "feat_slot", "slot_tok"):
+        with pytest.raises(AttributeError):
+            setattr(fi, name, tok.long())
+
+
+def test_every_slot_has_a_coefficient(pkg):
+    fi = pkg.FeatureIndex(*(torch.zeros(n, dtype=torch.int32) for n in (5, 8, 8)))
+    pkg.ops._req_slots(fi, torch.zeros(8))
+    with pytest.raises(ValueError, match="7 coefficients"):
+        pkg.ops._req_slots(fi, torch.zeros(7))
+
+
 def test_the_kernels_have_no_cpu_fallback(pkg):
     ops = pkg.ops
     q = ops.Rows8(torch.zeros(3, 80, dtype=torch.uint8), 40)
