@@ -522,7 +522,7 @@ int sae_transpose_padded(const void *src, int src_dtype, int64_t rows, int64_t c
 
 /* out[i, j] = sum_t left[t, i] right[t, j] for left [tokens, m] and right [tokens, n], each in SAE_F32, SAE_BF16 or SAE_ROWS8: a
  * weight gradient over the token axis (dW = d(pre)^T x, acts^T d(recon)) whose saved side may be held in records.  Any widths
- * and token counts; records enter exactly.  With an fp32 operand fp32 products are formed and out is SAE_F32; otherwise bf16
+ * up to m = 2^24 and n = 65535 * 64, any token counts; records enter exactly.  With an fp32 operand fp32 products are formed and out is SAE_F32; otherwise bf16
  * products with fp32 sums, out in SAE_F32 or SAE_BF16.  n_slices > 1 cuts the tokens (slabs of 64, or 32 with an fp32 operand;
  * at most one slice per slab) for products with few outputs: partials is then fp32 [n_slices, m, n], summed in token order.
  * Made for products that are small or that no slab divides; sae_gemm_bf16 runs large ones faster. */

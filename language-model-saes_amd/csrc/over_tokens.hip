@@ -17,6 +17,7 @@
 namespace sae {
 
 constexpr int OT_TILE = 64;
+constexpr int64_t OT_COLUMNS = 1LL << 24;   // of an operand: 64 bf16 or 32 fp32 rows, a slab, stay within 32-bit offsets
 constexpr int OT_AHEAD = 2;   // slabs on their way in registers (four: no less time)
 typedef __attribute__((ext_vector_type(4))) float ot_f32x4;
 typedef __attribute__((ext_vector_type(8))) __bf16 ot_bf16x8;
@@ -341,7 +342,8 @@ extern "C" int sae_gemm_over_tokens(const void *left, int left_dtype, const void
   const bool wide = left_dtype == SAE_F32 || right_dtype == SAE_F32;
   SAE_REQUIRE(out_dtype == SAE_F32 || (out_dtype == SAE_BF16 && !wide), SAE_ERR_INVALID_ARG, "gemm_over_tokens: bad out_dtype %d", out_dtype);
   const int64_t slab = wide ? 32 : 64, slabs = (tokens + slab - 1) / slab;
-  SAE_REQUIRE(m <= 65535LL * OT_TILE && n <= 65535LL * OT_TILE && slabs < (1LL << 30), SAE_ERR_UNSUPPORTED, "gemm_over_tokens: size too large");
+  // left's tiles are the grid's x, right's its y, which ends at 65535
+  SAE_REQUIRE(m <= OT_COLUMNS && n <= 65535LL * OT_TILE && slabs < (1LL << 30), SAE_ERR_UNSUPPORTED, "gemm_over_tokens: size too large");
   SAE_REQUIRE(n_slices == 1 || (m * n + 1023) / 1024 < (1LL << 31), SAE_ERR_UNSUPPORTED, "gemm_over_tokens: too many outputs for slices");
   SAE_REQUIRE(n_slices <= 65535 && n_slices <= slabs && (n_slices == 1 || partials), SAE_ERR_INVALID_ARG,
               "gemm_over_tokens: %lld slices of %lld slabs (with partial results for more than one)", (long long)n_slices, (long long)slabs);

@@ -1541,6 +1541,7 @@ def _operand_dt(t) -> int:
 
 
 OVER_TOKENS_FLOP = 4.3e10      # of a product on 64 x 64 tiles at most, a tile counted 1000 tokens longer than it is
+OVER_TOKENS_WIDTHS = (1 << 24, 65535 * 64)      # of left and right on 64 x 64 tiles at most
 
 
 @functools.lru_cache(maxsize=1024)
@@ -1567,8 +1568,8 @@ def _over_tokens_slices(tokens: int, m: int, n: int, wide: bool) -> int:
 
 def gemm_over_tokens(left, right, out_dtype: torch.dtype = torch.float32) -> torch.Tensor:
     """left^T @ right -> [m, n] for left [tokens, m] and right [tokens, n], each bf16, fp32 or `Rows8`: a weight gradient
-    d(pre)^T x or acts^T d(recon) whose saved side is held in 8 bits.  Any number of tokens and any widths.  Operands held in 8
-    bits are exact in bf16; with an fp32 operand the product is an fp32 product (and so is `out_dtype`), otherwise a bf16
+    d(pre)^T x or acts^T d(recon) whose saved side is held in 8 bits.  Any number of tokens and any widths (with an fp32
+    operand up to 2^24).  Operands held in 8 bits are exact in bf16; with an fp32 operand the product is an fp32 product (and so is `out_dtype`), otherwise a bf16
     product with fp32 accumulation.
 
     Small and middle products, and all fp32 ones, run on a kernel of 64 x 64 tiles that reads every operand as it lies; larger
@@ -1598,7 +1599,9 @@ def gemm_over_tokens(left, right, out_dtype: torch.dtype = torch.float32) -> tor
         raise TypeError(f"out_dtype {out_dtype} of a product of {'fp32' if wide else 'bf16'} operands")
     if T == 0:
         return torch.zeros(m, n, dtype=out_dtype, device=dev)
-    if wide or 2.0 * (T + 1000) * m * n <= OVER_TOKENS_FLOP:
+    if wide or (2.0 * (T + 1000) * m * n <= OVER_TOKENS_FLOP and max(m, n) <= OVER_TOKENS_WIDTHS[0]):
+        if n > OVER_TOKENS_WIDTHS[1] >= m:       # the tiles of left take a wider one: the same sums, the other way round
+            return gemm_over_tokens(right, left, out_dtype).t().contiguous()
         slices = _over_tokens_slices(T, m, n, wide)
         out = torch.empty(m, n, dtype=out_dtype, device=dev)
         part = torch.empty(slices * m * n, dtype=torch.float32, device=dev) if slices > 1 else None

@@ -360,6 +360,24 @@ def test_what_is_not_finite_stays_in_its_row_and_column(pkg, dev, kind):
     assert torch.isnan(got[:, :32]).all() and torch.equal(got[:, 32:], want[:, 32:])
 
 
+def whole(shape, seed, dev, top=2):
+    """Whole numbers up to `top`: every product and sum of few of them is exact in any order, in bf16 products too."""
+    return torch.randint(-top, top + 1, shape, generator=torch.Generator(device=dev).manual_seed(seed), device=dev).float()
+
+
+@pytest.mark.parametrize("T,m,n", [(64, 4300000, 4), (65, 3, 4300001), (1, 4194241, 1), (2, 1, 4194241)])
+@pytest.mark.parametrize("kind", ["bf16", "f32", "rows8"])
+def test_products_of_very_wide_operands(pkg, dev, T, m, n, kind):
+    ops = pkg.ops
+    left, right = whole((T, m), 1, dev), whole((T, n), 2, dev)
+    want = left.t() @ right
+    make = {"bf16": lambda x: x.bfloat16(), "f32": lambda x: x, "rows8": ops.quantize_rows}[kind]
+    got = ops.gemm_over_tokens(make(left), ops.quantize_rows(right))
+    assert got.dtype == torch.float32 and got.is_contiguous() and torch.equal(got, want)
+    got = ops.gemm_over_tokens(ops.quantize_rows(left), make(right), torch.float32 if kind == "f32" else torch.bfloat16)
+    assert got.is_contiguous() and torch.equal(got.float(), want.to(got.dtype).float())
+
+
 def test_no_tokens(pkg, dev):
     ops = pkg.ops
     q = ops.quantize_rows(torch.empty(0, 40, device=dev))
