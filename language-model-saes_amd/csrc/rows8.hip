@@ -240,9 +240,9 @@ __global__ __launch_bounds__(256) void rows8_gather_kernel(const uint8_t *__rest
 // fall on 64 banks), so that an output row leaves in whole 16-byte stores of 8 tokens.
 template <int SRC>
 __global__ __launch_bounds__(256) void transpose_padded_kernel(const void *__restrict__ src, int64_t rows, int64_t cols, uint16_t *__restrict__ dst,
-                                                               int64_t dst_pitch) {
+                                                               int64_t dst_pitch, uint32_t col_blocks) {
   __shared__ uint32_t tile[2][64 * 33];
-  const int64_t r0 = (int64_t)blockIdx.y * 128, c0 = (int64_t)blockIdx.x * 64;
+  const int64_t r0 = (int64_t)(blockIdx.x / col_blocks) * 128, c0 = (int64_t)(blockIdx.x % col_blocks) * 64;
   const int group = threadIdx.x & 7, pair = threadIdx.x >> 3;   // 8 columns, and 32 pairs of rows
   const int64_t col = c0 + group * 8, end = SRC == SAE_ROWS8 ? r8_blocks(cols) * R8_BLOCK : cols;
   const size_t pitch = dense_row_bytes<SRC>(cols);
@@ -673,13 +673,15 @@ extern "C" int sae_transpose_padded(const void *src, int src_dtype, int64_t rows
   SAE_REQUIRE(((uintptr_t)dst & 15) == 0 && (src_dtype != SAE_ROWS8 || ((uintptr_t)src & 15) == 0), SAE_ERR_INVALID_ARG,
               "transpose_padded: 16-byte alignment required");
   const int64_t gy = (dst_pitch + 127) / 128, gx = (cols + 63) / 64;
-  SAE_REQUIRE(gy <= 65535 && cols < (1LL << 30), SAE_ERR_UNSUPPORTED, "transpose_padded: %lld rows, at most %d", (long long)dst_pitch, 65535 * 128);
-  const dim3 grid((unsigned)gx, (unsigned)gy);
+  // one grid axis of less than 2^32 threads: 2^24 workgroups write 256 GiB
+  SAE_REQUIRE(dst_pitch < (1LL << 30) && cols < (1LL << 30) && gx * gy < (1LL << 24), SAE_ERR_UNSUPPORTED,
+              "transpose_padded: %lld x %lld is too large", (long long)dst_pitch, (long long)cols);
+  const dim3 grid((unsigned)(gx * gy));
   uint16_t *out = reinterpret_cast<uint16_t *>(dst);
   if (src_dtype == SAE_ROWS8)
-    hipLaunchKernelGGL(transpose_padded_kernel<SAE_ROWS8>, grid, dim3(256), 0, (hipStream_t)stream, src, rows, cols, out, dst_pitch);
+    hipLaunchKernelGGL(transpose_padded_kernel<SAE_ROWS8>, grid, dim3(256), 0, (hipStream_t)stream, src, rows, cols, out, dst_pitch, (uint32_t)gx);
   else
-    hipLaunchKernelGGL(transpose_padded_kernel<SAE_BF16>, grid, dim3(256), 0, (hipStream_t)stream, src, rows, cols, out, dst_pitch);
+    hipLaunchKernelGGL(transpose_padded_kernel<SAE_BF16>, grid, dim3(256), 0, (hipStream_t)stream, src, rows, cols, out, dst_pitch, (uint32_t)gx);
   return check_launch("transpose_padded");
 }
 

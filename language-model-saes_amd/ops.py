@@ -1599,7 +1599,9 @@ def gemm_over_tokens(left, right, out_dtype: torch.dtype = torch.float32) -> tor
         raise TypeError(f"out_dtype {out_dtype} of a product of {'fp32' if wide else 'bf16'} operands")
     if T == 0:
         return torch.zeros(m, n, dtype=out_dtype, device=dev)
-    if wide or (2.0 * (T + 1000) * m * n <= OVER_TOKENS_FLOP and max(m, n) <= OVER_TOKENS_WIDTHS[0]):
+    pitch = -(-T // 64) * 64
+    small = 2.0 * (T + 1000) * m * n <= OVER_TOKENS_FLOP and max(m, n) <= OVER_TOKENS_WIDTHS[0]
+    if wide or small or pitch >= 1 << 28:                   # the GEMM kernel's contractions end there
         if n > OVER_TOKENS_WIDTHS[1] >= m:       # the tiles of left take a wider one: the same sums, the other way round
             return gemm_over_tokens(right, left, out_dtype).t().contiguous()
         slices = _over_tokens_slices(T, m, n, wide)
@@ -1609,7 +1611,6 @@ def gemm_over_tokens(left, right, out_dtype: torch.dtype = torch.float32) -> tor
         _launch("gemm_over_tokens", lt, _lib.load().sae_gemm_over_tokens, lt.data_ptr(), left_dt, rt.data_ptr(), right_dt, T, m, n,
                 out.data_ptr(), _dt(out), slices, _ptr(part))
         return out
-    pitch = -(-T // 64) * 64
 
     def operand(t, rows, other_rows, a_side):
         """(operand, whether it is stored [tokens, columns])"""

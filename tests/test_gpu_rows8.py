@@ -378,6 +378,21 @@ def test_products_of_very_wide_operands(pkg, dev, T, m, n, kind):
     assert got.is_contiguous() and torch.equal(got.float(), want.to(got.dtype).float())
 
 
+@pytest.mark.parametrize("kind", ["bf16", "rows8"])
+def test_products_over_very_many_tokens(pkg, dev, kind):
+    """More tokens than one grid axis of 128-token tiles counts; sums of ones, exact in fp32 in any order."""
+    ops = pkg.ops
+    T, m, n = 65535 * 128 + 77, 72, 66
+    left, right = whole((T, m), 3, dev, 1).bfloat16(), whole((T, n), 4, dev, 1)
+    q, l8 = ops.quantize_rows(right), ops.quantize_rows(left)
+    assert 2.0 * T * m * n > ops.OVER_TOKENS_FLOP
+    want = torch.zeros(m, n, dtype=torch.float64, device=dev)
+    for t in range(0, T, 1 << 20):
+        want += left[t : t + (1 << 20)].double().t() @ right[t : t + (1 << 20)].double()
+    got = ops.gemm_over_tokens(left if kind == "bf16" else l8, q)
+    assert torch.equal(got.double(), want)
+
+
 def test_no_tokens(pkg, dev):
     ops = pkg.ops
     q = ops.quantize_rows(torch.empty(0, 40, device=dev))
