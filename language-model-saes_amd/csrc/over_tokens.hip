@@ -327,7 +327,7 @@ extern "C" int sae_join_slices(const float *partials, int64_t n_slices, int64_t 
   SAE_REQUIRE(partials && out, SAE_ERR_INVALID_ARG, "join_slices: null pointer");
   SAE_REQUIRE(n_slices > 0 && count > 0, SAE_ERR_INVALID_ARG, "join_slices: sizes must be positive");
   SAE_REQUIRE(out_dtype == SAE_F32 || out_dtype == SAE_BF16, SAE_ERR_INVALID_ARG, "join_slices: bad dtype %d", out_dtype);
-  SAE_REQUIRE(n_slices < (1LL << 31) && (count + 1023) / 1024 < (1LL << 31), SAE_ERR_UNSUPPORTED, "join_slices: size too large");
+  SAE_REQUIRE(n_slices < (1LL << 31) && (count + 1023) / 1024 < (1LL << 24), SAE_ERR_UNSUPPORTED, "join_slices: size too large");
   launch_join(partials, count, n_slices, out, out_dtype, (hipStream_t)stream);
   return check_launch("join_slices");
 }
@@ -344,7 +344,7 @@ extern "C" int sae_gemm_over_tokens(const void *left, int left_dtype, const void
   const int64_t slab = wide ? 32 : 64, slabs = (tokens + slab - 1) / slab;
   // left's tiles are the grid's x, right's its y, which ends at 65535
   SAE_REQUIRE(m <= OT_COLUMNS && n <= 65535LL * OT_TILE && slabs < (1LL << 30), SAE_ERR_UNSUPPORTED, "gemm_over_tokens: size too large");
-  SAE_REQUIRE(n_slices == 1 || (m * n + 1023) / 1024 < (1LL << 31), SAE_ERR_UNSUPPORTED, "gemm_over_tokens: too many outputs for slices");
+  SAE_REQUIRE(n_slices == 1 || (m * n + 1023) / 1024 < (1LL << 24), SAE_ERR_UNSUPPORTED, "gemm_over_tokens: too many outputs for slices");
   SAE_REQUIRE(n_slices <= 65535 && n_slices <= slabs && (n_slices == 1 || partials), SAE_ERR_INVALID_ARG,
               "gemm_over_tokens: %lld slices of %lld slabs (with partial results for more than one)", (long long)n_slices, (long long)slabs);
   SAE_REQUIRE((left_dtype != SAE_ROWS8 || ((uintptr_t)left & 15) == 0) && (right_dtype != SAE_ROWS8 || ((uintptr_t)right & 15) == 0),

@@ -8,6 +8,8 @@
 // value = code * step.  A code has 7 magnitude bits and the step is a power of two between 2^-126 and 2^121, so every value
 // is exact in bf16 and the product below is exact in fp32; field 255 is the float infinity, and 0 * inf makes every value of
 // such a block NaN without a test.
+#include <algorithm>
+
 #include "common.h"
 
 namespace sae {
@@ -713,13 +715,18 @@ extern "C" int sae_rows8_grad_rows(const int32_t *feat_ptr, const int32_t *feat_
   const uint8_t *rec = reinterpret_cast<const uint8_t *>(rows);
   const int64_t feat_blocks = (F + 3) / 4, chunks = (r8_blocks(d) * R8_BLOCK + R8_COLS - 1) / R8_COLS, tasks = windows * chunks;
   const int64_t per_xcd = (tasks + 7) / 8, blocks = (per_xcd + 3) / 4 * 8;
-  SAE_REQUIRE(blocks < (1LL << 31), SAE_ERR_UNSUPPORTED, "rows8_grad_rows: size too large");
+  // a grid's first axis counts less than 2^32 threads; every launch is checked before the first is made
+  const int64_t short_blocks = (F + 7) / 8, prepare_blocks = feat_blocks + (positions + 255) / 256;
+  const int64_t threads = need == 0 ? short_blocks * 512
+                                    : std::max(std::max(prepare_blocks, blocks) * 256, windows * (d <= 256 ? 128 : 512));
+  SAE_REQUIRE(threads < (1LL << 32), SAE_ERR_UNSUPPORTED, "rows8_grad_rows: %lld slots of %lld features are too many", (long long)n_slots,
+              (long long)F);
   if (need == 0) {
-    hipLaunchKernelGGL(rows8_grad_short_kernel, dim3((unsigned)((F + 7) / 8), (unsigned)chunks), dim3(512), 0, st, feat_ptr, feat_slot, slot_tok,
+    hipLaunchKernelGGL(rows8_grad_short_kernel, dim3((unsigned)short_blocks, (unsigned)chunks), dim3(512), 0, st, feat_ptr, feat_slot, slot_tok,
                        coef, rec, out, bias_out, F, d);
     return check_launch("rows8_grad_rows");
   }
-  hipLaunchKernelGGL(rows8_grad_prepare_kernel, dim3((unsigned)(feat_blocks + (positions + 255) / 256)), dim3(256), 0, st, feat_ptr, feat_slot,
+  hipLaunchKernelGGL(rows8_grad_prepare_kernel, dim3((unsigned)prepare_blocks), dim3(256), 0, st, feat_ptr, feat_slot,
                      slot_tok, coef, pos_feat, pos_tok, pos_coef, out, bias_out, F, d, (uint32_t)feat_blocks, length);
 #define SAE_R8_GRAD(W)                                                                                                              \
   hipLaunchKernelGGL(rows8_grad_window_kernel<W>, dim3((unsigned)blocks), dim3(256), 0, st, feat_ptr, pos_feat, pos_tok, pos_coef, rec, out, \

@@ -108,6 +108,25 @@ def test_entry_points_refuse_before_any_launch(pkg):
     assert lib.sae_sparse_grad_rows(P, P, P, P, P, 2, P, None, 4, 40, None) == -1      # records have their own entry point
 
 
+def test_launches_that_one_grid_cannot_hold_are_refused(pkg):
+    """A grid's first axis counts less than 2^32 threads: larger calls are refused before the first launch, not by the last."""
+    lib = pkg._lib.load()
+    P = 1 << 20
+
+    def rows(nr, F, d, n):
+        return lib.sae_rows8_grad_rows(P, P, P, P, P, nr, P, None, F, d, n, P, 1 << 62, None)
+
+    assert rows(100, (1 << 26) + 1, 1, 10) == -2                     # one launch, eight features a workgroup of 512
+    assert rows(4096, (1 << 26) + 1, 1, 10) == -2                    # the first of three, four features a workgroup of 256
+    assert rows(4096, (1 << 26) - 8, 1, 1 << 30) == -2               # features and positions together
+    assert rows(4096, 1000, 4096, (1 << 29) + 1) == -2               # the second: a wave per window and 256 columns
+    assert rows(4096, 1000, 260, (1 << 30) + 1) == -2                # the third: 512 threads per window
+    join = lambda count, s=2: lib.sae_join_slices(P, s, count, P, 0, None)   # noqa: E731
+    assert join((1 << 34) - 1023) == -2
+    ot = lambda m, n, s: lib.sae_gemm_over_tokens(P, 1, P, 1, 640, m, n, P, 0, s, P, None)   # noqa: E731
+    assert ot(1 << 20, 1 << 14, 2) == -2
+
+
 # ---- records made and read without a GPU; the pipeline that carries them -----------------------------------------------
 
 def exact_values(x):
