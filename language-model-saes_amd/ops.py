@@ -1547,16 +1547,20 @@ OVER_TOKENS_WIDTHS = (1 << 24, 65535 * 64)      # of left and right on 64 x 64 t
 @functools.lru_cache(maxsize=1024)
 def _over_tokens_slices(tokens: int, m: int, n: int, wide: bool) -> int:
     """Into how many slices of the tokens the product of 64 x 64 tiles is cut: the least estimated time.  A slab (64 tokens, 32
-    in fp32) takes a workgroup 0.47 us alone on its CU and 0.2 us more with each further one there (fp32: 0.9 and 0.35); joining
-    costs a launch of 4 us, 0.3 us per slice and 8 bytes per output and slice at 4 TB/s.  Measured in 1 / 2 / 4 / 8 slices:
-    4096 x 1024 x 768 (192 tiles) 33 / 27 / 24 / 28 us; 8192 x 2048 x 512 (256) 64 / 45 / 44 / 48; 8192 x 64 x 64 (one) 60 / 29 /
-    18 / 13; 1000 x 1003 x 521 (144) 12 / 15 / 18 / 23; 2048 x 2048 x 768 (384) 24 / 27 / 30 / 38; fp32 4096 x 1024 x 768 112 / 82 /
-    62 / 63."""
+    in fp32) takes a workgroup 0.47 us alone on its CU and 0.2 us more with each further one there (fp32: 0.9 and 0.35), up to the
+    four that a CU holds (by LDS in fp32, by registers otherwise): those beyond wait for a place and gain nothing.  Joining
+    costs a launch of 4 us, 0.3 us per slice and 8 bytes per output and slice at 4 TB/s.  Measured in 1 / 2 / 4 / 8 slices, us:
+    4096 x 1024 x 768 (192 tiles) 30 / 26 / 23 / 28; 8192 x 2048 x 512 (256) 60 / 43 / 43 / 48; 8192 x 64 x 64 (one) 47 / 28 /
+    17 / 13; 1000 x 1003 x 521 (144) 10 / 14 / 17 / 23; 2048 x 2048 x 768 (384) 20 / 25 / 29 / 38; 6000 x 1600 x 1600 (625) 81 / 86 / 90 /
+    99; fp32 4096 x 1024 x 768 97 / 79 / 60 / 62; fp32 65536 x 1024 x 1024 (256) 1607 / 1174 / 1079 / 1060; with the card full in one
+    piece, fp32 4096 x 2048 x 2048 (1024) 269 / 276 / 280 / 293, 32768 x 2048 x 2048 2119 / 2092 / 2067 / 2069 and 8192 x 4096 x 2048 (2048)
+    1045 / 1051 / 1058 / 1090."""
     slabs, tiles = -(-tokens // (32 if wide else 64)), -(-m // 64) * -(-n // 64)
     alone, more = (0.55, 0.35) if wide else (0.27, 0.2)
 
     def slab_us(s):
-        return alone + more * -(-tiles * s // 256)
+        on_a_cu = -(-tiles * s // 256)
+        return alone * -(-on_a_cu // 4) + more * on_a_cu
 
     best, best_us = 1, slabs * slab_us(1)
     for s in (2, 4, 8, 16, 32):

@@ -22,6 +22,13 @@ def test_a_slice_holds_a_slab(pkg, tokens, m, n, wide):
     assert 1 <= s <= -(-tokens // (32 if wide else 64))
 
 
+@pytest.mark.parametrize("tokens,m,n", [(32768, 2048, 2048), (131072, 32768, 2048), (8192, 4096, 2048), (16384, 4096, 4096), (65536, 8192, 8192)])
+@pytest.mark.parametrize("wide", [False, True])
+def test_a_full_card_is_not_cut(pkg, tokens, m, n, wide):
+    """Whole rounds of the four workgroups that each of 256 CUs holds: slices would take partial results and save nothing."""
+    assert -(-m // 64) * -(-n // 64) % 1024 == 0 and pkg.ops._over_tokens_slices(tokens, m, n, wide) == 1
+
+
 def test_rows8_holds_whole_records(pkg):
     R = pkg.Rows8
     ok = R(torch.zeros(3, 80, dtype=torch.uint8), 40)
