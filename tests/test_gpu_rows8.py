@@ -499,6 +499,48 @@ def test_adam_and_norm_over_8_bit_rows(pkg, dev, d, lowp):
         assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("lowp", [False, True])
+@pytest.mark.parametrize("T,d", [(517, 64), (700, 768), (1030, 1028), (603, 2052)])
+def test_adam_and_norm_over_long_segments_of_8_bit_rows(pkg, dev, T, d, lowp):
+    """Features that nearly all tokens keep: segments of more than two chunks of looked-up slots (192 or 256 each), and ragged ends.
+    The same bits as over the bf16 rows; the gradient's square sum and the bias gradient against 64-bit sums."""
+    ops = pkg.ops
+    F, k = 24, 6
+    q = ops.quantize_rows(activations(T, d, 31))
+    floats = ops.restore_rows(q)
+    code = sparse_code(ops, T, F, k, 32, dev, True)
+    fi = ops.build_feature_index(code)
+    longest = int((fi.feat_ptr[1:] - fi.feat_ptr[:-1]).max())
+    assert longest > 512 and longest % 8
+    dt = torch.bfloat16 if lowp else torch.float32
+    results = []
+    for dense in (q, floats):
+        g = torch.Generator(device=dev).manual_seed(33)
+        p = torch.randn(F, d, generator=g, device=dev).to(dt)
+        m, v = torch.zeros_like(p), torch.zeros_like(p)
+        bias, norm = torch.empty(F, device=dev), torch.empty(F, device=dev)
+        acc = torch.zeros(2, dtype=torch.float64, device=dev)
+        ops.adam_step_sparse_rows(fi, code.val, dense, p, m, v, lr=1e-3, beta1=0.9, beta2=0.99, eps=1e-8, step=3, bias_grad_out=bias,
+                                  row_norm_out=norm, grad_sq_nnz_acc=acc)
+        sums, bias2 = torch.zeros(2, dtype=torch.float64, device=dev), torch.empty(F, device=dev)
+        ops.sparse_rows_grad_sq_nnz(fi, code.val, dense, sums, bias_grad_out=bias2)
+        results.append((p, m, v, bias, norm, acc, sums, bias2))
+    for a, b in zip(*results):
+        assert torch.equal(a, b)
+    coef = torch.zeros(F, T, dtype=torch.float64, device=dev)
+    tok = fi.slot_tok.long()
+    coef.index_put_((code.idx.long(), tok), code.val.double(), accumulate=True)
+    grad, size = coef @ floats.double(), coef.abs() @ floats.double().abs()
+    _, _, _, bias, _, acc, sums, bias2 = results[0]
+    # an entry: one rounding of each of at most `longest` additions; where the state is bf16 the Adam pass rounds the sum to bf16
+    off = 1.01 * longest * 2.0**-24 * size
+    low = off + (2.0**-8 * (grad.abs() + off) if lowp else 0.0)
+    for total, e in ((acc[0], low), (sums[0], off)):       # squares added by fours in fp32, those in 64 bits
+        assert (total - grad.square().sum()).abs() <= (2 * grad.abs() * e + e * e).sum() + 4 * 2.0**-24 * (grad.abs() + e).square().sum()
+    b_sum, b_off = coef.sum(1), 1.01 * longest * 2.0**-24 * coef.abs().sum(1)
+    assert ((bias.double() - b_sum).abs() <= b_off).all() and ((bias2.double() - b_sum).abs() <= b_off).all()
+
+
 def test_blocks_that_are_not_finite_stay_in_their_rows(pkg, dev):
     ops = pkg.ops
     x = activations(6, 96, 18)
