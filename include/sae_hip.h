@@ -534,11 +534,12 @@ int sae_gemm_over_tokens(const void *left, int left_dtype, const void *right, in
 int sae_join_slices(const float *partials, int64_t n_slices, int64_t count, void *out, int out_dtype, void *stream);
 
 /* sae_sparse_grad_rows for a dense operand held as records (any d): out[f, :] = sum over the slots s of feature f of
- * coef[s] * values of record slot_tok[s]; rows without slots are written as zeros; bias_out (nullable) [F].  n_slots: the
- * length of feat_slot (positions feat_ptr[0] .. feat_ptr[F] of it are in use: the index may be a stretch of a longer one's
- * features).  A feature's slots are added in ascending order, as
- * sae_sparse_grad_rows adds them; where they cross a multiple of 32, 64 or 128 (by n_slots and d) in feat_slot the pieces are summed apart and
- * then joined in a fixed order, so a feature that many tokens keep costs no more time than as many slots of rare ones (of
+ * coef[s] * values of record slot_tok[s]; rows without slots are written as zeros; bias_out (nullable) [F].  n_slots: at least
+ * the number of positions of feat_slot in use, feat_ptr[F] - feat_ptr[0] (the index may be a stretch of a longer one's features);
+ * work and workspace go by it.  Where more are in use the rows and sums are NaN, unless one launch does it all (workspace 0), which
+ * needs no bound.  A feature's slots are added in ascending order, as
+ * sae_sparse_grad_rows adds them; where they cross a multiple of 32, 64 or 128 (by n_slots and d), counted from feat_ptr[0], the
+ * pieces are summed apart and then joined in a fixed order, so a feature that many tokens keep costs no more time than as many slots of rare ones (of
  * few slots, in one launch: a feature's up to 32 one after the other, more in eighths).  slot_tok's values are below n_rows.
  * workspace: sae_rows8_grad_rows_workspace_bytes(n_rows, n_slots, F, d) bytes (0: may be NULL), 16-byte aligned, as is out where d is a multiple of
  * 4. */

@@ -117,6 +117,7 @@ class _FusedCLTStep(torch.autograd.Function):
             stacked = ops.select_topk_row(pre_all.view(L * B, F), b_enc, None if norms is None else norms.contiguous(),
                                           min(k, F), granule_max=gmax.view(L * B, -1), rows_per_group=B)
             cat, layer_cnt = ops.merge_layer_codes(stacked, L)
+            layer_slots = stacked.n_slots // L
             pres = list(pre_all.unbind(0))
         elif act in ("topk", "batchtopk"):
             pres = [ops.encoder_gemm(x_op[l], w_enc_op[l], out_dtype) for l in range(L)]
@@ -124,6 +125,7 @@ class _FusedCLTStep(torch.autograd.Function):
                   (lambda p, b, s: ops.select_topk_batch(p, b, s, k * B))
             codes = [sel(pres[l], b_enc[l], None if norms is None else norms[l]) for l in range(L)]
             cat, layer_cnt = merge_layer_codes(codes)
+            layer_slots = max(c.n_slots for c in codes)
         else:
             pres = [ops.encoder_gemm(x_op[l], w_enc_op[l], out_dtype) for l in range(L)]
             pre_cat = torch.stack(pres, dim=1).view(B, L * F) if act == "layertopk" else None
@@ -137,6 +139,8 @@ class _FusedCLTStep(torch.autograd.Function):
                 cat = ops.select_topk_batch(torch.stack(pres, dim=2).view(B, F * L), tr(b_enc), tr(norms), k * B)
                 cat = relabel_feature_major_code(cat, L, F)
             layer_cnt = layer_counts(cat, L, F)
+            layer_slots = cat.n_slots
+        ctx.layer_slots = layer_slots                                     # entries of one layer at most
         prefix = torch.cumsum(layer_cnt, dim=1).to(torch.int32)           # entries of layers <= j, per token
         tok_w = torch.full((B,), 1.0 / (L * B), dtype=torch.float32, device=x.device)
         w_dec_ops = m._w_dec_operands(amp)
@@ -194,7 +198,7 @@ class _FusedCLTStep(torch.autograd.Function):
                 continue
             rows, _ = ops.sparse_grad_rows(fi_j, coef_dec, ctx.grads[j], (j + 1) * F)
             dW_D.append(rows.view(j + 1, F, d))
-            rows_e, bias_e = ops.sparse_grad_rows(fi_l, coef_enc, ctx.x_rows[j], F, want_bias=True)
+            rows_e, bias_e = ops.sparse_grad_rows(fi_l, coef_enc, ctx.x_rows[j], F, want_bias=True, max_slots=ctx.layer_slots)
             dW_E.append(rows_e); db_E.append(bias_e)
         if defer:
             m.W_E._sparse_grad = SparseRowGradPieces(enc_pieces, L * F, bias_param=m.b_E)

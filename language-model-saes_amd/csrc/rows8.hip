@@ -332,25 +332,33 @@ static int r8_window(int64_t n_slots, int64_t d) {
   return tasks < 1024 ? 32 : tasks < 8192 ? 64 : 128;
 }
 
+// Positions in use, counted from the first feature's: the index may be a stretch of a longer one's features.  0 where they are
+// more than the host was told: the launches behind the first then find nothing to do.
+__device__ __forceinline__ int r8_used(const int32_t *__restrict__ feat_ptr, int64_t F, int n_slots) {
+  const int used = feat_ptr[F] - feat_ptr[0];
+  return used <= n_slots ? used : 0;
+}
+
 // The first launch.  Workgroups below feat_blocks, a wave per feature: the feature of each of its positions, a zero row where
 // it has none, its coefficients' sum.  The others, a thread per position: token and coefficient in index order, so that the
 // waves of the second launch, one per window and chunk of columns, read them in line (by slot they would touch a cache line
-// per entry, once for every chunk).  Positions in front of the first feature's and behind the last's, up to a whole window, get
-// feature -1.
+// per entry, once for every chunk).  Positions behind the last feature's, up to a whole window, get feature -1.  More positions in
+// use than the host was told: rows and sums of NaN.
 __global__ __launch_bounds__(256) void rows8_grad_prepare_kernel(const int32_t *__restrict__ feat_ptr, const int32_t *__restrict__ feat_slot,
                                                                  const int32_t *__restrict__ slot_tok, const float *__restrict__ coef,
                                                                  int32_t *__restrict__ pos_feat, int32_t *__restrict__ pos_tok,
                                                                  float *__restrict__ pos_coef, float *__restrict__ out,
                                                                  float *__restrict__ bias_out, int64_t F, int64_t d, uint32_t feat_blocks,
-                                                                 int window) {
+                                                                 int window, int n_slots) {
+  const int first = feat_ptr[0];
   if (blockIdx.x >= feat_blocks) {
     const int64_t i = (int64_t)(blockIdx.x - feat_blocks) * 256 + threadIdx.x;
-    const int first = feat_ptr[0], total = feat_ptr[F];   // the index may be a stretch of a longer one's features
-    if (i >= first && i < total) {
-      const int slot = feat_slot[i];
+    const int total = r8_used(feat_ptr, F, n_slots);
+    if (i < total) {
+      const int slot = feat_slot[first + i];
       pos_tok[i] = slot_tok[slot];
       pos_coef[i] = coef[slot];
-    } else if (i < first || i < ((int64_t)total + window - 1) / window * window) {
+    } else if (i < ((int64_t)total + window - 1) / window * window) {
       pos_feat[i] = -1;
       pos_tok[i] = 0;
       pos_coef[i] = 0.f;
@@ -361,20 +369,23 @@ __global__ __launch_bounds__(256) void rows8_grad_prepare_kernel(const int32_t *
   const int lane = threadIdx.x & 63;
   if (f >= F) return;
   const int lo = feat_ptr[f], hi = feat_ptr[f + 1];
-  for (int i = lo + lane; i < hi; i += 64) pos_feat[i] = (int32_t)f;
+  const bool fits = feat_ptr[F] - first <= n_slots;
+  const float empty = fits ? 0.f : __uint_as_float(0x7fc00000u);
+  if (fits)
+    for (int i = lo + lane; i < hi; i += 64) pos_feat[i - first] = (int32_t)f;
   if (bias_out) {
-    float s = 0.f;
+    float s = empty;
 #pragma unroll 4
     for (int i = lo + lane; i < hi; i += 64) s += coef[feat_slot[i]];
     s = wave_sum(s);
     if (lane == 0) bias_out[f] = s;
   }
-  if (lo < hi) return;
+  if (lo < hi && fits) return;
   float *row = out + f * d;
   if ((d & 3) == 0) {
-    for (int64_t j = lane; j < (d >> 2); j += 64) store_stream(row, j, make_float4(0.f, 0.f, 0.f, 0.f));
+    for (int64_t j = lane; j < (d >> 2); j += 64) store_stream(row, j, make_float4(empty, empty, empty, empty));
   } else {
-    for (int64_t j = lane; j < d; j += 64) row[j] = 0.f;
+    for (int64_t j = lane; j < d; j += 64) row[j] = empty;
   }
 }
 
@@ -385,7 +396,7 @@ __global__ __launch_bounds__(256) void rows8_grad_window_kernel(const int32_t *_
                                                                 const int32_t *__restrict__ pos_tok, const float *__restrict__ pos_coef,
                                                                 const uint8_t *__restrict__ rows, float *__restrict__ out,
                                                                 float *__restrict__ part, int64_t F, int64_t d, int64_t n_windows,
-                                                                int64_t n_tasks) {
+                                                                int64_t n_tasks, int n_slots) {
   constexpr int G = 16;   // records requested together
   const int lane = threadIdx.x & 63;
   // tasks in chunk-major order, one contiguous eighth per XCD (workgroups go round the XCDs): what an XCD reads at a time
@@ -395,9 +406,9 @@ __global__ __launch_bounds__(256) void rows8_grad_window_kernel(const int32_t *_
   const int64_t task = (int64_t)(blockIdx.x & 7) * per_xcd + local;
   if (local >= per_xcd || task >= n_tasks) return;
   const int64_t chunk = task / n_windows, window = task % n_windows;
-  const int total = feat_ptr[F];
+  const int total = r8_used(feat_ptr, F, n_slots);
   const int w0 = (int)(window * WINDOW), w1 = w0 + WINDOW;
-  if (w0 >= total || w1 <= feat_ptr[0]) return;
+  if (w0 >= total) return;
   const int64_t codes = r8_blocks(d) * R8_BLOCK;
   const uint32_t pitch = (uint32_t)r8_pitch(d);
   const int64_t col = chunk * R8_COLS + lane * 4;
@@ -468,13 +479,13 @@ __global__ __launch_bounds__(256) void rows8_grad_window_kernel(const int32_t *_
 template <int LANES>
 __global__ __launch_bounds__(2 * LANES) void rows8_grad_join_kernel(const int32_t *__restrict__ feat_ptr, const int32_t *__restrict__ pos_feat,
                                                               const float *__restrict__ part, float *__restrict__ out, int64_t F, int64_t d,
-                                                             int length) {
+                                                             int length, int n_slots) {
   const int64_t window = blockIdx.x;
-  const int total = feat_ptr[F];
+  const int total = r8_used(feat_ptr, F, n_slots);
   const int64_t w0 = window * length, w1 = w0 + length;
   const int f = pos_feat[w1 < (int64_t)gridDim.x * length ? w1 : w0], inside = pos_feat[w1 - 1], before = pos_feat[w0 > 0 ? w0 - 1 : 0];
   if (w1 >= total || f < 0 || inside != f || (w0 > 0 && before == f)) return;
-  const int64_t last = (feat_ptr[f + 1] - 1) / length, codes = r8_blocks(d) * R8_BLOCK;
+  const int64_t last = (feat_ptr[f + 1] - feat_ptr[0] - 1) / length, codes = r8_blocks(d) * R8_BLOCK;
   __shared__ float4 sums[LANES];
   const int half = threadIdx.x / LANES, at = threadIdx.x % LANES;
   const int64_t j = ((int64_t)blockIdx.y * LANES + at) * 4;
@@ -727,18 +738,19 @@ extern "C" int sae_rows8_grad_rows(const int32_t *feat_ptr, const int32_t *feat_
     return check_launch("rows8_grad_rows");
   }
   hipLaunchKernelGGL(rows8_grad_prepare_kernel, dim3((unsigned)prepare_blocks), dim3(256), 0, st, feat_ptr, feat_slot,
-                     slot_tok, coef, pos_feat, pos_tok, pos_coef, out, bias_out, F, d, (uint32_t)feat_blocks, length);
+                     slot_tok, coef, pos_feat, pos_tok, pos_coef, out, bias_out, F, d, (uint32_t)feat_blocks, length, (int)n_slots);
 #define SAE_R8_GRAD(W)                                                                                                              \
   hipLaunchKernelGGL(rows8_grad_window_kernel<W>, dim3((unsigned)blocks), dim3(256), 0, st, feat_ptr, pos_feat, pos_tok, pos_coef, rec, out, \
-                     part, F, d, windows, tasks)
+                     part, F, d, windows, tasks, (int)n_slots)
   if (length == 32) SAE_R8_GRAD(32);
   else if (length == 64) SAE_R8_GRAD(64);
   else SAE_R8_GRAD(128);
 #undef SAE_R8_GRAD
   if (d <= 256)
-    hipLaunchKernelGGL(rows8_grad_join_kernel<64>, dim3((unsigned)windows), dim3(128), 0, st, feat_ptr, pos_feat, part, out, F, d, length);
+    hipLaunchKernelGGL(rows8_grad_join_kernel<64>, dim3((unsigned)windows), dim3(128), 0, st, feat_ptr, pos_feat, part, out, F, d, length,
+                       (int)n_slots);
   else
     hipLaunchKernelGGL(rows8_grad_join_kernel<256>, dim3((unsigned)windows, (unsigned)((d + 1023) / 1024)), dim3(512), 0, st, feat_ptr, pos_feat,
-                       part, out, F, d, length);
+                       part, out, F, d, length, (int)n_slots);
   return check_launch("rows8_grad_rows");
 }

@@ -564,6 +564,72 @@ def test_a_stretch_of_an_index(pkg, dev, T):
         assert close(rows, whole[lo:hi], size[lo:hi], T, False) and torch.equal(b, bias[lo:hi]) and (frame[0] == 7).all() and (frame[-1] == 7).all()
 
 
+@pytest.mark.parametrize("T,F,k,d", [(1100, 90, 9, 132), (2000, 300, 24, 40), (1500, 64, 40, 1030), (60, 90, 9, 132)])
+def test_a_stretch_whose_slots_are_counted(pkg, dev, T, F, k, d):
+    """With its largest number of slots said, a stretch gives the bits of the index that begins with it; with too few said the
+    rows are NaN (right, where one launch does it all), and nothing beside them is touched."""
+    ops = pkg.ops
+    g = torch.Generator(device=dev).manual_seed(5)
+    score = torch.rand(T, F, generator=g, device=dev)
+    score[:, F // 2] = 2.0                                                     # a feature of every token
+    idx = score.topk(k, 1).indices.sort(1).values.to(torch.int32).reshape(-1).contiguous()
+    val = torch.randn(T * k, generator=g, device=dev)
+    code = ops.SparseCode(idx, val, torch.arange(T, device=dev) * k, torch.full((T,), k, dtype=torch.int32, device=dev), T, F)
+    fi = ops.build_feature_index(code)
+    ptr = fi.feat_ptr.tolist()
+    q = ops.quantize_rows(torch.randn(T, d, generator=g, device=dev))
+    lib = pkg._lib.load()
+    for lo, hi in ((0, F), (0, F // 3), (F // 3, F - 2), (F // 2, F // 2 + 1), (F - 1, F)):
+        used, n = ptr[hi] - ptr[lo], hi - lo
+        part = ops.FeatureIndex(fi.feat_ptr[lo : hi + 1], fi.feat_slot, fi.slot_tok)
+        front = ops.FeatureIndex(part.feat_ptr - ptr[lo], torch.roll(fi.feat_slot, -ptr[lo]), fi.slot_tok)
+        for said in (used, used + 1, used + 777, 10**9):
+            frame = torch.full((n + 2, d), 7.0, device=dev)
+            rows, b = ops.sparse_grad_rows(part, val, q, n, want_bias=True, out=frame[1:-1], max_slots=said)
+            want, b0 = ops.sparse_grad_rows(front, val, q, n, want_bias=True, max_slots=said)
+            assert torch.equal(rows, want) and torch.equal(b, b0) and (frame[0] == 7).all() and (frame[-1] == 7).all()
+        frame = torch.full((n + 2, d), 7.0, device=dev)
+        rows, b = ops.sparse_grad_rows(part, val, q, n, want_bias=True, out=frame[1:-1], max_slots=used - 1)
+        if lib.sae_rows8_grad_rows_workspace_bytes(T, used - 1, n, d):
+            assert rows.isnan().all() and b.isnan().all()
+        else:
+            assert torch.isfinite(rows).all() and torch.equal(b, b0)
+        assert (frame[0] == 7).all() and (frame[-1] == 7).all()
+    with pytest.raises(ValueError):
+        ops.sparse_grad_rows(fi, val, q, F, max_slots=-1)
+
+
+@pytest.mark.parametrize("act_fn", ["topk", "batchtopk", "layertopk"])
+@pytest.mark.parametrize("granule", [True, False])
+def test_a_layer_pays_for_its_own_slots(pkg, dev, monkeypatch, act_fn, granule):
+    """The cross-layer transcoder says how many slots a layer has at most: all there are in it, and no more than one layer's share
+    where every layer selects by itself."""
+    L, d, F, k, B = 4, 64, 256, 6, 1200
+    hin, hout = [f"i{l}" for l in range(L)], [f"o{l}" for l in range(L)]
+    clt = pkg.CrossLayerTranscoder(pkg.CLTConfig(hook_points_in=hin, hook_points_out=hout, d_model=d, expansion_factor=F / d, act_fn=act_fn,
+                                                 top_k=k, norm_activation="inference", device="cuda", dtype=torch.float32))
+    clt.granule_select = granule
+    g = torch.Generator(device=dev).manual_seed(2)
+    with torch.no_grad():
+        for p in clt.parameters():
+            p.copy_(torch.randn(p.shape, generator=g, device=dev) * 0.1)
+    x = held(pkg, torch.randn(B, L, d, generator=g, device=dev))
+    batch = {h: x[:, l].contiguous() for l, h in enumerate(hin)} | {h: torch.randn(B, d, generator=g, device=dev) for h in hout}
+    batch["tokens"] = torch.zeros(B, device=dev)
+    said, plain = [], pkg.ops.sparse_grad_rows
+
+    def sparse_grad_rows(fi, coef, rows, F, *a, **kw):
+        if isinstance(rows, pkg.Rows8):
+            said.append((int(fi.feat_ptr[-1] - fi.feat_ptr[0]), kw["max_slots"]))
+        return plain(fi, coef, rows, F, *a, **kw)
+
+    monkeypatch.setattr(pkg.ops, "sparse_grad_rows", sparse_grad_rows)
+    _, got = run(clt, batch, True, True)
+    assert len(said) == L and all(used <= most for used, most in said) and all(torch.isfinite(v).all() for v in got.values())
+    if act_fn != "layertopk":
+        assert all(most <= B * k for _, most in said)
+
+
 def make_variant(pkg, dev, kind):
     """A small crosscoder, cross-layer transcoder or Lorsa, and a batch of it."""
     n, d, F, B = 2, 64, 256, 128
