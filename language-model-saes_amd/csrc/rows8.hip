@@ -324,12 +324,12 @@ constexpr int R8_COLS = 256;   // columns of a chunk: four per lane (eight per l
                                // stores)
 
 // Positions per window.  Long windows leave fewer partial rows, short ones more waves: with few waves per CU a window's
-// records, read one group after the other, are what takes the time.  us at 32 / 64 / 128 positions: 33 / 29 / 31 at 4096
-// tokens, k = 32, d = 768 (1024 windows of 128 in three chunks), 192 / 159 / 145 at 8192, 64, 2048 (4096 in eight), 15 / 17 / 23 at
-// 1000, 32, 512 (250 in two), 27 / 26 / 30 at 8192, 8, 700 (512 in three), 53 / 46 / 44 at 8192, 32, 768 (2048 in three).
+// records, read one group after the other, are what takes the time.  us at 32 / 64 / 128 positions, by windows of 128 times
+// chunks: 550 (1100 tokens, k = 32, d = 512) 16 / 18 / 24; 1536 (2048, 32, 768) 23 / 22 / 28; 3072 (4096, 32, 768) 33 / 29 / 31; 4096 (4096, 32,
+// 1024) 37 / 34 / 34; 6144 (8192, 32, 768) 53 / 46 / 45; 8192 (16384, 32, 512) 89 / 74 / 69; 32768 (8192, 64, 2048) 192 / 158 / 146.
 static int r8_window(int64_t n_slots, int64_t d) {
   const int64_t tasks = (n_slots + 127) / 128 * ((d + R8_COLS - 1) / R8_COLS);
-  return tasks < 1024 ? 32 : tasks < 8192 ? 64 : 128;
+  return tasks < 1024 ? 32 : tasks < 4096 ? 64 : 128;
 }
 
 // Positions in use, counted from the first feature's: the index may be a stretch of a longer one's features.  0 where they are

@@ -134,6 +134,15 @@ def test_launches_that_one_grid_cannot_hold_are_refused(pkg):
     assert ot(1 << 20, 1 << 14, 2) == -2
 
 
+@pytest.mark.parametrize("T,k,d,length", [(1100, 32, 512, 32), (2048, 32, 768, 64), (4096, 32, 768, 64), (4096, 64, 768, 128), (8192, 32, 768, 128),
+                                          (8192, 64, 2048, 128)])
+def test_windows_are_those_measured_best(pkg, T, k, d, length):
+    """Seen by the workspace: feature, token and coefficient of every position, two partial rows per window."""
+    windows = -(-T * k // length)
+    want = windows * (length * 12 + 2 * -(-d // 32) * 32 * 4)
+    assert pkg._lib.load().sae_rows8_grad_rows_workspace_bytes(T, T * k, 8192, d) == want
+
+
 # ---- records made and read without a GPU; the pipeline that carries them -----------------------------------------------
 
 def exact_values(x):
