@@ -7,7 +7,8 @@
 // those, a slice of the tokens: slices are joined in order by a second launch); operands are read as they lie, any width, any
 // token count, records widened to bf16 (exactly) on their way into LDS.  A slab is multiplied while the next is written to LDS
 // and two more are on their way in registers; nothing tests or moves what is still on its way, or the loads would be waited
-// for at once (1000 x 1003 x 521 uncut 27 us then, 12 now; 4096 x 4096 x 768 70 and 55; fp32 4096 x 2048 x 2048 334 and 274).
+// for at once (1000 x 1003 x 521 uncut 27 us then, 11 now; 4096 x 4096 x 768 70 and 59; fp32 4096 x 2048 x 2048 334 and 268).
+// A small product is a chain: 1000 x 1003 x 521 is 3.9 us of start, first slab and store and 15 slabs of 0.46 us behind it.
 //
 // bf16 and 8-bit operands: slabs of 64 tokens, v_mfma_f32_16x16x32_bf16, whose fragments (8 consecutive tokens of one column)
 // are read across the token rows with ds_read_b64_tr_b16 (see encoder_gemm.hip).  With an fp32 operand: slabs of 32 tokens as

@@ -317,9 +317,10 @@ __global__ __launch_bounds__(256) void transpose_padded_kernel(const void *__res
 // Some features are kept by most tokens and most by few, so work is cut by position in feat_slot, not by feature: a wave
 // owns a window of positions and 256 columns.  A segment that lies inside a window goes straight to its row; one that crosses
 // leaves one partial row per window, joined in a fixed order by a third launch.
-// (8192 tokens, 64 of 32768 features, d = 2048: 147 us; a workgroup per feature takes 33 ms there, the most frequent feature's
-// 8000 records one after the other.  292 MB have to move, 42 us at the rate of a large fill; the second launch's vector
-// instructions alone are 94 us of its 122: 13 per record and four columns.)
+// (8192 tokens, 64 of 32768 features, d = 2048: 147 us; a workgroup per feature, as the first form here, took 33 ms there, the
+// most frequent feature's 8192 records one after the other.  292 MB have to move, 42 us at the rate of a large fill.  The second
+// launch is 121-132 us, 252 to 279 thousand cycles: its vector units issue for 225 thousand of them (13 instructions per record and
+// four columns), the address units of its vector loads, two per record and chunk, are busy for 190.)
 constexpr int R8_COLS = 256;   // columns of a chunk: four per lane (eight per lane: 196 us instead of 184, before the streaming
                                // stores)
 

@@ -1587,10 +1587,11 @@ def gemm_over_tokens(left, right, out_dtype: torch.dtype = torch.float32) -> tor
     ones on the GEMM kernel's 256 x 256 tiles, for which rows held in 8 bits (and operands that its slabs do not divide) are
     first copied into a transposed bf16 operand: their steps change along the contraction, so codes cannot enter the matrix
     cores as they are, and widening them inside that product's tiles would be done again for every tile of the other side.
-    Measured, us on 64 x 64 tiles against us with copies: 1000 x 1003 x 521 12 / 46, 4096 x 4096 x 768 59 / 80,
-    4096 x 2048 x 2048 75 / 86, 8192 x 4096 x 768 117 / 90, 8192 x 2048 x 2048 138 / 105; with many outputs for their tokens
-    1024 x 4096 x 2048 43 / 46, 512 x 8192 x 2048 49 / 42, 64 x 8192 x 2048 22 / 30; fp32 4096 x 2048 x 2048 282 us (122
-    TFLOP/s)."""
+    Measured, us on 64 x 64 tiles against us with copies: 1000 x 1003 x 521 11 / 46, 4096 x 4096 x 768 59 / 79,
+    4096 x 2048 x 2048 73 / 83, 8192 x 4096 x 768 106 / 88, 8192 x 2048 x 2048 134 / 103; with many outputs for their tokens
+    1024 x 4096 x 2048 40 / 46, 512 x 8192 x 2048 50 / 42, 64 x 8192 x 2048 21 / 30; fp32 4096 x 2048 x 2048 268 us (128
+    TFLOP/s).  The copies are [columns, tokens] in bf16: of wide records (a dense dictionary's activations) twice their bytes for
+    the length of the product."""
     for name, t in (("left", left), ("right", right)):
         if isinstance(t, Rows8):
             _req_rows8(t, name)

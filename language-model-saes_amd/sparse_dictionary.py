@@ -73,7 +73,11 @@ class LazyDict(dict):
 
 class SparseDictionary(nn.Module):
     # True: what the backward pass of a step reads of its inputs, and of dense activations, is held in 8 bits between the
-    # two passes (`ops.Rows8`): half the bytes of bf16 rows, a quarter of fp32 ones.  The forward pass is unchanged; of the
+    # two passes (`ops.Rows8`): half the bytes of bf16 rows, a quarter of fp32 ones.  It lowers what a graph holds while it waits
+    # for its backward pass (several losses before one backward, work of other models between the passes), not the largest
+    # need of one step by itself: records are written beside the rows they are made of, and wide ones are copied to bf16 where
+    # the backward pass multiplies them (dense JumpReLU 2048 x 32768, 8192 tokens: 1120 -> 857 MiB held, 1760 -> 2009 MiB at
+    # most).  The forward pass is unchanged; of the
     # gradients the encoder's weights change (and, where activations are dense, the decoder's), by the rounding of the rows
     # they are summed over.  Inputs that 8 bits hold exactly (a batch read from an 8-bit buffer without a scale) give the
     # same gradients, up to the order of the sums where dense gradients are written.  Taken by the kernel steps of
