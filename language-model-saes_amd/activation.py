@@ -448,7 +448,7 @@ class _RowStore:
                 return ops.gather_rows(ops.Rows8(d, self.width), idx_host.to(d.device), out_dtype=to, scale=scale)
             return rows8_unpack(d.index_select(0, idx_host.to(d.device)), self.width, to, scale)
         floaty = d.ndim == 2 and d.dtype in (torch.float32, torch.bfloat16)
-        if d.is_cuda and floaty:
+        if d.is_cuda and floaty and (out_dtype or d.dtype) in (torch.float32, torch.bfloat16):
             return ops.gather_rows(d, idx_host.to(d.device), out_dtype=out_dtype or d.dtype, scale=scale)
         out = d.index_select(0, idx_host.to(d.device))
         if floaty or d.is_floating_point():
@@ -552,9 +552,10 @@ def cached_activation_stream(cache_dir: str | Path, hook_points: Sequence[str], 
                              rows8: bool = False) -> Iterator[dict[str, torch.Tensor]]:
     """Loader -> mask filter -> batchler, the chain the reference's ActivationFactory builds for a cached
     source with a batch size (activation/factory.py:246-345): yields `{hook: [batch, d], tokens: [batch], ...}`.
-    With `rows8` files of 8-bit rows stay records up to the batch: half the bytes of bf16 over the bus and in the buffer."""
+    With `rows8` files of 8-bit rows stay records up to the batch: half the bytes of bf16 over the bus and in the buffer.
+    Without, the buffer holds the floats that the loader gives."""
     loader = CachedActivationLoader({hp: os.path.join(str(cache_dir), hp) for hp in hook_points}, device=device, dtype=dtype,
                                     keep_rows8=rows8)
     batchler = ActivationBatchler(batch_size, buffer_size, buffer_shuffle_config, override_dtype=override_dtype or (dtype if rows8 else None),
-                                  rows8=loader.rows8_widths)
+                                  rows8=loader.rows8_widths if rows8 else None)
     return batchler.process(ActivationTransformer().process(loader.process()))

@@ -769,3 +769,20 @@ def test_chunks_of_several_types_and_forms_on_the_gpu(pkg, dev, tmp_path):
         assert next(it)["h"].dtype == next(it)["h"].dtype == f32
         with pytest.raises(ValueError, match="float rows after"):
             next(it)
+
+
+def test_a_stream_of_floats_holds_floats_on_the_gpu(pkg, dev, tmp_path):
+    """Rows of a float file in front of 8-bit ones reach the batches as they are, however far ahead the reader is."""
+    for i, form in enumerate(("float", "rows8", "rows8")):
+        t = torch.arange(16)[None] + 100 * i
+        x = torch.randn(1, 16, 40, generator=torch.Generator().manual_seed(i))
+        pkg.ActivationWriter(pkg.ActivationWriterConfig(cache_dir=str(tmp_path), hook_points=["h"], row_format=form)).process(
+            [{"h": x, "tokens": t, "mask": torch.ones_like(t), "attention_mask": torch.ones_like(t)}], start_shard=i)
+    kw = dict(batch_size=8, buffer_size=24, buffer_shuffle_config=pkg.BufferShuffleConfig(perm_seed=7))
+    cpu, gpu = (list(pkg.cached_activation_stream(tmp_path, ["h"], device=d, **kw)) for d in ("cpu", "cuda"))
+    assert len(cpu) == len(gpu) == 6
+    for a, b in zip(cpu, gpu):
+        assert torch.equal(a["tokens"], b["tokens"].cpu()) and torch.equal(a["h"], b["h"].cpu())
+    x = torch.randn(1, 16, 40, generator=torch.Generator().manual_seed(0))[0]
+    rows = torch.cat([b["h"].cpu() for b in gpu])[torch.cat([b["tokens"].cpu() for b in gpu]).reshape(-1).argsort()]
+    assert torch.equal(rows[:16], x)

@@ -265,6 +265,35 @@ def test_stream_of_records_gives_the_rows_they_hold(pkg, tmp_path):
             assert torch.equal(b[hp].float(), a[hp]) and torch.equal(c[hp], a[hp]) and torch.equal(o[hp], a[hp].half())
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32, None])
+def test_a_stream_of_floats_holds_floats(pkg, tmp_path, dtype):
+    """Unless records are asked for, nothing rounds the loader's floats to 8 bits again: fp16 values past its largest stay
+    infinities by themselves, and rows of a float file in front of 8-bit ones stay what they are."""
+    want = torch.cat([w.reshape(-1, 40) for w in write_chunks(pkg, tmp_path, [(40, torch.float32, "float"), (40, torch.float32, "rows8")])])
+    want = want.to(dtype) if dtype is not None else want
+    got = list(pkg.cached_activation_stream(tmp_path, ["h0"], batch_size=5, buffer_size=10, device="cpu", dtype=dtype))
+    assert len(got) > 1 and all(b["h0"].dtype == want.dtype for b in got)
+    got = torch.cat([b["h0"] for b in got])
+    kept = torch.cat([c["mask"].reshape(-1) for c in pkg.CachedActivationLoader({"h0": tmp_path / "h0"}).process()]).bool()
+    assert not got.isnan().any() and torch.equal(got.sort(0).values, want[kept].sort(0).values)
+    if dtype == torch.float16:
+        assert int(got.isinf().sum()) == int(want[kept].isinf().sum())
+
+
+def test_a_float_stream_of_records_is_not_rounded_again(pkg, tmp_path):
+    """The same over 8-bit files alone: the floats of the records, cast."""
+    part = list(samples(2, 4, 40, torch.float32))
+    part[0]["h0"][0, 1, 3] = 1e5
+    pkg.ActivationWriter(pkg.ActivationWriterConfig(cache_dir=str(tmp_path), hook_points=["h0"], n_samples_per_chunk=2, row_format="rows8")
+                         ).process(part)
+    (chunk,) = pkg.CachedActivationLoader({"h0": tmp_path / "h0"}, dtype=torch.float16).process()
+    want = chunk["h0"].reshape(-1, 40)[chunk["mask"].reshape(-1).bool()]
+    assert int(want.isinf().sum()) == 1
+    got = torch.cat([b["h0"] for b in pkg.cached_activation_stream(tmp_path, ["h0"], batch_size=5, buffer_size=10, device="cpu",
+                                                                   dtype=torch.float16)])
+    assert not got.isnan().any() and torch.equal(got.sort(0).values, want.sort(0).values)
+
+
 def test_buffer_that_quantises_what_arrives(pkg):
     data = [{"x": rows(n, 45, n), "y": torch.arange(n)} for n in (7, 20, 3, 31)]
     kw = dict(buffer_size=24, buffer_shuffle_config=pkg.BufferShuffleConfig(perm_seed=1))
