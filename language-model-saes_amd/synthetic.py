@@ -4,7 +4,7 @@ Activation generator G(d, r, seed): x = 0.05 * N(0, 1)^{B x d} + z U^T with U in
 Q factor of a seeded Gaussian (orthonormal columns) and z ~ N(0, 4); rows rescaled to norm sqrt(d).
 Weights: W_E ~ U(-1/sqrt(d), 1/sqrt(d)) (the nn.Linear default bound), W_D = W_E^T with rows
 normalised to unit L2, b_E = 0, b_D = mean of x.  Everything is drawn on the CPU generator so that
-the CPU oracle and the GPU path see identical inputs.
+a CPU run and the GPU path see identical inputs.
 """
 
 from __future__ import annotations
